@@ -13,6 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import AiciError
+from .tch_cuda import _on_device, _raw_stream
 
 PAGED_DECODE = 1
 TABLES_FOR_ALL = 2
@@ -171,3 +172,73 @@ class BatchInfoBuilder:
         seq_ids = [e[0] for e in self.entries]
         self.entries = []
         return BatchInfo(buffer, lay, list(order), seq_ids, self.block_size, step_no)
+
+
+class StepTables:
+    """Index tensors of one step, built on the GPU by `step_tables` (fields as in BatchInfo)."""
+    __slots__ = ("seqlens_q", "positions", "slot_mapping", "logit_idxs", "context_lens", "free_count")
+
+    def __init__(self, seqlens_q, positions, slot_mapping, logit_idxs, context_lens, free_count):
+        self.seqlens_q = seqlens_q        # int32 [requests + 1]
+        self.positions = positions        # int64 [max_tokens], 0 behind the last token
+        self.slot_mapping = slot_mapping  # int32 [max_tokens], -1 behind the last token
+        self.logit_idxs = logit_idxs      # int32 [requests], -1 for a request without new tokens
+        self.context_lens = context_lens  # int32 [requests], new tokens included
+        self.free_count = free_count      # int32 [1]
+
+
+def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor,
+                free_blocks: torch.Tensor, free_count: torch.Tensor, num_blocks: int, max_tokens: int,
+                block_size: int = 16, out: Optional[StepTables] = None) -> StepTables:
+    """The index tensors of one step from request lengths on the GPU (aici_step_tables): what
+    BatchInfoBuilder.finish builds on the host from slot lists, without the host.
+
+    Request i has context_lens[i] tokens in the cache and query_lens[i] new ones; `block_tables`
+    [requests, max_blocks] names its blocks and is extended in place by the blocks that the new tokens
+    begin, taken from the end of `free_blocks[:free_count]`.  `max_tokens` is the size of the token
+    tensors (at least the number of new tokens; a captured step takes its largest).  With `out` the
+    tensors of an earlier result are written again; out.context_lens may be `context_lens` and
+    out.free_count may be `free_count`, which advances the state in place.  A step that does not fit
+    (lengths, tokens, free blocks) changes nothing and sets a status bit (see _lib.last_status).
+    Returns a StepTables."""
+    fn = "step_tables"
+    for t in (query_lens, context_lens, block_tables, free_blocks, free_count):
+        if not t.is_cuda:
+            raise AiciError("%s: tensor must be on a CUDA device (there is no CPU path)" % fn)
+        if t.device != query_lens.device:
+            raise AiciError("%s: tensors are on different devices" % fn)
+        if t.dtype != torch.int32:
+            raise AiciError("%s: lengths, tables and free list must be int32" % fn)
+    n = query_lens.numel()
+    if query_lens.dim() != 1 or context_lens.shape != query_lens.shape or free_blocks.dim() != 1 or \
+            free_count.numel() != 1 or not query_lens.is_contiguous() or not context_lens.is_contiguous() or \
+            not free_blocks.is_contiguous():
+        raise AiciError("%s: query_lens and context_lens must be contiguous [requests], free_blocks contiguous "
+                        "[blocks], free_count [1]" % fn)
+    if block_tables.dim() != 2 or block_tables.shape[0] != n or block_tables.stride(1) != 1:
+        raise AiciError("%s: block_tables must be [requests, max_blocks] with contiguous rows" % fn)
+    dev = query_lens.device
+    if out is None:
+        # one allocation; the token tensors first, for their alignment
+        T4 = (max_tokens + 3) // 4 * 4
+        buf = torch.empty(3 * T4 + 3 * n + 2, dtype=torch.int32, device=dev)
+        positions, slots, seqlens, logits, context, count, _ = buf.split_with_sizes(
+            (2 * T4, T4, n + 1, n, n, 1, 0))
+        positions = positions.view(torch.int64)
+        if T4 != max_tokens:
+            positions, slots = positions[:max_tokens], slots[:max_tokens]
+        out = StepTables(seqlens, positions, slots, logits, context, count)
+    else:
+        for t, count, dtype in ((out.seqlens_q, n + 1, torch.int32), (out.positions, max_tokens, torch.int64),
+                                (out.slot_mapping, max_tokens, torch.int32), (out.logit_idxs, n, torch.int32),
+                                (out.context_lens, n, torch.int32), (out.free_count, 1, torch.int32)):
+            if t.device != dev or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+                raise AiciError("%s: out does not match the call (device, types or sizes)" % fn)
+    with _on_device(dev):
+        _lib.check(fn, _lib.lib().aici_step_tables(
+            query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(),
+            free_count.data_ptr(), n, block_tables.shape[1], block_tables.stride(0), free_blocks.numel(),
+            num_blocks, block_size, max_tokens, out.seqlens_q.data_ptr(), out.positions.data_ptr(),
+            out.slot_mapping.data_ptr(), out.logit_idxs.data_ptr(), out.context_lens.data_ptr(),
+            out.free_count.data_ptr(), _raw_stream(dev)))
+    return out

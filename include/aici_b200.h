@@ -10,7 +10,8 @@
  *
  * Supported shapes: bf16 (AICI_DTYPE_BF16), head_size 128, block_size 16,
  * num_heads / num_kv_heads in {1, 2, 4, 8}.  Anything else returns an error string; there
- * is no fallback path.
+ * is no fallback path.  (The rotary and windowed operators near the end of this file also take f16
+ * and more shapes, each as its own comment says.)
  *
  * KV-cache layout (rllm-cuda/src/llm/paged/cache_engine.rs:81-108), x = 16 / sizeof(T) = 8:
  *   key_cache   [num_blocks, num_kv_heads, head_size / x, block_size, x]
@@ -45,7 +46,8 @@ enum {
   AICI_STATUS_BAD_BLOCK = 1,   /* a block-table entry was outside [0, num_blocks)        */
   AICI_STATUS_BAD_SLOT = 2,    /* a slot index was outside the cache                      */
   AICI_STATUS_WAIT_TIMEOUT = 4, /* a bounded wait on a shared-memory barrier gave up      */
-  AICI_STATUS_PEER_TIMEOUT = 8  /* a peer GPU did not reach a barrier within its bounded wait */
+  AICI_STATUS_PEER_TIMEOUT = 8, /* a peer GPU did not reach a barrier within its bounded wait */
+  AICI_STATUS_NO_BLOCKS = 16    /* aici_step_tables: the free list holds too few blocks for the step */
 };
 
 /* Library version string (static storage). */
@@ -422,6 +424,117 @@ char *aici_batch_info_build(const aici_batch_entry *entries, int num_entries, in
                             int block_size, int64_t max_model_len, void *staging,
                             size_t staging_bytes, void *device_dst, size_t device_bytes,
                             aici_batch_layout *layout, int32_t *entry_order, aici_stream_t stream);
+
+/* ---- step tables on the GPU -----------------------------------------------------------------
+ * The index tensors of one step from request lengths that live in device memory: the counterpart of
+ * aici_batch_info_build for a step that no host allocator takes part in (a captured decode loop).
+ * Request i has context_lens[i] tokens in the cache and brings query_lens[i] >= 0 new ones; row i of
+ * block_tables (rows block_table_stride entries apart) names its blocks.  Outputs:
+ *   seqlens_q     [num_requests + 1]  running sums of query_lens
+ *   positions     [max_tokens]        of the new tokens, request after request; 0 behind the last one
+ *   slot_mapping  [max_tokens]        block * 16 + position % 16; -1 (skipped by the cache writes)
+ *                                     behind the last token
+ *   logit_idxs    [num_requests]      index of each request's last new token, -1 without new tokens
+ *   context_lens_out [num_requests]   context_lens + query_lens
+ *   free_count_out   [1]              free_count less the blocks that the step took
+ * A position that is a multiple of 16 begins a new block: the k-th of the step, in token order, is
+ * free_blocks[free_count - 1 - k], and is entered in block_tables.  No other entry is touched.  A
+ * block that is only partly filled must belong to its request alone (aici_copy_blocks after a fork).
+ * context_lens_out may be context_lens and free_count_out may be free_count: the call then advances
+ * the state in place.
+ * The step happens whole or not at all.  If a length is negative or does not fit its row, or there are
+ * more than max_tokens new tokens (AICI_STATUS_BAD_BLOCK), or free_count is below what the step needs
+ * (AICI_STATUS_NO_BLOCKS), the status bit is set and the outputs are those of a step without new
+ * tokens; tables, lengths and count keep their values.  A block id outside [0, num_blocks) gives slot
+ * -1 and AICI_STATUS_BAD_BLOCK.  At most 16384 requests; positions and slot_mapping 16-byte aligned. */
+char *aici_step_tables(const int32_t *query_lens, const int32_t *context_lens, int32_t *block_tables,
+                       const int32_t *free_blocks, const int32_t *free_count, int num_requests,
+                       int max_blocks_per_seq, int64_t block_table_stride, int free_capacity,
+                       int64_t num_blocks, int block_size, int max_tokens, int32_t *seqlens_q,
+                       int64_t *positions, int32_t *slot_mapping, int32_t *logit_idxs,
+                       int32_t *context_lens_out, int32_t *free_count_out, aici_stream_t stream);
+
+/* ---- rotary positions -------------------------------------------------------------------------
+ * Table of cosines and sines [max_position, rot_dim] = [cos | sin] of AICI_DTYPE_F32, _BF16 or _F16:
+ * pair j turns by base^(-2 j / rot_dim) per position, scaled for contexts longer than the trained one:
+ *   AICI_ROPE_LINEAR  positions divided by factor
+ *   AICI_ROPE_NTK     base multiplied by factor^(rot_dim / (rot_dim - 2))
+ *   AICI_ROPE_YARN    pairs with fewer than one turn in original_context positions are slowed down by
+ *                     factor, those with more than 32 keep their speed, the ones between are mixed; cosine
+ *                     and sine are multiplied by 0.1 ln(factor) + 1
+ * Angles are computed in 64 bits.  rot_dim even, at most 256; factor >= 1. */
+enum { AICI_ROPE_NONE = 0, AICI_ROPE_LINEAR = 1, AICI_ROPE_NTK = 2, AICI_ROPE_YARN = 3 };
+char *aici_rotary_cos_sin_cache(void *out, int64_t max_position, int rot_dim, double base, int scaling,
+                                double factor, int64_t original_context, int dtype, aici_stream_t stream);
+
+/* Replaces rotary_embedding_C (lib.rs:139-146; kernels/vllm/pos_encoding_kernels.cu:40-128) in its
+ * general form: query [num_tokens, num_heads, head_size] and key [num_tokens, num_kv_heads, head_size]
+ * (token strides in elements, multiples of 8) are turned in place, is_neox != 0: element j with
+ * j + rot_dim / 2, else 2 j with 2 j + 1; elements from rot_dim on stay.  bf16 or f16; cos_sin_cache
+ * [max_position, rot_dim] of f32 (table_dtype AICI_DTYPE_F32) or the query's type.  head_size and
+ * rot_dim are multiples of 16 up to 256.  Arithmetic in fp32, rounded once (the reference rounds every
+ * product; aici_rotary_reshape_and_cache follows it).  A token whose position is outside the table
+ * stays as it is (AICI_STATUS_BAD_SLOT). */
+char *aici_rotary_embedding(const int64_t *positions, void *query, void *key, const void *cos_sin_cache,
+                            int num_tokens, int num_heads, int num_kv_heads, int head_size, int rot_dim,
+                            int is_neox, int64_t max_position, int64_t query_stride, int64_t key_stride,
+                            int table_dtype, int dtype, aici_stream_t stream);
+
+/* The same in one pass with the cache write: the turned key and `value` also go to the paged cache at
+ * slot_mapping (negative slots are skipped; the slots of a call are distinct).  Caches
+ * [num_blocks, num_kv_heads, head_size / 8, 16, 8] and [num_blocks, num_kv_heads, head_size, 16]. */
+char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, void *key, const void *value,
+                                      const void *cos_sin_cache, void *key_cache, void *value_cache,
+                                      const void *slot_mapping, int slot_is_int64, int num_tokens,
+                                      int num_heads, int num_kv_heads, int head_size, int rot_dim,
+                                      int is_neox, int64_t max_position, int block_size, int64_t num_blocks,
+                                      int64_t query_stride, int64_t key_stride, int64_t value_stride,
+                                      int table_dtype, int dtype, aici_stream_t stream);
+
+/* ---- attention with a sliding window and sinks ----------------------------------------------------
+ * The query at position p of its sequence sees the tokens t <= p with t > p - window or t < sinks
+ * (window >= 1, sinks >= 0; a window that covers the context gives causal attention).  bf16 or f16,
+ * head_size 128, block_size 16; fp32 scores and sums, probabilities rounded to the 16-bit type before
+ * they meet the values.  A row that sees nothing is zero.
+ *
+ * Decode over the paged cache, arguments as in aici_paged_attention_v1: one query per sequence at
+ * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number.  Blocks that hold no
+ * visible token are not read (their table entries may be anything), and tokens that are not visible
+ * may hold anything, NaN included.  `workspace` as there, of the size that
+ * aici_paged_attention_window_workspace_bytes gives; calls that overlap on the GPU need one each. */
+size_t aici_paged_attention_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
+                                                   int max_context_len, int window, int sinks);
+char *aici_paged_attention_window(void *out, const void *query, const void *key_cache,
+                                  const void *value_cache, int num_kv_heads, float scale,
+                                  const int32_t *block_tables, const int32_t *context_lens, int block_size,
+                                  int max_context_len, int window, int sinks, int num_seqs, int num_heads,
+                                  int head_size, int max_num_blocks_per_seq, int64_t num_blocks,
+                                  int64_t q_stride, int64_t kv_block_stride, int64_t kv_head_stride,
+                                  void *workspace, size_t workspace_bytes, int dtype, aici_stream_t stream);
+
+/* Prefill over packed keys and values (arguments as in aici_mha_varlen_fwd) and over the paged cache
+ * (as in aici_mha_varlen_paged_fwd); row r of a sequence is the token at position len_k - len_q + r, any
+ * number of query heads per kv head.  Tokens that none of the 128 rows of a query tile (rows
+ * 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token that one of
+ * them sees are not read. */
+char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
+                                 const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
+                                 int total_q, int total_k, int num_heads, int num_heads_k, int head_size,
+                                 int max_seqlen_q, int max_seqlen_k, int window, int sinks,
+                                 int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride,
+                                 int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                                 int64_t o_tok_stride, int64_t o_head_stride, float softmax_scale,
+                                 int dtype, aici_stream_t stream);
+char *aici_mha_varlen_paged_window_fwd(void *out, const void *q, const void *key_cache,
+                                       const void *value_cache, const int32_t *cu_seqlens_q,
+                                       const int32_t *context_lens, const int32_t *block_tables, int batch,
+                                       int total_q, int num_heads, int num_kv_heads, int head_size,
+                                       int block_size, int max_seqlen_q, int max_context_len,
+                                       int max_num_blocks_per_seq, int64_t num_blocks, int window,
+                                       int sinks, int64_t q_tok_stride, int64_t q_head_stride,
+                                       int64_t o_tok_stride, int64_t o_head_stride,
+                                       int64_t kv_block_stride, int64_t kv_head_stride,
+                                       float softmax_scale, int dtype, aici_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,149 @@
+"""Rotary positions: the table, both pairings, part of the head, both 16-bit types, with and without the
+cache write, against the definition in 64 bits."""
+import pytest
+import torch
+
+from aici_b200 import _lib, tch_cuda
+from oracle import window_ref as W
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n,rot,base,scaling,factor,original,dtype", [
+    (1, 2, 1e4, "none", 1.0, 0, torch.float32), (33, 16, 1e4, "none", 1.0, 0, torch.float32),
+    (257, 96, 1e4, "linear", 2.5, 0, torch.float32), (300, 128, 5e5, "ntk", 4.0, 0, torch.float32),
+    (5000, 128, 1e6, "yarn", 8.0, 512, torch.float32), (70, 2, 1e4, "ntk", 2.0, 0, torch.float32),
+    (129, 256, 1e4, "yarn", 1.0, 64, torch.bfloat16), (130, 66, 1e4, "none", 1.0, 0, torch.float16)])
+def test_table(cuda_device, n, rot, base, scaling, factor, original, dtype):
+    got = tch_cuda.rotary_cos_sin_cache(n, rot, base, dtype, cuda_device, scaling=scaling, factor=factor,
+                                        original_context=original).cpu().double()
+    if rot == 2 and scaling == "ntk":  # one pair turns by 1 per position whatever the base
+        scaling = "none"
+    want = W.cos_sin(range(n), rot, base, scaling, factor, original)
+    # half a step of the type; the angle in 64 bits, off by some 2^-50 of itself at most
+    under = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -149
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + n * 2.0 ** -49 + under
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
+def test_table_far_positions(cuda_device):
+    n, rot = 1 << 20, 16
+    got = tch_cuda.rotary_cos_sin_cache(n, rot, 1e4, torch.float32, cuda_device)
+    at = [0, 1, 65535, 65536, 99999, 524287, 524288, n - 2, n - 1]
+    want = W.cos_sin(at, rot, 1e4, "none", 1.0, 0)
+    assert ((got[at].cpu().double() - want).abs() <= 2.0 ** -24 * want.abs() + n * 2.0 ** -49 + 2.0 ** -60).all()
+
+
+def inputs(seed, T, H, Hk, D, rot, dtype, table, gap=0):
+    g = torch.Generator().manual_seed(seed)
+    wide = torch.randn(T, (H + 2 * Hk) * D + gap, generator=g).to(dtype)
+    cs = W.cos_sin(range(500), rot, 1e4, "none", 1.0, 0).to(table)
+    pos = torch.randint(0, 500, (T,), generator=g)
+    nblk = (T + 40) // 16 + 6
+    slots = torch.randperm(nblk * 16 - 64, generator=g)[:T] + 64
+    if T >= 40:  # a run that starts inside a block, as a chunk does, and one on a block's start
+        slots[:21] = torch.arange(21) + 5
+        slots[21:37] = torch.arange(16) + 32
+    if T > 2:
+        slots[2] = -1
+    kc = torch.randn(nblk, Hk, D // 8, 16, 8, generator=g).to(dtype)
+    vc = torch.randn(nblk, Hk, D, 16, generator=g).to(dtype)
+    return wide, cs, pos, slots, kc, vc
+
+
+def close(got, want, mag, dtype):
+    """Half a step of the type, three fp32 roundings of the products' magnitudes; f16 below its normals."""
+    under = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    bound = torch.finfo(dtype).eps / 2 * want.abs() * 1.01 + 2.0 ** -22 * mag + under
+    d = (got.cpu().double() - want).abs()
+    assert (d <= bound).all(), float((d / bound.clamp(min=1e-30)).max())
+
+
+CASES = [(1, 1, 1, 16, 16, True), (1, 8, 2, 128, 128, True), (3, 5, 1, 64, 32, False), (16, 4, 4, 80, 32, True),
+         (17, 6, 2, 96, 96, False), (40, 8, 8, 128, 64, False), (50, 7, 1, 128, 48, True), (41, 2, 2, 256, 256, False),
+         (200, 32, 8, 128, 128, True), (64, 3, 3, 256, 16, True)]
+
+
+@pytest.mark.parametrize("dtype,table", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                         (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("T,H,Hk,D,rot,neox", CASES)
+def test_with_cache_write(cuda_device, T, H, Hk, D, rot, neox, dtype, table):
+    dev = cuda_device
+    wide, cs, pos, slots, kc, vc = inputs(T * 7 + rot, T, H, Hk, D, rot, dtype, table, gap=8)
+    x = wide.to(dev)
+    q, k, v = x[:, :H * D], x[:, H * D:(H + Hk) * D], x[:, (H + Hk) * D:(H + 2 * Hk) * D]
+    kc_d, vc_d = kc.to(dev), vc.to(dev)
+    slot_d = slots.to(dev) if T % 2 else slots.to(torch.int32).to(dev)
+    tch_cuda.rotary_embedding_and_cache(pos.to(dev), q, k, v, D, cs.to(dev), neox, kc_d, vc_d, slot_d)
+    wq, mq = W.rotate(wide[:, :H * D].view(T, H, D), cs[pos], neox)
+    wk, mk = W.rotate(wide[:, H * D:(H + Hk) * D].reshape(T, Hk, D), cs[pos], neox)
+    close(q.reshape(T, H, D), wq, mq, dtype)
+    close(k.reshape(T, Hk, D), wk, mk, dtype)
+    assert torch.equal(x[:, (H + Hk) * D:].cpu(), wide[:, (H + Hk) * D:])  # values and what lies behind them
+    W.write_cache(k.reshape(T, Hk, D).cpu(), v.reshape(T, Hk, D).cpu(), kc, vc, slots)
+    assert torch.equal(kc_d.cpu().view(torch.int16), kc.view(torch.int16))
+    assert torch.equal(vc_d.cpu().view(torch.int16), vc.view(torch.int16))
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("T,H,Hk,D,rot,neox", CASES)
+def test_alone_gives_what_it_gives_with_the_cache(cuda_device, T, H, Hk, D, rot, neox):
+    dev, dtype = cuda_device, torch.bfloat16
+    wide, cs, pos, slots, kc, vc = inputs(T + 3 * D, T, H, Hk, D, rot, dtype, torch.float32)
+    a, b = wide.to(dev), wide.to(dev)
+    cut = lambda x: (x[:, :H * D], x[:, H * D:(H + Hk) * D], x[:, (H + Hk) * D:])  # noqa: E731
+    tch_cuda.rotary_embedding(pos.to(dev), *cut(a)[:2], D, cs.to(dev), neox)
+    tch_cuda.rotary_embedding_and_cache(pos.to(dev), *cut(b), D, cs.to(dev), neox, kc.to(dev), vc.to(dev), slots.to(dev))
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    h = wide.to(dev)  # the same rows as [tokens, heads, head_size]
+    q3, k3 = h[:, :H * D].unflatten(1, (H, D)), h[:, H * D:(H + Hk) * D].unflatten(1, (Hk, D))
+    tch_cuda.rotary_embedding(pos.to(dev), q3, k3, D, cs.to(dev), neox)
+    assert torch.equal(a.view(torch.int16), h.view(torch.int16))
+
+
+def test_bad_positions_and_slots_leave_their_tokens(cuda_device):
+    dev, T, H, Hk, D = cuda_device, 20, 4, 2, 128
+    wide, cs, pos, slots, kc, vc = inputs(5, T, H, Hk, D, 128, torch.bfloat16, torch.float32)
+    pos[4], pos[11], slots[7] = 500, -1, kc.shape[0] * 16
+    x, kc_d, vc_d = wide.to(dev), kc.to(dev), vc.to(dev)
+    q, k, v = x[:, :H * D], x[:, H * D:(H + Hk) * D], x[:, (H + Hk) * D:]
+    tch_cuda.rotary_embedding_and_cache(pos.to(dev), q, k, v, D, cs.to(dev), True, kc_d, vc_d, slots.to(dev))
+    assert _lib.last_status() == 2
+    for t in (4, 11):
+        assert torch.equal(x[t].cpu(), wide[t])
+    good = slots.clone()
+    good[[4, 7, 11]] = -1
+    W.write_cache(k.reshape(T, Hk, D).cpu(), v.reshape(T, Hk, D).cpu(), kc, vc, good)
+    assert torch.equal(kc_d.cpu(), kc) and torch.equal(vc_d.cpu(), vc)
+
+
+def test_cache_offsets_past_32_bits(cuda_device):
+    """A pool of more than 2^31 elements; only its last blocks are written."""
+    dev, Hk, D = cuda_device, 8, 128
+    nblk = (1 << 31) // (Hk * D * 16) + 16
+    kc = torch.zeros(nblk, Hk, D // 8, 16, 8, dtype=torch.float16, device=dev)
+    vc = torch.zeros(nblk, Hk, D, 16, dtype=torch.float16, device=dev)
+    wide, cs, pos, _, _, _ = inputs(6, 20, 8, Hk, D, 64, torch.float16, torch.float32)
+    x = wide.to(dev)
+    q, k, v = x[:, :8 * D], x[:, 8 * D:16 * D], x[:, 16 * D:]
+    slots = torch.arange(20) + (nblk - 3) * 16 + 7
+    tch_cuda.rotary_embedding_and_cache(pos.to(dev), q, k, v, D, cs.to(dev), False, kc, vc, slots.to(dev))
+    want_k, want_v = torch.zeros(8, Hk, 16, 16, 8, dtype=torch.float16), torch.zeros(8, Hk, 128, 16, dtype=torch.float16)
+    W.write_cache(k.reshape(20, Hk, D).cpu(), v.reshape(20, Hk, D).cpu(), want_k, want_v, slots - (nblk - 8) * 16)
+    assert torch.equal(kc[-8:].cpu(), want_k) and torch.equal(vc[-8:].cpu(), want_v)
+    assert not kc[:8].any() and not vc[:8].any() and _lib.last_status() == 0
+
+
+def test_refuses_mismatched_tensors(cuda_device):
+    dev = cuda_device
+    wide, cs, pos, slots, kc, vc = (t.to(dev) for t in inputs(7, 4, 4, 2, 128, 128, torch.bfloat16, torch.float32))
+    q, k, v = wide[:, :512], wide[:, 512:768], wide[:, 768:]
+    ok = (pos, q, k, v, 128, cs, True, kc, vc, slots)
+    for i, bad, match in ((0, pos.int(), "positions"), (0, pos[:3], "positions"), (2, k.half(), "same dtype"),
+                          (3, v.half(), "dtypes differ"), (4, 64, "head_size"), (5, cs.t(), "cos_sin_cache"),
+                          (5, cs.half(), "cos_sin_cache"), (7, kc.half(), "dtypes differ"), (9, slots[:2], "slot_mapping"),
+                          (2, wide[:, 512:1024], "width"), (3, v[:3], "differ in length")):
+        args = list(ok)
+        args[i] = bad
+        with pytest.raises(_lib.AiciError, match=match):
+            tch_cuda.rotary_embedding_and_cache(*args)

@@ -1,0 +1,356 @@
+"""Attention with a sliding window and sinks -- decode over the paged cache, prefill over packed tensors
+and over the cache -- against the definition in 64 bits, at the sizes and masks where it can go wrong."""
+import math
+import random
+
+import pytest
+import torch
+
+from aici_b200 import _lib, tch_cuda
+from oracle import window_ref as W
+
+pytestmark = pytest.mark.gpu
+D, SCALE = 128, 1 / math.sqrt(128)
+NAN = float("nan")
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def normal(g, dtype, *shape):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def paged(g, lens, Hk, dtype, extra_blocks=3):
+    """Sequences in shuffled blocks: caches, table, and the tokens [n, Hk, D] of each.  Everything that is
+    no token is NaN, and table entries that name no block are -1."""
+    counts = [-(-n // 16) for n in lens]
+    nblk = sum(counts) + extra_blocks
+    perm = torch.randperm(nblk, generator=g).tolist()
+    kc = torch.full((nblk, Hk, D // 8, 16, 8), NAN, dtype=dtype)
+    vc = torch.full((nblk, Hk, D, 16), NAN, dtype=dtype)
+    table = torch.full((len(lens), max(max(counts), 1) + 1), -1, dtype=torch.int32)
+    ks, vs = [], []
+    for i, n in enumerate(lens):
+        row = [perm.pop() for _ in range(counts[i])]
+        table[i, :len(row)] = torch.tensor(row, dtype=torch.int32)
+        k, v = normal(g, dtype, n, Hk, D), normal(g, dtype, n, Hk, D)
+        slots = torch.tensor([row[t // 16] * 16 + t % 16 for t in range(n)], dtype=torch.int64)
+        W.write_cache(k, v, kc, vc, slots)
+        ks.append(k)
+        vs.append(v)
+    return kc, vc, table, ks, vs
+
+
+def hide_unseen(kc, vc, table, i, n, seen):
+    """NaN into the tokens 0 .. n - 1 of sequence i that nobody sees; -1 into entries of unseen blocks."""
+    for t in range(n):
+        if t not in seen:
+            b, o = int(table[i, t // 16]), t % 16
+            kc[b, :, :, o] = NAN
+            vc[b, :, :, o] = NAN
+    for b in range(-(-n // 16)):
+        if not any(t in seen for t in range(16 * b, 16 * b + 16)):
+            table[i, b] = -1
+
+
+def near(got, q, k, v, positions, window, sinks, dtype, scale=SCALE):
+    worst = 0.0
+    for r, p in enumerate(positions):
+        o, a, n, size = W.attention_row(q[r], k, v, p, window, sinks, scale)
+        vmax = float(v[W.visible(p, window, sinks)].abs().max()) if n else 0.0
+        bound = W.attention_bound(o, a, n, size, vmax, dtype)
+        d = (got[r].double() - o).abs()
+        assert torch.isfinite(got[r]).all(), (r, p)
+        worst = max(worst, float((d / bound).max()))
+    assert worst <= 1, worst
+
+
+# ---- decode -------------------------------------------------------------------------------------------
+def decode(dev, q, kc, vc, table, ctx, window, sinks, scale=SCALE):
+    out = torch.full((len(ctx), q.shape[1], D), NAN, dtype=q.dtype, device=dev)
+    tch_cuda.paged_attention_window(out, q.to(dev), kc.to(dev), vc.to(dev), kc.shape[1], scale, table.to(dev),
+                                    torch.tensor(ctx, dtype=torch.int32, device=dev), 16, max(max(ctx), 1), window, sinks)
+    return out.cpu()
+
+
+DECODES = [  # contexts, heads, kv heads, window, sinks
+    ([1], 1, 1, 1, 0), ([0], 2, 1, 8, 4), ([16, 17, 15, 0, 1], 8, 2, 16, 0), ([33, 64, 100], 4, 4, 5, 3),
+    ([200, 3, 47, 0, 129], 8, 1, 40, 17), ([300], 6, 2, 1, 1), ([500, 77], 16, 1, 100, 50), ([129, 128, 127], 15, 3, 128, 128),
+    ([40, 41, 42, 43], 7, 1, 1000, 2), ([1025], 32, 8, 600, 0), ([700, 1, 0, 350], 5, 5, 64, 300), ([90], 24, 2, 33, 4000),
+    ([2000, 1999], 12, 1, 1111, 31), ([260] * 40, 4, 1, 70, 4)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ctx,H,Hk,window,sinks", DECODES)
+def test_decode(cuda_device, ctx, H, Hk, window, sinks, dtype):
+    g = torch.Generator().manual_seed(sum(ctx) + H + window)
+    kc, vc, table, ks, vs = paged(g, ctx, Hk, dtype)
+    for i, n in enumerate(ctx):
+        hide_unseen(kc, vc, table, i, n, set(W.visible(n - 1, window, sinks)))
+    q = normal(g, dtype, len(ctx), H, D)
+    got = decode(cuda_device, q, kc, vc, table, ctx, window, sinks)
+    for i, n in enumerate(ctx):
+        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], window, sinks, dtype)
+    assert _lib.last_status() == 0
+
+
+def test_decode_many_sequences(cuda_device):
+    """More rows than the GPU has places for, some of them empty."""
+    r = random.Random(4)
+    ctx = [r.choice([0, 1, r.randint(1, 90), 40]) for _ in range(2500)]
+    g = torch.Generator().manual_seed(4)
+    kc, vc, table, ks, vs = paged(g, ctx, 2, torch.bfloat16)
+    q = normal(g, torch.bfloat16, len(ctx), 4, D)
+    got = decode(cuda_device, q, kc, vc, table, ctx, 24, 2)
+    for i in r.sample(range(len(ctx)), 200) + [0, len(ctx) - 1]:
+        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [ctx[i] - 1], 24, 2, torch.bfloat16)
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_decode_uneven_scores(cuda_device, dtype):
+    """One token far above the rest, at either end of the window and among the sinks."""
+    g = torch.Generator().manual_seed(9)
+    ctx = [400, 400, 400, 400]
+    kc, vc, table, ks, vs = paged(g, ctx, 1, dtype)
+    q = normal(g, dtype, 4, 4, D)
+    for i, t in enumerate((2, 300, 399, 350)):
+        ks[i][t] = (q[i, 0] * (6.0 if i else 30.0)).to(dtype)
+        W.write_cache(ks[i][t:t + 1], vs[i][t:t + 1], kc, vc, table[i, t // 16:t // 16 + 1].long() * 16 + t % 16)
+    got = decode(cuda_device, q, kc, vc, table, ctx, 100, 4)
+    for i in range(4):
+        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [399], 100, 4, dtype)
+
+
+def test_decode_strided_queries_and_infinite_masked_tokens(cuda_device):
+    dev, dtype = cuda_device, torch.bfloat16
+    g = torch.Generator().manual_seed(10)
+    ctx = [70, 35]
+    kc, vc, table, ks, vs = paged(g, ctx, 2, dtype)
+    for i, n in enumerate(ctx):
+        seen = set(W.visible(n - 1, 20, 3))
+        for t in range(n):
+            if t not in seen:
+                kc[table[i, t // 16], :, :, t % 16] = float("inf")
+                vc[table[i, t // 16], :, :, t % 16] = -float("inf")
+    wide = normal(g, dtype, 2, 8 * D + 64)
+    q = wide[:, :8 * D].unflatten(1, (8, D))
+    out = torch.empty(2, 8, D, dtype=dtype, device=dev)
+    wd = wide.to(dev)
+    tch_cuda.paged_attention_window(out, wd[:, :8 * D].unflatten(1, (8, D)), kc.to(dev), vc.to(dev), 2, SCALE, table.to(dev),
+                                    torch.tensor(ctx, dtype=torch.int32, device=dev), 16, 70, 20, 3)
+    for i, n in enumerate(ctx):
+        near(out.cpu()[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 20, 3, dtype)
+
+
+def test_decode_bad_visible_block_is_reported(cuda_device):
+    g = torch.Generator().manual_seed(11)
+    kc, vc, table, _, _ = paged(g, [100, 40], 1, torch.bfloat16)
+    kc, vc = kc.nan_to_num(0.0), vc.nan_to_num(0.0)
+    table[0, 6] = kc.shape[0]
+    q = normal(g, torch.bfloat16, 2, 2, D)
+    got = decode(cuda_device, q, kc, vc, table, [100, 40], 30, 0)
+    assert torch.isfinite(got).all() and _lib.last_status() == 1
+    decode(cuda_device, q, kc, vc, table, [100 + 16 * 30, 40], 30, 0)  # longer than its table row
+    assert _lib.last_status() == 1
+
+
+def test_decode_cache_offsets_past_32_bits(cuda_device):
+    dev, Hk = cuda_device, 8
+    nblk = (1 << 31) // (Hk * D * 16) + 64
+    kc = torch.empty(nblk, Hk, D // 8, 16, 8, dtype=torch.bfloat16, device=dev)
+    vc = torch.empty(nblk, Hk, D, 16, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(12)
+    k, v, ctx = normal(g, torch.bfloat16, 200, Hk, D), normal(g, torch.bfloat16, 200, Hk, D), 200
+    row = torch.arange(nblk - 13, nblk, dtype=torch.int32)
+    small_k, small_v = torch.zeros(13, Hk, 16, 16, 8, dtype=torch.bfloat16), torch.zeros(13, Hk, D, 16, dtype=torch.bfloat16)
+    W.write_cache(k, v, small_k, small_v, torch.arange(200))
+    kc[-13:], vc[-13:] = small_k.to(dev), small_v.to(dev)
+    q = normal(g, torch.bfloat16, 1, 16, D)
+    out = torch.empty(1, 16, D, dtype=torch.bfloat16, device=dev)
+    tch_cuda.paged_attention_window(out, q.to(dev), kc, vc, Hk, SCALE, row.view(1, -1).to(dev),
+                                    torch.tensor([ctx], dtype=torch.int32, device=dev), 16, ctx, 90, 2)
+    near(out.cpu(), q, k, v, [ctx - 1], 90, 2, torch.bfloat16)
+    o2 = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc, vc, torch.tensor([0, 1], dtype=torch.int32, device=dev),
+                                                 torch.tensor([ctx], dtype=torch.int32, device=dev), row.view(1, -1).to(dev),
+                                                 1, ctx, SCALE, 90, 2)
+    near(o2.cpu(), q, k, v, [ctx - 1], 90, 2, torch.bfloat16)
+    assert _lib.last_status() == 0
+
+
+def test_decode_two_graphs_at_once(cuda_device):
+    """Two captured calls of different batches replayed on two streams: neither disturbs the other."""
+    dev, dtype = cuda_device, torch.bfloat16
+    jobs = []
+    for seed, S, n in ((1, 3, 900), (2, 50, 300)):
+        g = torch.Generator().manual_seed(seed)
+        ctx = [n - 7 * i % 40 for i in range(S)]
+        kc, vc, table, _, _ = paged(g, ctx, 4, dtype)
+        q = normal(g, dtype, S, 8, D).to(dev)
+        args = (q, kc.to(dev), vc.to(dev), 4, SCALE, table.to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev), 16, n, 500, 4)
+        out, ref = torch.empty_like(q), torch.empty_like(q)
+        tch_cuda.paged_attention_window(ref, *args)
+        stream = torch.cuda.Stream(dev)
+        stream.wait_stream(torch.cuda.current_stream(dev))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            tch_cuda.paged_attention_window(out, *args)
+        jobs.append((graph, stream, out, ref))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream, out, _ in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, ref in jobs:
+        assert torch.equal(out, ref)
+
+
+def test_results_do_not_depend_on_the_run(cuda_device):
+    g = torch.Generator().manual_seed(13)
+    ctx = [1500, 20, 700]
+    kc, vc, table, _, _ = paged(g, ctx, 2, torch.bfloat16)
+    q = normal(g, torch.bfloat16, 3, 8, D)
+    a = decode(cuda_device, q, kc, vc, table, ctx, 1200, 4)
+    for _ in range(5):
+        assert torch.equal(a, decode(cuda_device, q, kc, vc, table, ctx, 1200, 4))
+
+
+# ---- prefill ------------------------------------------------------------------------------------------
+PREFILLS = [  # query lengths, key lengths, heads, kv heads, window, sinks
+    ([1], [1], 1, 1, 1, 0), ([5, 0, 1], [5, 0, 9], 2, 1, 3, 1), ([128], [128], 2, 2, 128, 0), ([127, 129], [127, 129], 4, 2, 16, 4),
+    ([130], [300], 2, 1, 100, 20), ([300], [300], 3, 1, 1, 0), ([64, 200], [264, 200], 8, 2, 70, 0), ([140], [40], 2, 1, 30, 2),
+    ([257], [257], 2, 2, 129, 130), ([100, 3], [1000, 700], 4, 1, 200, 5), ([260], [260], 6, 2, 5000, 0), ([40], [700], 10, 2, 64, 300),
+    ([20, 150], [20, 10], 2, 2, 12, 0), ([384], [512], 4, 2, 256, 128), ([1, 1, 1], [600, 17, 128], 5, 1, 33, 1)]
+
+
+def run_prefill(dev, g, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged, hide=True):
+    seen = []
+    for lq, lk in zip(lens_q, lens_k):
+        s = set()
+        for r in range(lq):
+            s |= set(W.visible(lk - lq + r, window, sinks))
+        seen.append(s)
+    total = sum(lens_q)
+    wide = normal(g, dtype, total, H + 3, D)
+    q = wide[:, 1:H + 1]
+    cu = lambda lens: torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=dev)  # noqa: E731
+    wd = wide.to(dev)
+    if is_paged:
+        kc, vc, table, ks, vs = paged(g, lens_k, Hk, dtype)
+        for i, n in enumerate(lens_k):
+            if hide:
+                hide_unseen(kc, vc, table, i, n, seen[i])
+        out = tch_cuda.flash_attn_varlen_paged_window(wd[:, 1:H + 1], kc.to(dev), vc.to(dev), cu(lens_q),
+                                                      torch.tensor(lens_k, dtype=torch.int32, device=dev), table.to(dev),
+                                                      max(lens_q), max(lens_k), SCALE, window, sinks)
+    else:
+        ks = [normal(g, dtype, n, Hk, D) for n in lens_k]
+        vs = [normal(g, dtype, n, Hk, D) for n in lens_k]
+        k2, v2 = [k.clone() for k in ks], [v.clone() for v in vs]
+        for i, n in enumerate(lens_k):
+            for t in range(n):
+                if hide and t not in seen[i]:
+                    k2[i][t], v2[i][t] = NAN, NAN
+        kv = torch.cat([torch.cat(k2), torch.cat(v2)], 1).to(dev)  # strided keys and values
+        out = tch_cuda.flash_attn_varlen_window(wd[:, 1:H + 1], kv[:, :Hk], kv[:, Hk:], cu(lens_q), cu(lens_k), max(lens_q),
+                                                max(lens_k), SCALE, window, sinks)
+    return out.cpu(), q, ks, vs
+
+
+@pytest.mark.parametrize("is_paged", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", PREFILLS)
+def test_prefill(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged):
+    g = torch.Generator().manual_seed(sum(lens_q) * 3 + sum(lens_k) + window)
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged)
+    at = 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        near(out[at:at + lq], q[at:at + lq], ks[i], vs[i], range(lk - lq, lk), window, sinks, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("is_paged", [False, True])
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
+    ([2500], [2500], 4, 2, 700, 4), ([300, 900], [3500, 900], 8, 1, 2300, 200), ([700], [4400], 6, 6, 4096, 0),
+    ([129], [2700], 3, 1, 1000, 33)])
+def test_prefill_long(cuda_device, lens_q, lens_k, H, Hk, window, sinks, is_paged):
+    """Long enough for the shapes that long sequences take; a sample of the rows."""
+    dtype = torch.float16 if Hk == 1 else torch.bfloat16
+    g = torch.Generator().manual_seed(sum(lens_k))
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged, hide=len(lens_q) == 1)
+    r, at = random.Random(1), 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        rows = sorted(set(r.sample(range(lq), 60) + [0, 1, 127, min(128, lq - 1), lq - 1]))
+        near(out[at:at + lq][rows], q[at:at + lq][rows], ks[i], vs[i], [lk - lq + x for x in rows], window, sinks, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(60, 0), (200, 3), (1000, 0)])
+def test_prefill_uneven_scores(cuda_device, dtype, window, sinks):
+    """Keys that outgrow each other along the sequence and against it, scores up to some hundreds."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(window)
+    n, H = 520, 2
+    for order in (1, -1):
+        q, k, v = normal(g, dtype, n, H, D), normal(g, dtype, n, 1, D), normal(g, dtype, n, 1, D)
+        by = torch.linspace(0.05, 30, n).view(n, 1, 1)
+        by = by if order == 1 else by.flip(0)
+        k = (k.float() * by).to(dtype)
+        cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+        out = tch_cuda.flash_attn_varlen_window(q.to(dev), k.to(dev), v.to(dev), cu, cu, n, n, SCALE, window, sinks).cpu()
+        near(out[::7], q[::7], k, v, range(0, n, 7), window, sinks, dtype)
+
+
+def test_prefill_with_a_covering_window_is_causal_attention(cuda_device):
+    dev, g = cuda_device, torch.Generator().manual_seed(3)
+    q, k, v = (normal(g, torch.bfloat16, 700, h, D).to(dev) for h in (8, 2, 2))
+    cu = torch.tensor([0, 300, 700], dtype=torch.int32, device=dev)
+    a = tch_cuda.flash_attn_varlen_window(q, k, v, cu, cu, 400, 400, SCALE, 1 << 40).float()
+    b = tch_cuda.flash_attn_varlen(q, k, v, cu, cu, 400, 400, SCALE, True).float()
+    # both are within half a step of the output and one of each probability of the exact result
+    assert float((a - b).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
+
+
+def test_prefill_of_single_tokens_is_decode(cuda_device):
+    dev, dtype = cuda_device, torch.float16
+    g = torch.Generator().manual_seed(14)
+    ctx = [600, 17, 128, 1]
+    kc, vc, table, ks, vs = paged(g, ctx, 2, dtype)
+    q = normal(g, dtype, 4, 8, D)
+    got = decode(dev, q, kc, vc, table, ctx, 100, 4)
+    out = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc.to(dev), vc.to(dev), torch.arange(5, dtype=torch.int32, device=dev),
+                                                  torch.tensor(ctx, dtype=torch.int32, device=dev), table.to(dev), 1, 600,
+                                                  SCALE, 100, 4).cpu()
+    for i, n in enumerate(ctx):
+        for o in (got, out):
+            near(o[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 100, 4, dtype)
+
+
+def test_rows_behind_the_last_sequence_stay(cuda_device):
+    """A batch padded for a captured step: query rows that no sequence owns are not written."""
+    dev, g = cuda_device, torch.Generator().manual_seed(15)
+    q, k, v = (normal(g, torch.bfloat16, 200, 2, D).to(dev) for _ in range(3))
+    cu = torch.tensor([0, 130, 130], dtype=torch.int32, device=dev)
+    L, p = _lib.lib(), lambda t: t.data_ptr()  # noqa: E731
+    out = torch.full_like(q, 7.0)
+    _lib.check("x", L.aici_mha_varlen_window_fwd(
+        p(out), p(q), p(k), p(v), p(cu), p(cu), 2, 200, 200, 2, 2, D, 130, 130, 50, 0, *[256, 128] * 4, SCALE, 0,
+        torch.cuda.current_stream().cuda_stream))
+    near(out[:130].cpu(), q[:130].cpu(), k.cpu(), v.cpu(), range(130), 50, 0, torch.bfloat16)
+    assert (out[130:] == 7.0).all()
+
+
+def test_refuses_mismatched_tensors(cuda_device):
+    dev = cuda_device
+    q, i = torch.zeros(4, 2, D, dtype=torch.bfloat16, device=dev), torch.tensor([0, 4], dtype=torch.int32, device=dev)
+    f = lambda **c: tch_cuda.flash_attn_varlen_window(**{**dict(  # noqa: E731
+        q=q, k=q, v=q, seqlens_q=i, seqlens_k=i, max_seqlen_q=4, max_seqlen_k=4, softmax_scale=1.0, window=4), **c})
+    for change, match in ((dict(k=q.half()), "same dtype"), (dict(v=q[:3]), "k and v"), (dict(seqlens_q=i.long()), "seqlens_q"),
+                          (dict(seqlens_k=i[:1]), "seqlens_k"), (dict(q=q.float(), k=q.float(), v=q.float()), "only bf16 and f16"),
+                          (dict(q=q.transpose(1, 2)), "contiguous last"), (dict(window=0), "window"), (dict(sinks=-1), "sinks")):
+        with pytest.raises(_lib.AiciError, match=match):
+            f(**change)
+    f()
