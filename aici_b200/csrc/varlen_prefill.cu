@@ -28,6 +28,7 @@
 // (One-tile shape: warps 0-3 softmax, warp 4 producer, warp 5 issuer.)  The grid is ordered
 // (head, sequence, row tile), row tile slowest and longest first.
 // Every barrier wait is bounded; a timeout sets AICI_STATUS_WAIT_TIMEOUT and unwinds.
+#include "half_types.cuh"
 #include "tcgen05.cuh"
 
 namespace aici {
@@ -70,6 +71,7 @@ struct PrefillCfg {
 };
 constexpr float kRescaleThreshold = 8.f;  // log2 units: the running reference moves once a score exceeds it by this
 constexpr float kRescaleSum = 256.f;      // single-pass tiles: a row sum above this moves the reference (some score is 2^8 above it, or many are above it)
+constexpr float kDangerSumF16 = 3e4f;     // the same for f16 probabilities, whose range ends at 65504
 constexpr float kDangerSum = 1e30f;       // single-pass tiles: a row sum at or above this (or NaN) means the tile is redone exactly
 
 struct PrefillParams {
@@ -92,6 +94,8 @@ struct PrefillParams {
   const int32_t *k_lens;        // [batch] tokens of each sequence present in the cache
   int max_blocks;
   int64_t num_blocks;
+  // windowed variant: a row at position d sees the keys t <= d with t > d - window or t < sinks
+  int window, sinks;
 };
 
 // One tensor map per output buffer (this GPU's and, for the fused gather, every peer's).
@@ -113,6 +117,25 @@ struct TileInfo {
   int n_tiles;  // key/value tiles it visits; 0 = nothing visible
 };
 
+// Windowed variant: the keys that some row of a CTA's query tile sees are [0, sinks) and [lo, lim).
+// The tiles that hold them are visited from the diagonal downwards, sinks last: the first tile then
+// gives (nearly) every row its reference maximum, where an ascending order would start in tiles whose
+// leading columns most rows do not see.
+struct WindowTiles {
+  int lo, lim, sinks;
+  int first, n_win;  // first window tile, number of window tiles
+  int n_sink;        // tiles of sinks below the first window tile
+  __device__ __forceinline__ int tile(int i) const {
+    return i < n_win ? first + n_win - 1 - i : n_sink - 1 - (i - n_win);
+  }
+};
+
+// Bit i: column cb + i is in [lo, hi) or [0, sinks), and below hi.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t visible_bits(int cb, int lo, int hi, int sinks) {
+  return bits_below(hi - cb) & (~bits_below(lo - cb) | bits_below(sinks - cb));
+}
+
 __device__ __forceinline__ void zero_rows(const PrefillParams &p, int q0, const TileInfo &T, int tid,
                                           int nthreads) {
   for (int i = tid; i < T.rows * (kHD / 8); i += nthreads) {
@@ -130,7 +153,10 @@ __device__ __forceinline__ void zero_rows(const PrefillParams &p, int q0, const 
 //   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] loaded with the
 //   32-byte swizzle, one K = 16 MMA per block.  Value columns past the sequence end are zeroed in
 //   shared memory before P V (cache slots there may hold anything, NaN included).
-template <bool kPaged, int kShape>
+//
+// kWindow = true: sliding window and sinks (always causal); the CTA's tiles share their rows (one tile, or
+// two heads of one kv head).  T: bf16, or f16 in the windowed variant.
+template <bool kPaged, int kShape, bool kWindow = false, typename T16 = __nv_bfloat16>
 __global__ void __launch_bounds__(PrefillCfg<kShape>::kThreads, PrefillCfg<kShape>::kCtasPerSm)
 varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ CUtensorMap tmap_k,
@@ -140,6 +166,9 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   constexpr int kTiles = Cfg::kTiles;
   constexpr bool kPair = Cfg::kPair;
   static_assert(!(kPair && kPaged), "the CTA-pair shape reads packed K/V only");
+  static_assert(!(kPair && kWindow), "the CTA-pair shape has no window");
+  // a probability must stay inside the 16-bit type until the reference has moved
+  constexpr float kDanger = Half16<T16>::kDtype == AICI_DTYPE_F16 ? kDangerSumF16 : kDangerSum;
   constexpr int kKvStages = Cfg::kStages;
   constexpr int kStageBytes = Cfg::kStageBytes;
   constexpr int kPrefillThreads = Cfg::kThreads;
@@ -203,9 +232,28 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // tiles that see no key at all are zero rows (flash_fwd_kernel.h:1056)
   if (tiles[0].rows > 0 && tiles[0].n_tiles == 0) zero_rows(p, q0, tiles[0], tid, kPrefillThreads);
   if (tiles[1].rows > 0 && tiles[1].n_tiles == 0) zero_rows(p, q0, tiles[1], tid, kPrefillThreads);
+  WindowTiles win = {};
+  if (kWindow && (tiles[0].n_tiles > 0 || tiles[1].n_tiles > 0)) {
+    const TileInfo &R = tiles[0].n_tiles > 0 ? tiles[0] : tiles[1];
+    win.lim = min(lk, R.m0 + R.rows + lk - lq);
+    win.sinks = min(p.sinks, win.lim);
+    win.lo = max(0, R.m0 + lk - lq - min(p.window, lk) + 1);  // the first row's window begins here
+    win.first = win.lo / kBN;
+    win.n_win = R.n_tiles - win.first;
+    win.n_sink = min((win.sinks + kBN - 1) / kBN, win.first);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (tiles[t].n_tiles > 0) tiles[t].n_tiles = win.n_sink + win.n_win;
+  }
   const int nt0 = tiles[0].n_tiles, nt1 = tiles[1].n_tiles;
   const int nmax = max(nt0, nt1);
   if (nmax == 0) return;
+  auto tile_of = [&](int j) { return kWindow ? win.tile(j) : j; };  // key tile of the j-th visit
+  // end of the keys that count for this CTA, and whether any key of a 16-token block does
+  const int k_end = kWindow ? win.lim : lk;
+  auto block_counts = [&](int first_token) {
+    return first_token < k_end && (!kWindow || first_token + 16 > win.lo || first_token < win.sinks);
+  };
 
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem;                       // two tiles
@@ -273,9 +321,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       const int32_t *bt_row = p.block_tables + (int64_t)b * p.max_blocks;
       auto load_id = [&](int j) {
         int id = 0;
-        const int nb = min(8, (lk - j * kBN + 15) / 16);
-        if ((lane & 7) < nb && j < nmax) {
-          id = bt_row[j * 8 + (lane & 7)];
+        if (j < nmax && block_counts(tile_of(j) * kBN + (lane & 7) * 16)) {
+          id = bt_row[tile_of(j) * 8 + (lane & 7)];
           if (id < 0 || id >= p.num_blocks) {
             set_status(p.status, AICI_STATUS_BAD_BLOCK);
             id = 0;
@@ -293,14 +340,16 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
                         mbar_wait_abortable(&sh->kv_empty[stage], (((uint32_t)i / kKvStages) & 1u) ^ 1u, p.status));
         if (!ok) break;
         uint8_t *dst = sKV + stage * kTileBytes;
-        const int nb = min(8, (lk - j * kBN + 15) / 16);  // cache blocks of this tile that exist
-        if (lane == 0) mbar_expect_tx(&sh->kv_full[stage], nb * 4096);
         const int bi = lane & 7;
+        const bool counts = block_counts(tile_of(j) * kBN + bi * 16);  // cache blocks of this tile to load
+        const int nb = __popc(__ballot_sync(0xffffffffu, counts) & 0xffu);
+        if (lane == 0) mbar_expect_tx(&sh->kv_full[stage], nb * 4096);
+        __syncwarp();
         if (i & 1) {
-          if (lane < 8 && bi < nb) tma_load_4d(dst + bi * 4096, &tmap_v, 0, 0, hk, id_cur, &sh->kv_full[stage]);
+          if (lane < 8 && counts) tma_load_4d(dst + bi * 4096, &tmap_v, 0, 0, hk, id_cur, &sh->kv_full[stage]);
           id_cur = id_next;
         } else {
-          if (lane < 16 && bi < nb)
+          if (lane < 16 && counts)
             tma_load_5d(dst + bi * 4096 + (lane >> 3) * 2048, &tmap_k, 0, (lane >> 3) * 8, 0, hk, id_cur,
                         &sh->kv_full[stage]);
         }
@@ -314,8 +363,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         const CUtensorMap *tm = (i & 1) ? &tmap_v : &tmap_k;
         mbar_expect_tx(&sh->kv_full[stage], kStageBytes);
         if (!kPair) {
-          tma_load_3d(dst, tm, 0, hk, k0 + (i >> 1) * kBN, &sh->kv_full[stage]);
-          tma_load_3d(dst + kPanelBytes, tm, 64, hk, k0 + (i >> 1) * kBN, &sh->kv_full[stage]);
+          tma_load_3d(dst, tm, 0, hk, k0 + tile_of(i >> 1) * kBN, &sh->kv_full[stage]);
+          tma_load_3d(dst + kPanelBytes, tm, 64, hk, k0 + tile_of(i >> 1) * kBN, &sh->kv_full[stage]);
         } else if (i & 1) {
           // this CTA's half of the value tile: 64 of the 128 columns, all 128 tokens (one panel)
           tma_load_3d(dst, tm, 64 * (int)pair_rank, hk, k0 + (i >> 1) * kBN, &sh->kv_full[stage]);
@@ -360,8 +409,10 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     }
   } else if (warp == Cfg::kMmaWarp) {
     // ---------------------------------------------------------------- MMA issuer -------------
-    constexpr uint32_t idesc_s = idesc_bf16(kPair ? 2 * kBM : kBM, kBN, false);
-    constexpr uint32_t idesc_pv = idesc_bf16(kPair ? 2 * kBM : kBM, kHD, !kPaged);  // packed V: MN-major; cache V: K-major
+    constexpr bool kF16 = Half16<T16>::kDtype == AICI_DTYPE_F16;
+    constexpr uint32_t idesc_s = kF16 ? idesc_f16(kBM, kBN, false) : idesc_bf16(kPair ? 2 * kBM : kBM, kBN, false);
+    constexpr uint32_t idesc_pv =
+        kF16 ? idesc_f16(kBM, kHD, !kPaged) : idesc_bf16(kPair ? 2 * kBM : kBM, kHD, !kPaged);  // packed V: MN-major; cache V: K-major
     constexpr int kKPanel = kPair ? kPanelBytes / 2 : kPanelBytes;  // one 64-column panel of a key (half) tile
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -448,7 +499,41 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     for (int j = 0; ok && j < nmax; ++j) {
       const int i_v = 2 * j + 1, i_kn = 2 * j + 2;
       if (!wait_kv(i_v)) break;
-      if (kPaged && lk - j * kBN < kBN) {
+      if constexpr (kWindow) {
+        // Value rows that no row of this query tile sees -- past its last row's position, or between the
+        // sinks and its first row's window -- are cleared: their probabilities are 0, but 0 x NaN is
+        // NaN, and blocks without a visible token were not loaded at all.
+        const int n0 = tile_of(j) * kBN;
+        const int hi = min(kBN, win.lim - n0), dead0 = min(max(win.sinks - n0, 0), kBN), dead1 = min(max(win.lo - n0, 0), kBN);
+        if (hi < kBN || dead0 < dead1) {
+          uint8_t *vt = sKV + (i_v % kKvStages) * kStageBytes;
+          auto clear = [&](int a, int b) {  // tokens [a, b) of the tile
+            if (kPaged) {
+              for (int bi = a / 16; bi * 16 < b; ++bi) {
+                uint8_t *vb = vt + bi * 4096;
+                const int t0 = max(a - bi * 16, 0), t1 = min(b - bi * 16, 16);
+                if (t1 - t0 == 16) {
+                  for (int idx = lane; idx < 256; idx += 32) reinterpret_cast<uint4 *>(vb)[idx] = make_uint4(0, 0, 0, 0);
+                } else {
+                  for (int tok = t0; tok < t1; ++tok)
+                    for (int d = lane; d < kHD; d += 32)
+                      *reinterpret_cast<uint16_t *>(vb + d * 32 + ((((tok >> 3) ^ ((d >> 2) & 1))) << 4) + (tok & 7) * 2) = 0;
+                }
+              }
+            } else {
+              for (int idx = a * 16 + lane; idx < b * 16; idx += 32) {
+                const int r = idx / 16, c = idx % 16;
+                *reinterpret_cast<uint4 *>(vt + (c >> 3) * kPanelBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+            }
+          };
+          clear(dead0, max(dead0, dead1));
+          clear(hi, kBN);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
+      if (!kWindow && kPaged && lk - j * kBN < kBN) {
         // last tile of the sequence: zero the value columns of tokens >= lk (generic-proxy stores,
         // made visible to the tensor core with a proxy fence)
         const int valid = lk - j * kBN;
@@ -467,7 +552,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!kPaged && lk - j * kBN < kBN) {
+      if (!kWindow && !kPaged && lk - j * kBN < kBN) {
         // Packed layout, last tile of the sequence: the rows behind it belong to the next sequence
         // (or were zero-filled past the end of the tensor).  Their probabilities are 0, but 0 x NaN
         // is NaN, so the rows are cleared as the reference's predicated loads clear them
@@ -515,6 +600,10 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     const int qr = T.m0 + row;
     int lim_row = lk;
     if (p.causal) lim_row = min(lk, qr + 1 + lk - lq);
+    // windowed variant: the row sees [lo_row, lim_row) and [0, sinks); sees = it is a row and sees something
+    const int lo_row = kWindow ? max(0, qr + 1 + lk - lq - min(p.window, lk)) : 0;
+    const bool sees = row < T.rows && lim_row > 0;
+    if (kWindow && !sees) lim_row = 0;  // rows of other sequences behind this one's last have no columns
     const uint32_t t_s = tmem_base + t * 128 + ((uint32_t)(quad * 32) << 16);
     const uint32_t t_o = tmem_base + kOCol + t * 128 + ((uint32_t)(quad * 32) << 16);
     const float sc = p.scale_log2e;
@@ -526,7 +615,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int n0 = j * kBN;
+      const int n0 = tile_of(j) * kBN;
       // A rescale that the previous tile found necessary but left for now: the previous P V has
       // completed (s_full of this tile is committed after it), so O can be touched.
       if (__any_sync(0xffffffffu, pending)) {
@@ -549,10 +638,14 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         tmem_wait_st();
       }
 
-      const bool full_tile = n0 + kBN <= lim_row;
+      const bool full_tile =
+          n0 + kBN <= lim_row && (!kWindow || n0 >= lo_row || n0 + kBN <= win.sinks);
       // rows that have not seen a single column so far have no reference yet: exact path, except on
       // the first tile, which takes its reference from its own first 32 columns (below)
-      bool exact_path = (j > 0) && __any_sync(0xffffffffu, m_used == -INFINITY);
+      // (windowed: the columns a row sees in its first tile are no prefix, so that tile is exact too, and
+      // so are the next ones while some row of the warp has seen nothing)
+      bool exact_path = kWindow ? __any_sync(0xffffffffu, sees && m_used == -INFINITY)
+                                : (j > 0) && __any_sync(0xffffffffu, m_used == -INFINITY);
       if (!exact_path) {
         // ---- single pass against the running reference m_used --------------------------------
         // P is computed for the whole row in registers while S is still intact; if some score
@@ -564,7 +657,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         float l0 = 0.f, l1 = 0.f;
         uint64_t acc2 = pack_f32x2(0.f, 0.f);
         tmem_ld32(t_s, ra);
-        if (j == 0) {
+        if (!kWindow && j == 0) {
           // First tile: the reference is the largest visible score among the first 32 columns (the
           // visible columns of a row are a prefix, so a row that sees nothing here sees nothing in
           // the tile).  If the rest of the tile lies far above it, the row sum says so as usual.
@@ -592,19 +685,20 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
               unpack_f32x2(x, x0, x1);
               const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
               acc2 = add_f32x2(acc2, pack_f32x2(p0, p1));
-              pk[16 * c4 + (i >> 1)] = pack_bf16(p0, p1);
+              pk[16 * c4 + (i >> 1)] = Half16<T16>::pack(p0, p1);
             }
           } else {
             const int cb = n0 + 32 * c4;
+            const uint32_t vis = kWindow ? visible_bits(cb, lo_row, lim_row, win.sinks) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const uint64_t x = fma_f32x2(pack_f32x2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])), sc2, nm2);
               float x0, x1;
               unpack_f32x2(x, x0, x1);
-              const float p0 = fast_exp2((cb + i < lim_row) ? x0 : -INFINITY);
-              const float p1 = fast_exp2((cb + i + 1 < lim_row) ? x1 : -INFINITY);
+              const float p0 = fast_exp2((kWindow ? (vis >> i) & 1u : cb + i < lim_row) ? x0 : -INFINITY);
+              const float p1 = fast_exp2((kWindow ? (vis >> (i + 1)) & 1u : cb + i + 1 < lim_row) ? x1 : -INFINITY);
               acc2 = add_f32x2(acc2, pack_f32x2(p0, p1));
-              pk[16 * c4 + (i >> 1)] = pack_bf16(p0, p1);
+              pk[16 * c4 + (i >> 1)] = Half16<T16>::pack(p0, p1);
             }
           }
         }
@@ -618,7 +712,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           l1 += a1;
         }
         const float l_tile = l0 + l1;
-        if (__any_sync(0xffffffffu, !(l_tile < kDangerSum))) {
+        if (__any_sync(0xffffffffu, !(l_tile < kDanger))) {
           exact_path = true;  // S is untouched: redo the tile with an exact maximum
         } else {
 #pragma unroll
@@ -642,9 +736,14 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           tmem_ld32(t_s + 32 * c4, r);
           tmem_wait_ld();
           const int cb = n0 + 32 * c4;
-          if (cb + 32 <= lim_row) {
+          if (full_tile || (!kWindow && cb + 32 <= lim_row)) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+          } else if (kWindow) {
+            const uint32_t vis = visible_bits(cb, lo_row, lim_row, win.sinks);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((vis >> i) & 1u) mx = fmaxf(mx, __uint_as_float(r[i]));
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -685,7 +784,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           tmem_wait_ld();
           const int cb = n0 + 32 * c4;
           uint32_t pk[16];
-          if (cb + 32 <= lim_row) {
+          if (full_tile || (!kWindow && cb + 32 <= lim_row)) {
             const uint64_t sc2 = pack_f32x2(sc, sc), nb2 = pack_f32x2(-base, -base);
             uint64_t acc2 = pack_f32x2(0.f, 0.f);
 #pragma unroll
@@ -694,18 +793,21 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
               unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc2, nb2), x0, x1);
               const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
               acc2 = add_f32x2(acc2, pack_f32x2(p0, p1));
-              pk[i >> 1] = pack_bf16(p0, p1);
+              pk[i >> 1] = Half16<T16>::pack(p0, p1);
             }
             float a0, a1;
             unpack_f32x2(acc2, a0, a1);
             l_sum += a0 + a1;
           } else {
+            const uint32_t vis = kWindow ? visible_bits(cb, lo_row, lim_row, win.sinks) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float p0 = (cb + i < lim_row) ? fast_exp2(fmaf(__uint_as_float(r[i]), sc, -base)) : 0.f;
-              const float p1 = (cb + i + 1 < lim_row) ? fast_exp2(fmaf(__uint_as_float(r[i + 1]), sc, -base)) : 0.f;
+              const bool v0 = kWindow ? (vis >> i) & 1u : cb + i < lim_row;
+              const bool v1 = kWindow ? (vis >> (i + 1)) & 1u : cb + i + 1 < lim_row;
+              const float p0 = v0 ? fast_exp2(fmaf(__uint_as_float(r[i]), sc, -base)) : 0.f;
+              const float p1 = v1 ? fast_exp2(fmaf(__uint_as_float(r[i + 1]), sc, -base)) : 0.f;
               l_sum += p0 + p1;
-              pk[i >> 1] = pack_bf16(p0, p1);
+              pk[i >> 1] = Half16<T16>::pack(p0, p1);
             }
           }
           tmem_st16(t_s + 16 * c4, pk);
@@ -741,10 +843,10 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 v;
-          v.x = pack_bf16(__uint_as_float(r[8 * q + 0]) * inv, __uint_as_float(r[8 * q + 1]) * inv);
-          v.y = pack_bf16(__uint_as_float(r[8 * q + 2]) * inv, __uint_as_float(r[8 * q + 3]) * inv);
-          v.z = pack_bf16(__uint_as_float(r[8 * q + 4]) * inv, __uint_as_float(r[8 * q + 5]) * inv);
-          v.w = pack_bf16(__uint_as_float(r[8 * q + 6]) * inv, __uint_as_float(r[8 * q + 7]) * inv);
+          v.x = Half16<T16>::pack(__uint_as_float(r[8 * q + 0]) * inv, __uint_as_float(r[8 * q + 1]) * inv);
+          v.y = Half16<T16>::pack(__uint_as_float(r[8 * q + 2]) * inv, __uint_as_float(r[8 * q + 3]) * inv);
+          v.z = Half16<T16>::pack(__uint_as_float(r[8 * q + 4]) * inv, __uint_as_float(r[8 * q + 5]) * inv);
+          v.w = Half16<T16>::pack(__uint_as_float(r[8 * q + 6]) * inv, __uint_as_float(r[8 * q + 7]) * inv);
           const int chunk = 4 * c4 + q;
           *reinterpret_cast<uint4 *>(stage + (chunk >> 3) * kPanelBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
         }
@@ -919,14 +1021,14 @@ static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base,
 #define AICI_PREFILL_ONE_TILE_MAX_K 2048
 #endif
 
-template <bool kPaged, int kShape>
+template <bool kPaged, int kShape, bool kWindow = false, typename T16 = __nv_bfloat16>
 static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                                   const OutMaps &to, PrefillParams &p, int num_heads, int batch,
                                   int max_seqlen_q, cudaStream_t stream) {
   using Cfg = PrefillCfg<kShape>;
   static OncePerDevice once;
   if (char *e = once.run([]() -> char * {
-        AICI_CUDA(cudaFuncSetAttribute(varlen_prefill_kernel<kPaged, kShape>,
+        AICI_CUDA(cudaFuncSetAttribute(varlen_prefill_kernel<kPaged, kShape, kWindow, T16>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
         return nullptr;
       }))
@@ -957,17 +1059,17 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cudaError_t le = cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<kPaged, kShape>, tq, tk, tv, to, p);
+  cudaError_t le = cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<kPaged, kShape, kWindow, T16>, tq, tk, tv, to, p);
   if (le != cudaSuccess) {
     cudaGetLastError();
     int clusters = -1, max_size = -1;
     cudaError_t e1 = cudaSuccess, e2 = cudaSuccess;
     if (Cfg::kPair) {
-      e1 = cudaOccupancyMaxActiveClusters(&clusters, varlen_prefill_kernel<kPaged, kShape>, &cfg);
+      e1 = cudaOccupancyMaxActiveClusters(&clusters, varlen_prefill_kernel<kPaged, kShape, kWindow, T16>, &cfg);
       cudaLaunchConfig_t probe = cfg;
       probe.attrs = nullptr;
       probe.numAttrs = 0;
-      e2 = cudaOccupancyMaxPotentialClusterSize(&max_size, varlen_prefill_kernel<kPaged, kShape>, &probe);
+      e2 = cudaOccupancyMaxPotentialClusterSize(&max_size, varlen_prefill_kernel<kPaged, kShape, kWindow, T16>, &probe);
       cudaGetLastError();
     }
     return err("prefill launch (shape %d, grid %u x %u x %u, %d threads, %d bytes of shared memory) failed: %s "
@@ -976,6 +1078,19 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
                cudaGetErrorString(e1), max_size, cudaGetErrorString(e2));
   }
   return nullptr;
+}
+
+// Windowed variant.  A query tile visits window / 128 + 1 key tiles and the sinks' tiles: by that length
+// and not the sequence's a call takes shape 1 or 2; two tiles of a CTA are two heads of one kv head.
+template <bool kPaged, typename T16>
+static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
+                                   const OutMaps &to, PrefillParams &p, int num_heads, int batch, int max_seqlen_q,
+                                   int max_seqlen_k, cudaStream_t stream) {
+  p.pair_heads = 0;
+  const int64_t keys = (int64_t)p.window + p.sinks;
+  if (p.group % 2 != 0 || (keys < max_seqlen_k ? keys : max_seqlen_k) <= AICI_PREFILL_ONE_TILE_MAX_K)
+    return launch_prefill_shape<kPaged, 1, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
+  return launch_prefill_shape<kPaged, 2, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
 }
 
 // Which shape a call takes.  `forced` = 0: by sequence length -- shape 1 up to
@@ -1011,6 +1126,20 @@ static char *launch_prefill(int shape, const CUtensorMap &tq, const CUtensorMap 
 
 using namespace aici;
 
+// What the windowed entry points take besides the arguments of the others.
+struct WindowArgs {
+  int window, sinks;
+};
+
+static char *check_window(const char *fn, const WindowArgs &w, int num_heads, int num_kv_heads, int dtype) {
+  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn, dtype);
+  AICI_CHECK(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,
+             "%s: num_heads %d not divisible by num_kv_heads %d", fn, num_heads, num_kv_heads);
+  AICI_CHECK(w.window >= 1, "%s: window must be at least 1 (got %d)", fn, w.window);
+  AICI_CHECK(w.sinks >= 0, "%s: sinks must not be negative (got %d)", fn, w.sinks);
+  return nullptr;
+}
+
 static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, int out_head0, const void *q,
                                  const void *k, const void *v,
                                      const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
@@ -1021,12 +1150,16 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
                                      int64_t v_tok_stride, int64_t v_head_stride,
                                      int64_t o_tok_stride, int64_t o_head_stride,
                                      float softmax_scale, int is_causal, int dtype,
-                                     aici_stream_t stream, int forced_shape = 0) {
+                                     aici_stream_t stream, int forced_shape = 0,
+                                     const WindowArgs *win = nullptr) {
   void *out = outs[0];
   for (int w = 1; w < world; ++w)
     AICI_CHECK(outs[w] != nullptr && (uintptr_t)outs[w] % 16 == 0,
                "%s: peer output %d must be non-NULL and 16-byte aligned", fn, w);
-  AICI_CHECK(dtype == AICI_DTYPE_BF16, "%s: FlashAttention only support bf16 data type (dtype=%d)", fn, dtype);
+  if (win != nullptr) {
+    if (char *e = check_window(fn, *win, num_heads, num_heads_k, dtype)) return e;
+  }
+  AICI_CHECK(win != nullptr || dtype == AICI_DTYPE_BF16, "%s: FlashAttention only support bf16 data type (dtype=%d)", fn, dtype);
   AICI_CHECK(batch > 0, "%s: batch size must be positive", fn);
   AICI_CHECK(head_size == kHD, "%s: head_size must be 128 (got %d)", fn, head_size);
   AICI_CHECK(num_heads > 0 && num_heads_k > 0 && num_heads % num_heads_k == 0,
@@ -1081,6 +1214,8 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   p.k_lens = nullptr;
   p.max_blocks = 0;
   p.num_blocks = 0;
+  p.window = win ? win->window : 0;
+  p.sinks = win ? win->sinks : 0;
   // every output buffer gets a tensor map like the query's; this rank's heads start at out_head0
   OutMaps to = {};
   p.total_q = total_q;
@@ -1088,6 +1223,11 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   for (int w = 0; w < world; ++w)  // the kernel reads m[w] for w < world only
     if (char *e = make_tmap(fn, &to.m[w], outs[w], total_q, out_head0 + num_heads, o_tok_stride, o_head_stride))
       return e;
+  if (win != nullptr)
+    return with_half_type(dtype, [&](auto t) {
+      return launch_prefill_window<false, decltype(t)>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, max_seqlen_k,
+                                                       static_cast<cudaStream_t>(stream));
+    });
   return launch_prefill<false>(shape, tq, tk, tv, to, p, num_heads, batch, max_seqlen_q,
                                static_cast<cudaStream_t>(stream));
 }
@@ -1155,19 +1295,21 @@ extern "C" char *aici_mha_varlen_fwd_peers(void *const *outs, int world, int hea
                              stream);
 }
 
-extern "C" char *aici_mha_varlen_paged_fwd(void *out, const void *q, const void *key_cache,
-                                           const void *value_cache, const int32_t *cu_seqlens_q,
-                                           const int32_t *context_lens, const int32_t *block_tables,
-                                           int batch, int total_q, int num_heads, int num_kv_heads,
-                                           int head_size, int block_size, int max_seqlen_q,
-                                           int max_context_len, int max_num_blocks_per_seq,
-                                           int64_t num_blocks, int64_t q_tok_stride,
-                                           int64_t q_head_stride, int64_t o_tok_stride,
-                                           int64_t o_head_stride, int64_t kv_block_stride,
-                                           int64_t kv_head_stride, float softmax_scale, int is_causal,
-                                           int dtype, aici_stream_t stream) {
-  const char *fn = "aici_mha_varlen_paged_fwd";
-  AICI_CHECK(dtype == AICI_DTYPE_BF16, "%s: only bf16 is supported (dtype=%d)", fn, dtype);
+static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q, const void *key_cache,
+                                       const void *value_cache, const int32_t *cu_seqlens_q,
+                                       const int32_t *context_lens, const int32_t *block_tables,
+                                       int batch, int total_q, int num_heads, int num_kv_heads,
+                                       int head_size, int block_size, int max_seqlen_q,
+                                       int max_context_len, int max_num_blocks_per_seq,
+                                       int64_t num_blocks, int64_t q_tok_stride,
+                                       int64_t q_head_stride, int64_t o_tok_stride,
+                                       int64_t o_head_stride, int64_t kv_block_stride,
+                                       int64_t kv_head_stride, float softmax_scale, int is_causal,
+                                       int dtype, aici_stream_t stream, const WindowArgs *win = nullptr) {
+  if (win != nullptr) {
+    if (char *e = check_window(fn, *win, num_heads, num_kv_heads, dtype)) return e;
+  }
+  AICI_CHECK(win != nullptr || dtype == AICI_DTYPE_BF16, "%s: only bf16 is supported (dtype=%d)", fn, dtype);
   AICI_CHECK(batch > 0, "%s: batch size must be positive", fn);
   AICI_CHECK(head_size == kHD, "%s: head_size must be 128 (got %d)", fn, head_size);
   AICI_CHECK(block_size == 16, "%s: block_size must be 16 (got %d)", fn, block_size);
@@ -1216,12 +1358,72 @@ extern "C" char *aici_mha_varlen_paged_fwd(void *out, const void *q, const void 
   p.k_lens = context_lens;
   p.max_blocks = max_num_blocks_per_seq;
   p.num_blocks = num_blocks;
+  p.window = win ? win->window : 0;
+  p.sinks = win ? win->sinks : 0;
   OutMaps to = {};
   p.total_q = total_q;
   p.tma_store = 1;
   if (char *e = make_tmap(fn, &to.m[0], out, total_q, num_heads, o_tok_stride, o_head_stride)) return e;
+  if (win != nullptr)
+    return with_half_type(dtype, [&](auto t) {
+      return launch_prefill_window<true, decltype(t)>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, max_context_len,
+                                                      static_cast<cudaStream_t>(stream));
+    });
   int shape = 0;
   if (char *e = pick_shape(fn, 0, true, num_heads, num_heads / num_kv_heads, max_context_len, &shape)) return e;
   return launch_prefill<true>(shape, tq, tk, tv, to, p, num_heads, batch, max_seqlen_q,
                               static_cast<cudaStream_t>(stream));
+}
+
+extern "C" char *aici_mha_varlen_paged_fwd(void *out, const void *q, const void *key_cache,
+                                           const void *value_cache, const int32_t *cu_seqlens_q,
+                                           const int32_t *context_lens, const int32_t *block_tables,
+                                           int batch, int total_q, int num_heads, int num_kv_heads,
+                                           int head_size, int block_size, int max_seqlen_q,
+                                           int max_context_len, int max_num_blocks_per_seq,
+                                           int64_t num_blocks, int64_t q_tok_stride,
+                                           int64_t q_head_stride, int64_t o_tok_stride,
+                                           int64_t o_head_stride, int64_t kv_block_stride,
+                                           int64_t kv_head_stride, float softmax_scale, int is_causal,
+                                           int dtype, aici_stream_t stream) {
+  return mha_varlen_paged_fwd_impl("aici_mha_varlen_paged_fwd", out, q, key_cache, value_cache, cu_seqlens_q,
+                                   context_lens, block_tables, batch, total_q, num_heads, num_kv_heads, head_size,
+                                   block_size, max_seqlen_q, max_context_len, max_num_blocks_per_seq, num_blocks,
+                                   q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
+                                   kv_head_stride, softmax_scale, is_causal, dtype, stream);
+}
+
+// ---- sliding window and sinks ------------------------------------------------------------------------
+extern "C" char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
+                                            const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
+                                            int total_q, int total_k, int num_heads, int num_heads_k, int head_size,
+                                            int max_seqlen_q, int max_seqlen_k, int window, int sinks,
+                                            int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride,
+                                            int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                                            int64_t o_tok_stride, int64_t o_head_stride, float softmax_scale,
+                                            int dtype, aici_stream_t stream) {
+  void *outs[1] = {out};
+  const WindowArgs win = {window, sinks};
+  return mha_varlen_fwd_impl("aici_mha_varlen_window_fwd", outs, 1, 0, q, k, v, cu_seqlens_q, cu_seqlens_k, batch,
+                             total_q, total_k, num_heads, num_heads_k, head_size, max_seqlen_q, max_seqlen_k,
+                             q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride,
+                             o_tok_stride, o_head_stride, softmax_scale, 1, dtype, stream, 0, &win);
+}
+
+extern "C" char *aici_mha_varlen_paged_window_fwd(void *out, const void *q, const void *key_cache,
+                                                  const void *value_cache, const int32_t *cu_seqlens_q,
+                                                  const int32_t *context_lens, const int32_t *block_tables, int batch,
+                                                  int total_q, int num_heads, int num_kv_heads, int head_size,
+                                                  int block_size, int max_seqlen_q, int max_context_len,
+                                                  int max_num_blocks_per_seq, int64_t num_blocks, int window,
+                                                  int sinks, int64_t q_tok_stride, int64_t q_head_stride,
+                                                  int64_t o_tok_stride, int64_t o_head_stride,
+                                                  int64_t kv_block_stride, int64_t kv_head_stride,
+                                                  float softmax_scale, int dtype, aici_stream_t stream) {
+  const WindowArgs win = {window, sinks};
+  return mha_varlen_paged_fwd_impl("aici_mha_varlen_paged_window_fwd", out, q, key_cache, value_cache, cu_seqlens_q,
+                                   context_lens, block_tables, batch, total_q, num_heads, num_kv_heads, head_size,
+                                   block_size, max_seqlen_q, max_context_len, max_num_blocks_per_seq, num_blocks,
+                                   q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
+                                   kv_head_stride, softmax_scale, 1, dtype, stream, &win);
 }

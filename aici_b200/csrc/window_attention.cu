@@ -176,104 +176,3 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
   p.status = st;
   return launch_window(p, true, 1, dtype, static_cast<cudaStream_t>(stream));
 }
-
-static char *window_fwd(const char *fn, WindowParams p, bool paged, int max_seqlen_q, int dtype, aici_stream_t stream) {
-  if (char *e = check_on_current_device(fn, "q", p.q)) return e;
-  p.status = status_ptr();
-  AICI_CHECK(p.status != nullptr, "%s: no CUDA device", fn);
-  return launch_window(p, paged, max_seqlen_q, dtype, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
-                                            const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
-                                            int total_q, int total_k, int num_heads, int num_heads_k, int head_size,
-                                            int max_seqlen_q, int max_seqlen_k, int window, int sinks,
-                                            int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride,
-                                            int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride,
-                                            int64_t o_tok_stride, int64_t o_head_stride, float softmax_scale,
-                                            int dtype, aici_stream_t stream) {
-  const char *fn = "aici_mha_varlen_window_fwd";
-  if (char *e = check_window(fn, window, sinks, num_heads, num_heads_k, head_size, softmax_scale, dtype)) return e;
-  AICI_CHECK(batch > 0 && batch <= 65535 && num_heads <= 65535, "%s: batch and num_heads must fit a grid dimension", fn);
-  AICI_CHECK(total_q >= 0 && total_k >= 0 && max_seqlen_q >= 0 && max_seqlen_k >= 0, "%s: negative size", fn);
-  const int64_t strides[8] = {q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
-                              v_tok_stride, v_head_stride, o_tok_stride, o_head_stride};
-  for (int i = 0; i < 8; ++i)
-    AICI_CHECK(strides[i] >= kWinHead && strides[i] % 8 == 0,
-               "%s: token and head strides must be multiples of 8 elements and at least head_size", fn);
-  if (total_q == 0 || max_seqlen_q == 0) return nullptr;
-  AICI_CHECK(out && q && cu_seqlens_q && cu_seqlens_k && (total_k == 0 || (k && v)), "%s: NULL pointer", fn);
-  AICI_CHECK(((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0,
-             "%s: tensors must be 16-byte aligned", fn);
-  WindowParams p = {};
-  p.out = out;
-  p.q = q;
-  p.k = k;
-  p.v = v;
-  p.cu_q = cu_seqlens_q;
-  p.cu_k = cu_seqlens_k;
-  p.batch = batch;
-  p.num_heads = num_heads;
-  p.group = num_heads / num_heads_k;
-  p.window = window;
-  p.sinks = sinks;
-  p.q_tok = q_tok_stride;
-  p.q_head = q_head_stride;
-  p.k_tok = k_tok_stride;
-  p.k_head = k_head_stride;
-  p.v_tok = v_tok_stride;
-  p.v_head = v_head_stride;
-  p.o_tok = o_tok_stride;
-  p.o_head = o_head_stride;
-  p.scale = softmax_scale;
-  return window_fwd(fn, p, false, max_seqlen_q, dtype, stream);
-}
-
-extern "C" char *aici_mha_varlen_paged_window_fwd(void *out, const void *q, const void *key_cache,
-                                                  const void *value_cache, const int32_t *cu_seqlens_q,
-                                                  const int32_t *context_lens, const int32_t *block_tables, int batch,
-                                                  int total_q, int num_heads, int num_kv_heads, int head_size,
-                                                  int block_size, int max_seqlen_q, int max_context_len,
-                                                  int max_num_blocks_per_seq, int64_t num_blocks, int window,
-                                                  int sinks, int64_t q_tok_stride, int64_t q_head_stride,
-                                                  int64_t o_tok_stride, int64_t o_head_stride,
-                                                  int64_t kv_block_stride, int64_t kv_head_stride,
-                                                  float softmax_scale, int dtype, aici_stream_t stream) {
-  const char *fn = "aici_mha_varlen_paged_window_fwd";
-  if (char *e = check_window(fn, window, sinks, num_heads, num_kv_heads, head_size, softmax_scale, dtype)) return e;
-  if (char *e = check_cache(fn, block_size, num_blocks, num_kv_heads, kv_block_stride, kv_head_stride)) return e;
-  AICI_CHECK(batch > 0 && batch <= 65535 && num_heads <= 65535, "%s: batch and num_heads must fit a grid dimension", fn);
-  AICI_CHECK(total_q >= 0 && max_seqlen_q >= 0 && max_context_len >= 0 && max_num_blocks_per_seq >= 0,
-             "%s: negative size", fn);
-  const int64_t strides[4] = {q_tok_stride, q_head_stride, o_tok_stride, o_head_stride};
-  for (int i = 0; i < 4; ++i)
-    AICI_CHECK(strides[i] >= kWinHead && strides[i] % 8 == 0,
-               "%s: token and head strides must be multiples of 8 elements and at least head_size", fn);
-  if (total_q == 0 || max_seqlen_q == 0) return nullptr;
-  AICI_CHECK(out && q && key_cache && value_cache && cu_seqlens_q && context_lens && block_tables, "%s: NULL pointer", fn);
-  AICI_CHECK(((uintptr_t)out | (uintptr_t)q | (uintptr_t)key_cache | (uintptr_t)value_cache) % 16 == 0,
-             "%s: tensors must be 16-byte aligned", fn);
-  WindowParams p = {};
-  p.out = out;
-  p.q = q;
-  p.k = key_cache;
-  p.v = value_cache;
-  p.cu_q = cu_seqlens_q;
-  p.k_lens = context_lens;
-  p.block_tables = block_tables;
-  p.batch = batch;
-  p.num_heads = num_heads;
-  p.group = num_heads / num_kv_heads;
-  p.window = window;
-  p.sinks = sinks;
-  p.max_blocks = max_num_blocks_per_seq;
-  p.max_context = max_context_len;
-  p.num_blocks = num_blocks;
-  p.q_tok = q_tok_stride;
-  p.q_head = q_head_stride;
-  p.o_tok = o_tok_stride;
-  p.o_head = o_head_stride;
-  p.kv_block = kv_block_stride;
-  p.scale = softmax_scale;
-  return window_fwd(fn, p, true, max_seqlen_q, dtype, stream);
-}
