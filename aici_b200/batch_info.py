@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import AiciError
-from .tch_cuda import _on_device, _raw_stream
+from .tch_cuda import _call, _one_gpu
 
 PAGED_DECODE = 1
 TABLES_FOR_ALL = 2
@@ -202,28 +202,25 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     (lengths, tokens, free blocks) changes nothing and sets a status bit (see _lib.last_status).
     Returns a StepTables."""
     fn = "step_tables"
-    for t in (query_lens, context_lens, block_tables, free_blocks, free_count):
-        if not t.is_cuda:
-            raise AiciError("%s: tensor must be on a CUDA device (there is no CPU path)" % fn)
-        if t.device != query_lens.device:
-            raise AiciError("%s: tensors are on different devices" % fn)
-        if t.dtype != torch.int32:
+    given = (query_lens, context_lens, block_tables, free_blocks, free_count)
+    index = _one_gpu(fn, given)
+    for t in given:
+        if t.dtype is not torch.int32:
             raise AiciError("%s: lengths, tables and free list must be int32" % fn)
+        if not t.is_contiguous() and t is not block_tables:
+            raise AiciError("%s: lengths and free list must be contiguous" % fn)
     n = query_lens.numel()
     if query_lens.dim() != 1 or context_lens.shape != query_lens.shape or free_blocks.dim() != 1 or \
-            free_count.numel() != 1 or not query_lens.is_contiguous() or not context_lens.is_contiguous() or \
-            not free_blocks.is_contiguous():
-        raise AiciError("%s: query_lens and context_lens must be contiguous [requests], free_blocks contiguous "
-                        "[blocks], free_count [1]" % fn)
-    if block_tables.dim() != 2 or block_tables.shape[0] != n or block_tables.stride(1) != 1:
+            free_count.numel() != 1:
+        raise AiciError("%s: query_lens and context_lens must be [requests], free_blocks [blocks], free_count [1]" % fn)
+    table, rows = block_tables.shape, block_tables.stride()
+    if len(table) != 2 or table[0] != n or rows[1] != 1:
         raise AiciError("%s: block_tables must be [requests, max_blocks] with contiguous rows" % fn)
-    dev = query_lens.device
     if out is None:
         # one allocation; the token tensors first, for their alignment
         T4 = (max_tokens + 3) // 4 * 4
-        buf = torch.empty(3 * T4 + 3 * n + 2, dtype=torch.int32, device=dev)
-        positions, slots, seqlens, logits, context, count, _ = buf.split_with_sizes(
-            (2 * T4, T4, n + 1, n, n, 1, 0))
+        buf = torch.empty(3 * T4 + 3 * n + 2, dtype=torch.int32, device=query_lens.device)
+        positions, slots, seqlens, logits, context, count = buf.split_with_sizes((2 * T4, T4, n + 1, n, n, 1))
         positions = positions.view(torch.int64)
         if T4 != max_tokens:
             positions, slots = positions[:max_tokens], slots[:max_tokens]
@@ -232,13 +229,10 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
         for t, count, dtype in ((out.seqlens_q, n + 1, torch.int32), (out.positions, max_tokens, torch.int64),
                                 (out.slot_mapping, max_tokens, torch.int32), (out.logit_idxs, n, torch.int32),
                                 (out.context_lens, n, torch.int32), (out.free_count, 1, torch.int32)):
-            if t.device != dev or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+            if t.get_device() != index or t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
                 raise AiciError("%s: out does not match the call (device, types or sizes)" % fn)
-    with _on_device(dev):
-        _lib.check(fn, _lib.lib().aici_step_tables(
-            query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(),
-            free_count.data_ptr(), n, block_tables.shape[1], block_tables.stride(0), free_blocks.numel(),
-            num_blocks, block_size, max_tokens, out.seqlens_q.data_ptr(), out.positions.data_ptr(),
-            out.slot_mapping.data_ptr(), out.logit_idxs.data_ptr(), out.context_lens.data_ptr(),
-            out.free_count.data_ptr(), _raw_stream(dev)))
+    _call(fn, "aici_step_tables", index, query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
+          free_blocks.data_ptr(), free_count.data_ptr(), n, table[1], rows[0] if n > 1 else table[1],
+          free_blocks.numel(), num_blocks, block_size, max_tokens, out.seqlens_q.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(),
+          out.logit_idxs.data_ptr(), out.context_lens.data_ptr(), out.free_count.data_ptr())
     return out

@@ -9,9 +9,10 @@
 // follows the reference kernel, which rounds every product).
 //
 // Everything here is data movement with a handful of operations per 16 bytes.  A unit of work is a
-// "chunk": 8 pairs = two 16-byte vectors of a head (half: chunk c of each half; interleaved: 16
-// neighbouring elements) with their 8 cosines and 8 sines, so every access is a whole vector whatever
-// the layout; it asks for rot_dim to be a multiple of 16.
+// "chunk": the two 16-byte vectors at elements 8 c and rot_dim / 2 + 8 c of a head, which hold 8 pairs
+// in either layout (half: one across the vectors; interleaved: four inside each), with their 8 cosines
+// and 8 sines.  So every access is a whole vector and neighbouring threads take neighbouring vectors; it
+// asks for rot_dim to be a multiple of 16.
 #include <math.h>
 
 #include "half_types.cuh"
@@ -23,6 +24,13 @@ constexpr int kRotTok = 16;      // tokens of a cache-writing CTA: one cache blo
 constexpr int kRotBlock = 16;    // tokens of a cache block
 constexpr int kMaxHead = 256;
 
+// How the threads of a CTA share out the heads of whole tokens: thread = (token, head slot, chunk),
+// chunk fastest, so that a warp reads runs of a row; a thread takes every slots-th head of its token.
+struct HeadPlan {
+  int slots, tokens;  // head slots, tokens of a CTA at a time
+  int ctas;           // CTA i takes the i-th, (i + ctas)-th, ... such run of tokens
+};
+
 struct RotaryParams {
   const int64_t *positions;
   void *query, *key;
@@ -31,23 +39,30 @@ struct RotaryParams {
   int num_tokens, num_heads, num_kv_heads, head_size, rot_dim, slot_is_int64;
   int64_t max_position, num_slots, query_stride, key_stride, value_stride;
   unsigned int *status;
+  HeadPlan q_plan, k_plan;
+  int kv_heads_per_cta;  // cache-writing CTAs: heads of one, one after the other
 };
 
-__device__ __forceinline__ void load8(const float *src, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+// Four neighbouring table entries.
+__device__ __forceinline__ void load4(const float *src, float *x) {
+  const float4 a = *reinterpret_cast<const float4 *>(src);
   x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
-  const uint4 v = *reinterpret_cast<const uint4 *>(src);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Half16<T>::unpack(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ void load4(const T *src, float *x) {
+  const uint2 v = *reinterpret_cast<const uint2 *>(src);
+  const float2 a = Half16<T>::unpack(v.x), b = Half16<T>::unpack(v.y);
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+}
+// Cosines and sines of chunk c from a row of the table: pairs 8 c .. 8 c + 7 (half), or 4 c .. 4 c + 3 and
+// those rot_dim / 4 further on (interleaved).
+template <typename C, bool kNeox>
+__device__ __forceinline__ void load_turn(const C *row, int rot_dim, int c, float (&co)[8], float (&si)[8]) {
+  const int a = kNeox ? 8 * c : 4 * c, b = kNeox ? a + 4 : a + rot_dim / 4;
+  load4(row + a, co);
+  load4(row + b, co + 4);
+  load4(row + rot_dim / 2 + a, si);
+  load4(row + rot_dim / 2 + b, si + 4);
 }
 
 // Turns one chunk: xv, yv are its two vectors, c and s its cosines and sines.
@@ -73,145 +88,203 @@ __device__ __forceinline__ void turn(uint4 &xv, uint4 &yv, const float (&c)[8], 
   yv = make_uint4(y[0], y[1], y[2], y[3]);
 }
 
-// The heads of one token, turned in place: threads along (head, chunk), chunk fastest, so a warp reads
-// whole rows and the cosines and sines come out of the L1.
+// CTA `cta` of the plan: turns the heads of its tokens in place.  What bounds it is the chain position ->
+// table row -> store: the position of a thread's next token is fetched a round ahead, so that in all
+// rounds but the first the table row and four heads' vectors travel together.
 template <typename T, typename C, bool kNeox>
-__device__ __forceinline__ void turn_heads(T *row, int heads, const C *cs, const RotaryParams &p, int tid) {
+__device__ __forceinline__ void turn_heads(T *rows, int64_t row_stride, int heads, const HeadPlan &plan, int cta,
+                                           const RotaryParams &p) {
+  constexpr int kAhead = 4;
   const int nc = p.rot_dim / 16;  // chunks of a head
-  const int second = kNeox ? p.rot_dim / 2 : 8;
-  for (int i = tid; i < heads * nc; i += kRotThreads) {
-    const int h = i / nc, c = i - h * nc;
-    T *x = row + (int64_t)h * p.head_size + c * (kNeox ? 8 : 16);
-    uint4 xv = *reinterpret_cast<const uint4 *>(x), yv = *reinterpret_cast<const uint4 *>(x + second);
-    float co[8], si[8];
-    load8(cs + c * 8, co);
-    load8(cs + p.rot_dim / 2 + c * 8, si);
-    turn<T, kNeox>(xv, yv, co, si);
-    *reinterpret_cast<uint4 *>(x) = xv;
-    *reinterpret_cast<uint4 *>(x + second) = yv;
+  const int c = threadIdx.x % nc, rest = threadIdx.x / nc, slot = rest % plan.slots, tok = rest / plan.slots;
+  if (tok >= plan.tokens) return;
+  const int second = p.rot_dim / 2, stride = plan.ctas * plan.tokens;
+  int t = cta * plan.tokens + tok;
+  int64_t pos = t < p.num_tokens ? p.positions[t] : 0;
+  for (; t < p.num_tokens; t += stride) {
+    const int64_t next = t + stride < p.num_tokens ? p.positions[t + stride] : 0;
+    if (pos >= 0 && pos < p.max_position) {
+      T *x = rows + t * row_stride + c * 8;
+      float co[8], si[8];
+      for (int h0 = slot; h0 < heads; h0 += kAhead * plan.slots) {
+        uint4 xv[kAhead], yv[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int h = h0 + k * plan.slots;
+          if (h < heads) {
+            xv[k] = *reinterpret_cast<const uint4 *>(x + (int64_t)h * p.head_size);
+            yv[k] = *reinterpret_cast<const uint4 *>(x + (int64_t)h * p.head_size + second);
+          }
+        }
+        if (h0 == slot)
+          load_turn<C, kNeox>(static_cast<const C *>(p.table) + pos * p.rot_dim, p.rot_dim, c, co, si);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int h = h0 + k * plan.slots;
+          if (h < heads) {
+            turn<T, kNeox>(xv[k], yv[k], co, si);
+            *reinterpret_cast<uint4 *>(x + (int64_t)h * p.head_size) = xv[k];
+            *reinterpret_cast<uint4 *>(x + (int64_t)h * p.head_size + second) = yv[k];
+          }
+        }
+      }
+    } else {  // the token stays as it is
+      set_status(p.status, AICI_STATUS_BAD_SLOT);
+    }
+    pos = next;
   }
-}
-
-// One CTA to a token: query heads, and the key heads behind them.
-template <typename T, typename C, bool kNeox>
-__device__ __forceinline__ void rotate_token(const RotaryParams &p, int t, bool with_key) {
-  const int64_t pos = p.positions[t];
-  if (pos < 0 || pos >= p.max_position) {  // the token stays as it is
-    if (threadIdx.x == 0) set_status(p.status, AICI_STATUS_BAD_SLOT);
-    return;
-  }
-  const C *cs = static_cast<const C *>(p.table) + pos * p.rot_dim;
-  turn_heads<T, C, kNeox>(static_cast<T *>(p.query) + t * p.query_stride, p.num_heads, cs, p, threadIdx.x);
-  if (with_key)
-    turn_heads<T, C, kNeox>(static_cast<T *>(p.key) + t * p.key_stride, p.num_kv_heads, cs, p, threadIdx.x);
 }
 
 template <typename T, typename C, bool kNeox>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryParams p) {
-  rotate_token<T, C, kNeox>(p, blockIdx.x, true);
+  const int b = blockIdx.x;
+  if (b < p.q_plan.ctas)
+    turn_heads<T, C, kNeox>(static_cast<T *>(p.query), p.query_stride, p.num_heads, p.q_plan, b, p);
+  else
+    turn_heads<T, C, kNeox>(static_cast<T *>(p.key), p.key_stride, p.num_kv_heads, p.k_plan, b - p.q_plan.ctas, p);
 }
 
-// With the cache write.  The first CTAs take 16 tokens of one kv head each: the key is turned, put
-// back and written to the cache, the value goes through shared memory because the cache keeps it
-// transposed ([d][token]).  The CTAs behind them turn the query heads, one token each.
-template <typename T, typename C, bool kNeox>
+__device__ __forceinline__ void copy_async16(void *dst_smem, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst_smem)), "l"(src) : "memory");
+}
+
+// With the cache write.  The first CTAs take 16 tokens and some kv heads each, one head after the other:
+// the key is turned, put back and written to the cache, the value goes through shared memory because the
+// cache keeps it transposed ([d][token]).  The CTAs behind them turn the query heads.  Where a token goes
+// and how far it turns does not change what is read: the first head's keys and values are on their way
+// before slots and positions have arrived, and each head's while the one before it is worked on.  A
+// thread keeps its token's cosines and sines for all its heads.
+// kUnits: vectors of a key head that a thread handles (2 only for heads of more than 128 elements).
+template <typename T, typename C, bool kNeox, int kUnits>
 __global__ void __launch_bounds__(kRotThreads) rotary_cache_kernel(const RotaryParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
   const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
-  if (blockIdx.x >= (unsigned)(tiles * p.num_kv_heads)) {
-    rotate_token<T, C, kNeox>(p, blockIdx.x - tiles * p.num_kv_heads, false);
+  const int groups = (p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta;
+  if (blockIdx.x >= (unsigned)(tiles * groups)) {
+    turn_heads<T, C, kNeox>(static_cast<T *>(p.query), p.query_stride, p.num_heads, p.q_plan, blockIdx.x - tiles * groups, p);
     return;
   }
-  __shared__ int64_t s_slot[kRotTok], s_pos[kRotTok];
-  __shared__ __align__(16) T s_v[kRotTok][kMaxHead + 8];
-  const int h = blockIdx.x % p.num_kv_heads, t0 = blockIdx.x / p.num_kv_heads * kRotTok;
-  const int tid = threadIdx.x, D = p.head_size;
+  __shared__ int64_t s_slot[kRotTok];
+  const int h_begin = blockIdx.x % groups * p.kv_heads_per_cta, h_end = min(h_begin + p.kv_heads_per_cta, p.num_kv_heads);
+  const int t0 = blockIdx.x / groups * kRotTok;
+  const int tid = threadIdx.x, D = p.head_size, pitch = D + 8;
   const int tokens = min(kRotTok, p.num_tokens - t0);
-  if (tid < kRotTok) {
-    int64_t slot = -1, pos = -1;
-    if (tid < tokens) {
-      slot = p.slot_is_int64 ? static_cast<const int64_t *>(p.slots)[t0 + tid]
-                             : (int64_t) static_cast<const int32_t *>(p.slots)[t0 + tid];
-      if (slot >= p.num_slots) {
-        set_status(p.status, AICI_STATUS_BAD_SLOT);
-        slot = -1;
-      }
-      pos = p.positions[t0 + tid];
-      if (pos < 0 || pos >= p.max_position) {  // the token stays as it is and is not written
-        set_status(p.status, AICI_STATUS_BAD_SLOT);
-        pos = -1;
-        slot = -1;
-      }
+  auto buffer = [&](int h) { return reinterpret_cast<T *>(smem) + ((h - h_begin) & 1) * (kRotTok * pitch); };  // [16][D + 8]
+  auto fetch_value = [&](int h) {
+    T *dst = buffer(h);
+    for (int i = tid; i < tokens * (D / 8); i += kRotThreads) {
+      const int tok = i / (D / 8), c = i - tok * (D / 8);
+      copy_async16(dst + tok * pitch + c * 8,
+                   static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + (int64_t)h * D + c * 8);
     }
-    s_slot[tid] = slot;
-    s_pos[tid] = pos;
-  }
-  for (int i = tid; i < tokens * (D / 8); i += kRotThreads) {
-    const int tok = i / (D / 8), c = i - tok * (D / 8);
-    *reinterpret_cast<uint4 *>(&s_v[tok][c * 8]) = *reinterpret_cast<const uint4 *>(
-        static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + (int64_t)h * D + c * 8);
-  }
-  __syncthreads();
-
-  // keys: 16 consecutive threads take the 16 tokens of one chunk, so that the cache sees runs of 256
-  // bytes.  The chunks behind rot_dim are copied.
-  const int nc = p.rot_dim / 16, rest = (D - p.rot_dim) / 8;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // keys: 16 consecutive threads take the 16 tokens of one unit, so that the cache sees runs of 256
+  // bytes.  Units are the chunks, then the vectors behind rot_dim.
+  const int nc = p.rot_dim / 16, units = nc + (D - p.rot_dim) / 8;
   const int tok = tid & (kRotTok - 1);
-  if (tok < tokens && s_pos[tok] >= 0) {
-    T *k = static_cast<T *>(p.key) + (t0 + tok) * p.key_stride + (int64_t)h * D;
-    const C *cs = static_cast<const C *>(p.table) + s_pos[tok] * p.rot_dim;
-    const int64_t slot = s_slot[tok];
-    T *kc = static_cast<T *>(p.key_cache) +
-            (slot >= 0 ? (slot / kRotBlock * p.num_kv_heads + h) * D * kRotBlock + slot % kRotBlock * 8 : 0);
-    for (int c = tid / kRotTok; c < nc + rest; c += kRotThreads / kRotTok) {
-      if (c < nc) {
-        const int e0 = kNeox ? c * 8 : c * 16, e1 = e0 + (kNeox ? p.rot_dim / 2 : 8);
-        uint4 xv = *reinterpret_cast<const uint4 *>(k + e0), yv = *reinterpret_cast<const uint4 *>(k + e1);
-        float co[8], si[8];
-        load8(cs + c * 8, co);
-        load8(cs + p.rot_dim / 2 + c * 8, si);
-        turn<T, kNeox>(xv, yv, co, si);
-        *reinterpret_cast<uint4 *>(k + e0) = xv;
-        *reinterpret_cast<uint4 *>(k + e1) = yv;
-        if (slot >= 0) {
-          *reinterpret_cast<uint4 *>(kc + e0 * kRotBlock) = xv;  // vector e / 8 of the head: 16 tokens x 8 elements each
-          *reinterpret_cast<uint4 *>(kc + e1 * kRotBlock) = yv;
+  const bool mine = tok < tokens;
+  T *key = static_cast<T *>(p.key) + (t0 + tok) * p.key_stride;
+  int unit[kUnits], e0[kUnits], e1[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    unit[i] = tid / kRotTok + i * (kRotThreads / kRotTok);
+    e0[i] = unit[i] < nc ? unit[i] * 8 : p.rot_dim + (unit[i] - nc) * 8;
+    e1[i] = e0[i] + p.rot_dim / 2;
+  }
+  uint4 xv[kUnits], yv[kUnits];
+  auto fetch_key = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i)
+      if (mine && unit[i] < units) {
+        xv[i] = *reinterpret_cast<const uint4 *>(key + (int64_t)h * D + e0[i]);
+        if (unit[i] < nc) yv[i] = *reinterpret_cast<const uint4 *>(key + (int64_t)h * D + e1[i]);
+      }
+  };
+  fetch_value(h_begin);
+  fetch_key(h_begin);
+  int64_t slot = -1, pos = -1;
+  if (mine) {
+    slot = p.slot_is_int64 ? static_cast<const int64_t *>(p.slots)[t0 + tok]
+                           : (int64_t) static_cast<const int32_t *>(p.slots)[t0 + tok];
+    pos = p.positions[t0 + tok];
+    const bool bad_pos = pos < 0 || pos >= p.max_position;  // the token stays as it is and is not written
+    if (bad_pos || slot >= p.num_slots) {
+      set_status(p.status, AICI_STATUS_BAD_SLOT);
+      slot = -1;
+      if (bad_pos) pos = -1;
+    }
+  }
+  if (tid < kRotTok) s_slot[tid] = slot;
+  float co[kUnits][8], si[kUnits][8];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i)
+    if (pos >= 0 && unit[i] < nc)
+      load_turn<C, kNeox>(static_cast<const C *>(p.table) + pos * p.rot_dim, p.rot_dim, unit[i], co[i], si[i]);
+  T *kc = static_cast<T *>(p.key_cache) +
+          (slot >= 0 ? slot / kRotBlock * p.num_kv_heads * D * kRotBlock + slot % kRotBlock * 8 : 0);
+  T *vc = static_cast<T *>(p.value_cache);
+  uint32_t runs = 0;
+
+  for (int h = h_begin; h < h_end; ++h) {
+    uint4 x[kUnits], y[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      x[i] = xv[i];
+      y[i] = yv[i];
+    }
+    if (h + 1 < h_end) {
+      fetch_value(h + 1);
+      fetch_key(h + 1);
+    }
+    if (pos >= 0) {
+      T *to = kc + (int64_t)h * D * kRotBlock;  // vector e / 8 of the head: 16 tokens x 8 elements
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        if (unit[i] < nc) {
+          turn<T, kNeox>(x[i], y[i], co[i], si[i]);
+          *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e0[i]) = x[i];
+          *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e1[i]) = y[i];
         }
-      } else if (slot >= 0) {
-        const int e = p.rot_dim + (c - nc) * 8;
-        *reinterpret_cast<uint4 *>(kc + e * kRotBlock) = *reinterpret_cast<const uint4 *>(k + e);
+        if (slot >= 0 && unit[i] < units) {
+          *reinterpret_cast<uint4 *>(to + e0[i] * kRotBlock) = x[i];
+          if (unit[i] < nc) *reinterpret_cast<uint4 *>(to + e1[i] * kRotBlock) = y[i];
+        }
       }
     }
-  }
-
-  // values: 8 tokens whose slots are consecutive and start at a multiple of 8 leave as one vector, any
-  // others element by element with consecutive threads on consecutive tokens
-  T *vc = static_cast<T *>(p.value_cache);
-  bool run[2];
+    if (h + 1 < h_end) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // values: 8 tokens whose slots are consecutive and start at a multiple of 8 leave as one vector, any
+    // others element by element with consecutive threads on consecutive tokens
+    if (h == h_begin) {
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int64_t s0 = s_slot[8 * g];
-    run[g] = s0 >= 0 && s0 % 8 == 0;
+      for (int g = 0; g < kRotTok / 8; ++g) {
+        const int64_t s0 = s_slot[8 * g];
+        bool run = s0 >= 0 && s0 % 8 == 0;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) run[g] = run[g] && s_slot[8 * g + j] == s0 + j;
-  }
-  for (int i = tid; i < 2 * D; i += kRotThreads) {
-    const int g = i >= D, d = g ? i - D : i;
-    if (g ? run[1] : run[0]) {
-      uint4 val;
-      T *e = reinterpret_cast<T *>(&val);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = s_v[8 * g + j][d];
-      const int64_t s0 = s_slot[8 * g];
-      *reinterpret_cast<uint4 *>(vc + (s0 / kRotBlock * p.num_kv_heads + h) * D * kRotBlock + d * kRotBlock +
-                                 s0 % kRotBlock) = val;
+        for (int j = 1; j < 8; ++j) run = run && s_slot[8 * g + j] == s0 + j;
+        runs |= (run ? 1u : 0u) << g;
+      }
     }
-  }
-  if (!run[0] || !run[1]) {
-    const int64_t slot = s_slot[tok];
-    if (slot >= 0 && !(tok < 8 ? run[0] : run[1])) {
-      T *dst = vc + (slot / kRotBlock * p.num_kv_heads + h) * D * kRotBlock + slot % kRotBlock;
-      for (int d = tid / kRotTok; d < D; d += kRotThreads / kRotTok) dst[d * kRotBlock] = s_v[tok][d];
+    const T *s_v = buffer(h);
+    auto value_at = [&](int64_t s) { return vc + (s / kRotBlock * p.num_kv_heads + h) * D * kRotBlock + s % kRotBlock; };
+    if (runs != 0u)
+      for (int i = tid; i < 2 * D; i += kRotThreads) {  // both halves of a block's row side by side
+        const int g = i & 1, d = i >> 1;
+        if ((runs >> g) & 1u) {
+          uint4 val;
+          T *e = reinterpret_cast<T *>(&val);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = s_v[(8 * g + j) * pitch + d];
+          *reinterpret_cast<uint4 *>(value_at(s_slot[8 * g]) + d * kRotBlock) = val;
+        }
+      }
+    if (runs != 3u && slot >= 0 && !((runs >> (tok / 8)) & 1u)) {
+      T *dst = value_at(slot);
+      for (int d = tid / kRotTok; d < D; d += kRotThreads / kRotTok) dst[d * kRotBlock] = s_v[tok * pitch + d];
     }
+    if (h + 2 < h_end) __syncthreads();  // the next round's fetch goes into this buffer
   }
 }
 
@@ -222,24 +295,37 @@ struct TableParams {
   void *out;
   int64_t max_position;
   int rot_dim;
+  int walk;  // positions of a thread
 };
 
 __device__ __forceinline__ void put(float *dst, double x) { *dst = (float)x; }
 __device__ __forceinline__ void put(__nv_bfloat16 *dst, double x) { *dst = __double2bfloat16(x); }
 __device__ __forceinline__ void put(__half *dst, double x) { *dst = __double2half(x); }
 
+// One thread walks kWalk positions of a pair: sine and cosine of the first angle and of one position's
+// turn by the library, the ones between by complex products in 64 bits (each costs a relative 2^-52, so
+// kWalk of them stay far below the 2^-24 of the result).  Computing every angle on its own costs some 100
+// 64-bit operations an entry and takes seven times the store's time.
 template <typename C>
 __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ TableParams p) {
   const int half = p.rot_dim / 2;
   const int64_t i = (int64_t)blockIdx.x * kRotThreads + threadIdx.x;
-  const int64_t pos = i / half;
-  const int j = (int)(i - pos * half);
-  if (pos >= p.max_position) return;
-  double s, c;
-  sincos((double)pos * p.freq[j], &s, &c);
-  C *row = static_cast<C *>(p.out) + pos * p.rot_dim;
-  put(row + j, c * p.by);
-  put(row + half + j, s * p.by);
+  const int64_t run = i / half, pos0 = run * p.walk;
+  const int j = (int)(i - run * half);
+  if (pos0 >= p.max_position) return;
+  const int n = (int)min((int64_t)p.walk, p.max_position - pos0);
+  double s, c, ds, dc;
+  sincos((double)pos0 * p.freq[j], &s, &c);
+  sincos(p.freq[j], &ds, &dc);
+  C *row = static_cast<C *>(p.out) + pos0 * p.rot_dim + j;
+  for (int k = 0; k < n; ++k) {
+    put(row, c * p.by);
+    put(row + half, s * p.by);
+    const double t = c * dc - s * ds;
+    s = s * dc + c * ds;
+    c = t;
+    row += p.rot_dim;
+  }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
@@ -268,18 +354,41 @@ static char *check_rotary(const char *fn, const RotaryParams &p, int table_dtype
                "%s: token strides must be multiples of 8 elements and cover one row", fn);
     AICI_CHECK(p.num_slots > 0, "%s: num_blocks must be positive", fn);
   }
-  const int64_t tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
+  const int64_t tiles = (p.num_tokens + 15) / 16;
   AICI_CHECK(tiles * p.num_kv_heads + p.num_tokens < (1ll << 31), "%s: too many tokens and heads for one call", fn);
   return nullptr;
 }
 
+// Few tokens: one head to a thread, so that more of the GPU takes part; many: four, which share the
+// table row and are in flight together.
+static HeadPlan plan_heads(int tokens, int heads, int rot_dim) {
+  const int nc = rot_dim / 16, most = kRotThreads / nc;
+  const int per = (int64_t)tokens * heads * nc >= (int64_t)4 * 4 * kRotThreads * sm_count() ? 4 : 1;
+  HeadPlan plan;
+  plan.slots = (heads + per - 1) / per < most ? (heads + per - 1) / per : most;
+  plan.tokens = most / plan.slots;
+  const int runs = (tokens + plan.tokens - 1) / plan.tokens;
+  plan.ctas = per > 1 ? (runs + 3) / 4 : runs;
+  return plan;
+}
+
 template <typename T, typename C, bool kNeox>
-static char *launch_rotary(const RotaryParams &p, bool cache, cudaStream_t stream) {
-  if (cache) {
-    const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
-    rotary_cache_kernel<T, C, kNeox><<<tiles * p.num_kv_heads + p.num_tokens, kRotThreads, 0, stream>>>(p);
+static char *launch_rotary(RotaryParams p, bool cache, cudaStream_t stream) {
+  p.q_plan = plan_heads(p.num_tokens, p.num_heads, p.rot_dim);
+  p.k_plan = plan_heads(p.num_tokens, p.num_kv_heads, p.rot_dim);
+  if (!cache) {
+    rotary_kernel<T, C, kNeox><<<p.q_plan.ctas + p.k_plan.ctas, kRotThreads, 0, stream>>>(p);
   } else {
-    rotary_kernel<T, C, kNeox><<<p.num_tokens, kRotThreads, 0, stream>>>(p);
+    const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
+    p.kv_heads_per_cta = 1;
+    while (p.kv_heads_per_cta < 4 && (int64_t)tiles * p.num_kv_heads >= (int64_t)8 * p.kv_heads_per_cta * sm_count())
+      p.kv_heads_per_cta *= 2;
+    const int grid = tiles * ((p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta) + p.q_plan.ctas;
+    const size_t smem = 2 * kRotTok * (p.head_size + 8) * sizeof(T);
+    if (p.rot_dim / 16 + (p.head_size - p.rot_dim) / 8 <= kRotThreads / kRotTok)
+      rotary_cache_kernel<T, C, kNeox, 1><<<grid, kRotThreads, smem, stream>>>(p);
+    else
+      rotary_cache_kernel<T, C, kNeox, 2><<<grid, kRotThreads, smem, stream>>>(p);
   }
   AICI_CUDA(cudaGetLastError());
   return nullptr;
@@ -337,7 +446,7 @@ extern "C" char *aici_rotary_embedding_and_cache(const int64_t *positions, void 
   AICI_CHECK(block_size == kRotBlock, "%s: block_size must be 16 (got %d)", fn, block_size);
   RotaryParams p = {positions, query, key, value, cos_sin_cache, slot_mapping, key_cache, value_cache,
                     num_tokens, num_heads, num_kv_heads, head_size, rot_dim, slot_is_int64,
-                    max_position, num_blocks * kRotBlock, query_stride, key_stride, value_stride, nullptr};
+                    max_position, num_blocks * kRotBlock, query_stride, key_stride, value_stride, nullptr, {}, {}, 1};
   return rotary_impl(fn, p, is_neox, table_dtype, dtype, true, stream);
 }
 
@@ -378,7 +487,10 @@ extern "C" char *aici_rotary_cos_sin_cache(void *out, int64_t max_position, int 
     }
     p.freq[j] = f;
   }
-  const int64_t grid = (max_position * (rot_dim / 2) + kRotThreads - 1) / kRotThreads;
+  // 64 positions to a thread where that leaves eight warps per multiprocessor, fewer for short tables
+  p.walk = 64;
+  while (p.walk > 4 && max_position * (rot_dim / 2) < (int64_t)p.walk * 256 * sm_count()) p.walk /= 2;
+  const int64_t grid = ((max_position + p.walk - 1) / p.walk * (rot_dim / 2) + kRotThreads - 1) / kRotThreads;
   AICI_CHECK(grid < (1ll << 31), "%s: table too large", fn);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == AICI_DTYPE_F32) rotary_table_kernel<float><<<(unsigned)grid, kRotThreads, 0, s>>>(p);

@@ -18,8 +18,9 @@
 
 namespace aici {
 
-constexpr int kStepThreads = 512;
+constexpr int kStepThreads = 1024;  // of a CTA at most; a quarter for small steps
 constexpr int kStepWarps = kStepThreads / 32;
+constexpr int kStepBatch = 4;       // lengths a thread loads at once, tokens it works on together
 constexpr int kBlockTokens = 16;
 constexpr int kMaxStepRequests = 16384;        // 12 bytes of shared memory each
 constexpr int kMaxStepTokens = (1 << 30) - 1;
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
   int *s_ctx = reinterpret_cast<int *>(s_new + p.n + 1);
   __shared__ unsigned int s_warp_tok[kStepWarps], s_warp_new[kStepWarps];
   __shared__ int s_bad;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
   unsigned int rank, ctas;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
@@ -56,22 +57,31 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
 
   // ---- lengths: each thread a run of consecutive requests ------------------------------------------
   const int free_count = *p.free_count;
-  const int per = (p.n + kStepThreads - 1) / kStepThreads;
+  const int per = (p.n + nthreads - 1) / nthreads;
   const int i0 = min(tid * per, p.n), i1 = min(i0 + per, p.n);
   const int64_t row_tokens = (int64_t)p.max_blocks * kBlockTokens;
   unsigned int tok = 0, fresh = 0;
   bool bad = free_count < 0 || free_count > p.free_capacity;
-  for (int i = i0; i < i1; ++i) {
-    const int q = p.query_lens[i], c = p.context_lens[i];
-    const bool wrong = q < 0 || c < 0 || (int64_t)c + q > row_tokens;
-    bad |= wrong;
-    s_ctx[i] = c;
-    s_tok[i] = tok;  // relative to the thread's run; the runs before it are added below
-    s_new[i] = fresh;
-    if (!wrong) {
-      tok = sat_add(tok, (unsigned int)q);
-      fresh = sat_add(fresh, (unsigned int)(((int64_t)c + q + kBlockTokens - 1) / kBlockTokens -
-                                            ((int64_t)c + kBlockTokens - 1) / kBlockTokens));
+  for (int i = i0; i < i1; i += kStepBatch) {
+    int q[kStepBatch], c[kStepBatch];
+#pragma unroll
+    for (int k = 0; k < kStepBatch; ++k) {
+      q[k] = i + k < i1 ? p.query_lens[i + k] : 0;
+      c[k] = i + k < i1 ? p.context_lens[i + k] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kStepBatch; ++k) {
+      if (i + k >= i1) break;
+      const bool wrong = q[k] < 0 || c[k] < 0 || (int64_t)c[k] + q[k] > row_tokens;
+      bad |= wrong;
+      s_ctx[i + k] = c[k];
+      s_tok[i + k] = tok;  // relative to the thread's run; the runs before it are added below
+      s_new[i + k] = fresh;
+      if (!wrong) {
+        tok = sat_add(tok, (unsigned int)q[k]);
+        fresh = sat_add(fresh, (unsigned int)(((int64_t)c[k] + q[k] + kBlockTokens - 1) / kBlockTokens -
+                                              ((int64_t)c[k] + kBlockTokens - 1) / kBlockTokens));
+      }
     }
   }
   if (bad) s_bad = 1;
@@ -90,16 +100,23 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
     s_warp_new[warp] = new_incl;
   }
   __syncthreads();
-  unsigned int tok_base = 0, new_base = 0, tok_total = 0, new_total = 0;
+  // every warp scans the warps' sums for itself
+  unsigned int tok_warps = lane < nthreads / 32 ? s_warp_tok[lane] : 0u;
+  unsigned int new_warps = lane < nthreads / 32 ? s_warp_new[lane] : 0u;
 #pragma unroll
-  for (int w = 0; w < kStepWarps; ++w) {
-    if (w == warp) {
-      tok_base = tok_total;
-      new_base = new_total;
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned int a = __shfl_up_sync(0xffffffffu, tok_warps, o);
+    const unsigned int b = __shfl_up_sync(0xffffffffu, new_warps, o);
+    if (lane >= o) {
+      tok_warps = sat_add(tok_warps, a);
+      new_warps = sat_add(new_warps, b);
     }
-    tok_total = sat_add(tok_total, s_warp_tok[w]);
-    new_total = sat_add(new_total, s_warp_new[w]);
   }
+  const unsigned int tok_total = __shfl_sync(0xffffffffu, tok_warps, 31);
+  const unsigned int new_total = __shfl_sync(0xffffffffu, new_warps, 31);
+  unsigned int tok_base = __shfl_sync(0xffffffffu, tok_warps, max(warp - 1, 0));
+  unsigned int new_base = __shfl_sync(0xffffffffu, new_warps, max(warp - 1, 0));
+  if (warp == 0) tok_base = new_base = 0;
   // the runs of the lower lanes of this warp
   const unsigned int tok_prev = __shfl_up_sync(0xffffffffu, tok_incl, 1);
   const unsigned int new_prev = __shfl_up_sync(0xffffffffu, new_incl, 1);
@@ -124,54 +141,94 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
 
   // ---- tokens: four consecutive ones to a thread -----------------------------------------------------
   const int total = (int)s_tok[p.n];
-  const int gid = rank * kStepThreads + tid, threads = ctas * kStepThreads;
-  for (int64_t t0 = 4 * (int64_t)gid; t0 < p.max_tokens; t0 += 4 * (int64_t)threads) {
-    int64_t pos[4] = {0, 0, 0, 0};
-    int slot[4] = {-1, -1, -1, -1};
-    if (t0 < total) {
+  const int gid = rank * nthreads + tid, threads = ctas * nthreads;
+  auto block_of = [&](int req, int ctx, int blk) -> const int32_t * {  // where the id of a request's block is
+    const int held = (int)(((unsigned int)ctx + kBlockTokens - 1) / kBlockTokens);
+    return blk < held ? p.block_tables + req * p.table_stride + blk
+                      : p.free_blocks + (free_count - 1 - (int)(s_new[req] + (unsigned int)(blk - held)));
+  };
+  auto slot_of = [&](int id, int at) {
+    if (id >= 0 && id < p.num_blocks) return id * kBlockTokens + at % kBlockTokens;
+    set_status(p.status, AICI_STATUS_BAD_BLOCK);
+    return -1;
+  };
+  auto enter = [&](int req, int at, int id) {  // a token that begins a block enters it in the table
+    if (at % kBlockTokens == 0) p.block_tables[req * p.table_stride + at / kBlockTokens] = id;
+  };
+  for (int64_t t64 = (int64_t)kStepBatch * gid; t64 < p.max_tokens; t64 += (int64_t)kStepBatch * threads) {
+    const unsigned int t0 = (unsigned int)t64;
+    int pos0 = 0, pos1 = 0, pos2 = 0, pos3 = 0, slot0 = -1, slot1 = -1, slot2 = -1, slot3 = -1;
+    if (t0 < (unsigned int)total) {
       // the request of the first token: the last i with s_tok[i] <= t0 (requests without tokens share
       // their start with the one behind them, and the last of those is the one that has tokens)
       int lo = 0, hi = p.n;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (s_tok[mid] <= (unsigned int)t0) lo = mid;
+        if (s_tok[mid] <= t0) lo = mid;
         else hi = mid;
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned int t = (unsigned int)t0 + j;
-        if (t < (unsigned int)total) {
-          while (t >= s_tok[lo + 1]) ++lo;
-          const int c = s_ctx[lo];
-          const int at = c + (int)(t - s_tok[lo]);
-          const int blk = at / kBlockTokens, held = (c + kBlockTokens - 1) / kBlockTokens;
-          int32_t *entry = p.block_tables + lo * p.table_stride + blk;
-          int id;
-          if (blk < held) {
-            id = *entry;
-          } else {
-            id = p.free_blocks[free_count - 1 - (int)(s_new[lo] + (unsigned int)(blk - held))];
-            if (at % kBlockTokens == 0) *entry = id;
-          }
-          pos[j] = at;
-          if (id >= 0 && id < p.num_blocks) slot[j] = id * kBlockTokens + at % kBlockTokens;
-          else set_status(p.status, AICI_STATUS_BAD_BLOCK);
+      if (t0 + kStepBatch <= s_tok[lo + 1]) {
+        // all of one request: at most two blocks
+        const int ctx = s_ctx[lo];
+        pos0 = ctx + (int)(t0 - s_tok[lo]);
+        pos1 = pos0 + 1;
+        pos2 = pos0 + 2;
+        pos3 = pos0 + 3;
+        const int b0 = pos0 / kBlockTokens, b1 = pos3 / kBlockTokens;
+        const int id0 = *block_of(lo, ctx, b0), id1 = b1 != b0 ? *block_of(lo, ctx, b1) : id0;
+        slot0 = slot_of(id0, pos0);
+        slot1 = slot_of(pos1 / kBlockTokens == b0 ? id0 : id1, pos1);
+        slot2 = slot_of(pos2 / kBlockTokens == b0 ? id0 : id1, pos2);
+        slot3 = slot_of(id1, pos3);
+        if (pos0 % kBlockTokens == 0 || b1 != b0) {
+          const int begin = b1 * kBlockTokens;  // the block that begins within the four, at its first token
+          enter(lo, begin, b1 != b0 ? id1 : id0);
         }
+      } else {
+        // tokens of several requests: where each one's id is, then all the ids at once
+        int req0 = -1, req1 = -1, req2 = -1, req3 = -1;
+        auto locate = [&](unsigned int t, int &req, int &pos) -> const int32_t * {
+          if (t >= (unsigned int)total) return p.free_count;  // any readable word
+          while (t >= s_tok[lo + 1]) ++lo;
+          req = lo;
+          pos = s_ctx[lo] + (int)(t - s_tok[lo]);
+          return block_of(lo, s_ctx[lo], pos / kBlockTokens);
+        };
+        const int32_t *a0 = locate(t0, req0, pos0), *a1 = locate(t0 + 1, req1, pos1);
+        const int32_t *a2 = locate(t0 + 2, req2, pos2), *a3 = locate(t0 + 3, req3, pos3);
+        const int id0 = *a0, id1 = *a1, id2 = *a2, id3 = *a3;
+        auto settle = [&](int req, int pos, int id, int &slot) {
+          if (req < 0) return;
+          slot = slot_of(id, pos);
+          enter(req, pos, id);
+        };
+        settle(req0, pos0, id0, slot0);
+        settle(req1, pos1, id1, slot1);
+        settle(req2, pos2, id2, slot2);
+        settle(req3, pos3, id3, slot3);
       }
     }
-    if (t0 + 4 <= p.max_tokens) {
-      *reinterpret_cast<longlong2 *>(p.positions + t0) = make_longlong2(pos[0], pos[1]);
-      *reinterpret_cast<longlong2 *>(p.positions + t0 + 2) = make_longlong2(pos[2], pos[3]);
-      *reinterpret_cast<int4 *>(p.slot_mapping + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    if (t64 + kStepBatch <= p.max_tokens) {
+      *reinterpret_cast<longlong2 *>(p.positions + t64) = make_longlong2(pos0, pos1);
+      *reinterpret_cast<longlong2 *>(p.positions + t64 + 2) = make_longlong2(pos2, pos3);
+      *reinterpret_cast<int4 *>(p.slot_mapping + t64) = make_int4(slot0, slot1, slot2, slot3);
     } else {
-      for (int j = 0; t0 + j < p.max_tokens; ++j) {
-        p.positions[t0 + j] = pos[j];
-        p.slot_mapping[t0 + j] = slot[j];
+      const int left = (int)(p.max_tokens - t64);  // 1 to 3
+      p.positions[t64] = pos0;
+      p.slot_mapping[t64] = slot0;
+      if (left > 1) {
+        p.positions[t64 + 1] = pos1;
+        p.slot_mapping[t64 + 1] = slot1;
+      }
+      if (left > 2) {
+        p.positions[t64 + 2] = pos2;
+        p.slot_mapping[t64 + 2] = slot2;
       }
     }
   }
 
   // ---- requests -------------------------------------------------------------------------------------
+  __syncwarp();
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   for (int i = gid; i <= p.n; i += threads) {
     const unsigned int a = s_tok[i];
@@ -225,17 +282,19 @@ extern "C" char *aici_step_tables(const int32_t *query_lens, const int32_t *cont
   StepParams p = {query_lens, context_lens, block_tables, free_blocks, free_count, seqlens_q, slot_mapping,
                   logit_idxs, context_lens_out, free_count_out, positions, num_requests, max_blocks_per_seq,
                   max_tokens, free_capacity, num_blocks, block_table_stride, st};
+  // one small CTA, or up to eight large ones: a thread has one batch of tokens where that is possible
+  const int64_t work = (int64_t)max_tokens + num_requests;
+  const int threads = work <= kStepThreads ? kStepThreads / 4 : kStepThreads;
+  int ctas = 1;
+  while (ctas < 8 && work > (int64_t)kStepBatch * threads * ctas) ctas *= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  while (attr[0].val.clusterDim.x < 8 &&
-         (int64_t)max_tokens + num_requests > (int64_t)4 * kStepThreads * attr[0].val.clusterDim.x)
-    attr[0].val.clusterDim.x *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(attr[0].val.clusterDim.x);
-  cfg.blockDim = dim3(kStepThreads);
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = (3 * (size_t)num_requests + 2) * sizeof(int);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;

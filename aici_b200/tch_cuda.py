@@ -52,9 +52,29 @@ def _stream(dev: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _raw_stream(dev: torch.device) -> int:
-    """Handle of the device's current stream, without the Stream object around it."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _one_gpu(fn: str, tensors) -> int:
+    """Index of the GPU that all the tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index:
+            raise AiciError("%s: tensors are on different devices" % fn)
+    if index < 0:
+        raise AiciError("%s: tensor must be on a CUDA device (there is no CPU path)" % fn)
+    return index
+
+
+def _call(fn: str, name: str, index: int, *args) -> None:
+    """The library's `name`(*args, current stream of GPU `index`) with that GPU current.  For the entry
+    points whose parameter lists _lib knows: arguments are plain numbers, and what the call costs the host
+    is close to what the launch costs."""
+    entry = getattr(_lib.lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        res = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            res = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if res:
+        _lib.check(fn, res)
 
 
 def _require_cuda(fn: str, *tensors: torch.Tensor):
@@ -714,36 +734,39 @@ def rotary_cos_sin_cache(max_position: int, rot_dim: int, base: float, dtype: to
         raise AiciError("%s: unknown scaling %r" % (fn, scaling))
     if dtype not in _DTYPES:
         raise AiciError("%s: unsupported dtype %s" % (fn, dtype))
-    dev = torch.device(device)
-    if dev.type != "cuda":
+    if torch.device(device).type != "cuda":
         raise AiciError("%s: tensor must be on a CUDA device (there is no CPU path)" % fn)
-    out = torch.empty((max_position, rot_dim), dtype=dtype, device=dev)
-    with _on_device(out.device):
-        _lib.check(fn, _lib.lib().aici_rotary_cos_sin_cache(
-            out.data_ptr(), max_position, rot_dim, base, _SCALINGS[scaling], factor, original_context,
-            _DTYPES[dtype], _raw_stream(out.device)))
+    out = torch.empty((max_position, rot_dim), dtype=dtype, device=device)
+    _call(fn, "aici_rotary_cos_sin_cache", out.get_device(), out.data_ptr(), max_position, rot_dim, base,
+          _SCALINGS[scaling], factor, original_context, _DTYPES[dtype])
     return out
 
 
-def _rotary_rows(fn, positions, query, key, head_size, cos_sin_cache):
-    if positions.dtype != torch.int64 or not positions.is_contiguous() or positions.numel() != query.shape[0]:
+def _rows(fn, name, t, head_size):
+    """Heads per token and token stride of [num_tokens, heads * head_size] or [num_tokens, heads,
+    head_size]; the heads of a token are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2:
+        if shape[1] % head_size == 0 and (stride[1] == 1 or shape[1] == 1):
+            return shape[1] // head_size, stride[0]
+    elif len(shape) == 3:
+        if shape[2] == head_size and stride[2] == 1 and (stride[1] == head_size or shape[1] == 1):
+            return shape[1], stride[0]
+    raise AiciError("%s: %s must be [num_tokens, heads * head_size] or [num_tokens, heads, head_size] with "
+                    "contiguous rows" % (fn, name))
+
+
+def _check_rotary(fn, positions, query, key, head_size, cos_sin_cache):
+    if head_size <= 0:
+        raise AiciError("%s: head_size must be positive" % fn)
+    if positions.dtype is not torch.int64 or not positions.is_contiguous() or positions.numel() != query.shape[0]:
         raise AiciError("%s: positions must be contiguous int64 [num_tokens]" % fn)
     if cos_sin_cache.dim() != 2 or not cos_sin_cache.is_contiguous():
         raise AiciError("%s: cos_sin_cache must be contiguous [max_position, rot_dim]" % fn)
-    if key.dtype != query.dtype:
+    if key.dtype is not query.dtype:
         raise AiciError("%s: query and key must have the same dtype" % fn)
-    return _rows(fn, "query", query, head_size), _rows(fn, "key", key, head_size)
-
-
-def _rows(fn, name, t, head_size):
-    """Heads of one token of [num_tokens, heads * head_size] or [num_tokens, heads, head_size]."""
-    if t.dim() == 3:
-        if t.shape[2] == head_size and t.stride(2) == 1 and (t.stride(1) == head_size or t.shape[1] == 1):
-            return t.shape[1]
-    elif t.dim() == 2 and t.shape[1] % head_size == 0 and (t.stride(1) == 1 or t.shape[1] == 1):
-        return t.shape[1] // head_size
-    raise AiciError("%s: %s must be [num_tokens, heads * head_size] or [num_tokens, heads, head_size] with "
-                    "contiguous rows" % (fn, name))
+    if key.shape[0] != query.shape[0]:
+        raise AiciError("%s: query and key differ in length" % fn)
 
 
 def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, head_size: int,
@@ -753,16 +776,14 @@ def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Te
     [max_position, rot_dim] that `positions` names; is_neox pairs element j with j + rot_dim / 2, else 2 j
     with 2 j + 1; elements from rot_dim on stay.  bf16 or f16, the table f32 or of the same type."""
     fn = "rotary_embedding"
-    dev = _require_cuda(fn, positions, query, key, cos_sin_cache)
-    num_heads, num_kv_heads = _rotary_rows(fn, positions, query, key, head_size, cos_sin_cache)
-    if key.shape[0] != query.shape[0]:
-        raise AiciError("%s: query and key differ in length" % fn)
-    with _on_device(dev):
-        _lib.check(fn, _lib.lib().aici_rotary_embedding(
-            positions.data_ptr(), query.data_ptr(), key.data_ptr(), cos_sin_cache.data_ptr(), query.shape[0],
-            num_heads, num_kv_heads, head_size, cos_sin_cache.shape[1], 1 if is_neox else 0,
-            cos_sin_cache.shape[0], query.stride(0), key.stride(0), _dtype(fn, cos_sin_cache),
-            _dtype(fn, query), _raw_stream(dev)))
+    index = _one_gpu(fn, (positions, query, key, cos_sin_cache))
+    _check_rotary(fn, positions, query, key, head_size, cos_sin_cache)
+    num_heads, q_stride = _rows(fn, "query", query, head_size)
+    num_kv_heads, k_stride = _rows(fn, "key", key, head_size)
+    max_position, rot_dim = cos_sin_cache.shape
+    _call(fn, "aici_rotary_embedding", index, positions.data_ptr(), query.data_ptr(), key.data_ptr(),
+          cos_sin_cache.data_ptr(), query.shape[0], num_heads, num_kv_heads, head_size, rot_dim,
+          1 if is_neox else 0, max_position, q_stride, k_stride, _dtype(fn, cos_sin_cache), _dtype(fn, query))
 
 
 def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
@@ -774,35 +795,44 @@ def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key
     head, bf16 and f16, head sizes up to 256); rotary_embedding_reshape_and_cache is the bf16 form with the
     reference kernel's rounding."""
     fn = "rotary_embedding_and_cache"
-    dev = _require_cuda(fn, positions, query, key, value, cos_sin_cache, key_cache, value_cache, slot_mapping)
+    index = _one_gpu(fn, (positions, query, key, value, cos_sin_cache, key_cache, value_cache, slot_mapping))
     num_blocks, num_kv_heads, cache_head, block_size = _cache_dims(fn, key_cache, value_cache)
     if cache_head != head_size:
         raise AiciError("%s: head_size does not match the cache" % fn)
-    num_heads, key_heads = _rotary_rows(fn, positions, query, key, head_size, cos_sin_cache)
-    if key_heads != num_kv_heads or _rows(fn, "value", value, head_size) != num_kv_heads:
+    _check_rotary(fn, positions, query, key, head_size, cos_sin_cache)
+    num_heads, q_stride = _rows(fn, "query", query, head_size)
+    key_heads, k_stride = _rows(fn, "key", key, head_size)
+    value_heads, v_stride = _rows(fn, "value", value, head_size)
+    if key_heads != num_kv_heads or value_heads != num_kv_heads:
         raise AiciError("%s: key/value width does not match the cache" % fn)
-    T = query.shape[0]
-    if key.shape[0] != T or value.shape[0] != T:
+    T, dtype, slots = query.shape[0], query.dtype, slot_mapping.dtype
+    if value.shape[0] != T:
         raise AiciError("%s: query, key and value differ in length" % fn)
-    if value.dtype != query.dtype or key_cache.dtype != query.dtype or value_cache.dtype != query.dtype:
+    if value.dtype is not dtype or key_cache.dtype is not dtype or value_cache.dtype is not dtype:
         raise AiciError("%s: dtypes differ" % fn)
-    if slot_mapping.dtype not in (torch.int32, torch.int64) or not slot_mapping.is_contiguous() or \
+    if (slots is not torch.int32 and slots is not torch.int64) or not slot_mapping.is_contiguous() or \
             slot_mapping.numel() != T:
         raise AiciError("%s: slot_mapping must be contiguous int32 or int64 [num_tokens]" % fn)
-    with _on_device(dev):
-        _lib.check(fn, _lib.lib().aici_rotary_embedding_and_cache(
-            positions.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), cos_sin_cache.data_ptr(),
-            key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(),
-            1 if slot_mapping.dtype == torch.int64 else 0, T, num_heads, num_kv_heads, head_size,
-            cos_sin_cache.shape[1], 1 if is_neox else 0, cos_sin_cache.shape[0], block_size, num_blocks,
-            query.stride(0), key.stride(0), value.stride(0), _dtype(fn, cos_sin_cache), _dtype(fn, query),
-            _raw_stream(dev)))
+    max_position, rot_dim = cos_sin_cache.shape
+    _call(fn, "aici_rotary_embedding_and_cache", index, positions.data_ptr(), query.data_ptr(), key.data_ptr(),
+          value.data_ptr(), cos_sin_cache.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+          slot_mapping.data_ptr(), 1 if slots is torch.int64 else 0, T, num_heads, num_kv_heads, head_size,
+          rot_dim, 1 if is_neox else 0, max_position, block_size, num_blocks, q_stride, k_stride, v_stride,
+          _dtype(fn, cos_sin_cache), _dtype(fn, query))
 
 
 # ---- attention with a sliding window and sinks ----------------------------------------------------------
 def _int32(x: int) -> int:
     """A window or sink count as the C ABI takes it: what is longer than any sequence means the same."""
-    return min(int(x), 0x7fffffff)
+    return x if x < 0x7fffffff else 0x7fffffff
+
+
+def _check_table(fn, block_tables, context_lens, batch):
+    if block_tables.dtype is not torch.int32 or context_lens.dtype is not torch.int32 or \
+            not block_tables.is_contiguous() or not context_lens.is_contiguous():
+        raise AiciError("%s: block_tables and context_lens must be contiguous int32" % fn)
+    if block_tables.dim() != 2 or block_tables.shape[0] != batch or context_lens.numel() != batch:
+        raise AiciError("%s: block_tables must be [batch, max_blocks], context_lens [batch]" % fn)
 
 
 def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor,
@@ -813,35 +843,56 @@ def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: to
     the last `window` tokens, its own among them, and the first `sinks` tokens.  bf16 or f16, up to 16
     query heads per kv head.  Blocks without a visible token are never read."""
     fn = "paged_attention_window"
-    dev, num_blocks, head_size = _decode_common(fn, out, query, key_cache, value_cache, num_kv_heads,
-                                                block_tables, context_lens, block_size)
-    if value_cache.dtype != query.dtype:
+    index = _one_gpu(fn, (out, query, key_cache, value_cache, block_tables, context_lens))
+    num_blocks, cache_kv_heads, head_size, cache_block = _cache_dims(fn, key_cache, value_cache)
+    if cache_kv_heads != num_kv_heads or cache_block != block_size:
+        raise AiciError("%s: num_kv_heads / block_size do not match the cache" % fn)
+    shape, stride, dtype = query.shape, query.stride(), query.dtype
+    if len(shape) != 3 or out.shape != shape or shape[2] != head_size or stride[2] != 1 or \
+            (stride[1] != head_size and shape[1] != 1):
+        raise AiciError("%s: out and query must be [num_seqs, num_heads, head_size] of the cache's head_size, "
+                        "the heads of a row contiguous" % fn)
+    if not out.is_contiguous():
+        raise AiciError("%s: out must be contiguous" % fn)
+    if out.dtype is not dtype or key_cache.dtype is not dtype or value_cache.dtype is not dtype:
         raise AiciError("%s: dtypes differ" % fn)
-    num_seqs, num_heads, _ = query.shape
+    num_seqs, num_heads, _ = shape
+    _check_table(fn, block_tables, context_lens, num_seqs)
     window, sinks = _int32(window), _int32(sinks)
-    L = _lib.lib()
-    with _on_device(dev):
-        nbytes = L.aici_paged_attention_window_workspace_bytes(num_seqs, num_heads, num_kv_heads, max_context_len,
-                                                               window, sinks)
-        # a captured call keeps its workspace to itself: graphs may run at the same time
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if torch.cuda.is_current_stream_capturing() \
-            else _workspace(dev, nbytes)
-        _lib.check(fn, L.aici_paged_attention_window(
-            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), num_kv_heads, scale,
-            block_tables.data_ptr(), context_lens.data_ptr(), block_size, max_context_len, window, sinks, num_seqs,
-            num_heads, head_size, block_tables.shape[1], num_blocks, query.stride(0), key_cache.stride(0),
-            key_cache.stride(1), ws.data_ptr(), ws.numel(), _dtype(fn, query), _raw_stream(dev)))
+    nbytes = _window_workspace_bytes(index, num_seqs, num_heads, num_kv_heads, max_context_len, window, sinks)
+    ws = _window_workspace(index, nbytes) if nbytes else None
+    _call(fn, "aici_paged_attention_window", index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(),
+          value_cache.data_ptr(), num_kv_heads, scale, block_tables.data_ptr(), context_lens.data_ptr(), block_size,
+          max_context_len, window, sinks, num_seqs, num_heads, head_size, block_tables.shape[1], num_blocks,
+          stride[0], key_cache.stride(0), key_cache.stride(1), ws.data_ptr() if nbytes else None, nbytes,
+          _dtype(fn, query))
 
 
-def _window_common(fn, q, seqlens_q):
+def _window_workspace_bytes(index: int, *sizes) -> int:
+    # the size depends on the GPU's number of multiprocessors
+    if torch._C._cuda_getDevice() == index:
+        return _lib.lib().aici_paged_attention_window_workspace_bytes(*sizes)
+    with torch.cuda.device(index):
+        return _lib.lib().aici_paged_attention_window_workspace_bytes(*sizes)
+
+
+def _window_workspace(index: int, nbytes: int) -> torch.Tensor:
+    """The stream's scratch; a captured call gets one of its own, since graphs may run at the same time."""
+    dev = torch.device("cuda", index)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return _workspace(dev, nbytes)
+
+
+def _check_prefill(fn, q, seqlens_q):
     if q.dim() != 3 or q.stride(2) != 1:
         raise AiciError("%s: q must be [total_q, num_heads, head_size] with contiguous last dimension" % fn)
-    if seqlens_q.dtype != torch.int32 or not seqlens_q.is_contiguous():
+    if seqlens_q.dtype is not torch.int32 or not seqlens_q.is_contiguous():
         raise AiciError("%s: seqlens_q must be contiguous int32" % fn)
     batch = seqlens_q.numel() - 1
     if batch <= 0:
         raise AiciError("%s: batch size must be positive" % fn)
-    return batch, torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    return batch
 
 
 def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqlens_q: torch.Tensor,
@@ -850,20 +901,22 @@ def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     """flash_attn_varlen, causal, with a sliding window: a query at position p of its sequence sees the
     tokens t <= p with t > p - window or t < sinks.  bf16 or f16.  Returns [total_q, num_heads, head_size]."""
     fn = "flash_attn_varlen_window"
-    dev = _require_cuda(fn, q, k, v, seqlens_q, seqlens_k)
-    batch, out = _window_common(fn, q, seqlens_q)
-    if k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2] or k.stride(2) != 1 or v.stride(2) != 1:
+    index = _one_gpu(fn, (q, k, v, seqlens_q, seqlens_k))
+    batch = _check_prefill(fn, q, seqlens_q)
+    total_q, num_heads, head_size = q.shape
+    ks, vs = k.stride(), v.stride()
+    if len(ks) != 3 or v.shape != k.shape or k.shape[2] != head_size or ks[2] != 1 or vs[2] != 1:
         raise AiciError("%s: k and v must be [total_k, num_heads_k, head_size] with contiguous last dimension" % fn)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise AiciError("%s: query, key and value must have the same dtype" % fn)
-    if seqlens_k.dtype != torch.int32 or not seqlens_k.is_contiguous() or seqlens_k.numel() != batch + 1:
+    if seqlens_k.dtype is not torch.int32 or not seqlens_k.is_contiguous() or seqlens_k.numel() != batch + 1:
         raise AiciError("%s: seqlens_k must be contiguous int32 and as long as seqlens_q" % fn)
-    with _on_device(dev):
-        _lib.check(fn, _lib.lib().aici_mha_varlen_window_fwd(
-            out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), seqlens_q.data_ptr(), seqlens_k.data_ptr(),
-            batch, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], max_seqlen_q, max_seqlen_k,
-            _int32(window), _int32(sinks), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
-            out.stride(1), softmax_scale, _dtype(fn, q), _raw_stream(dev)))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_tok, q_head, _ = q.stride()
+    _call(fn, "aici_mha_varlen_window_fwd", index, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+          seqlens_q.data_ptr(), seqlens_k.data_ptr(), batch, total_q, k.shape[0], num_heads, k.shape[1], head_size,
+          max_seqlen_q, max_seqlen_k, _int32(window), _int32(sinks), q_tok, q_head, ks[0], ks[1], vs[0], vs[1],
+          num_heads * head_size, head_size, softmax_scale, _dtype(fn, q))
     return out
 
 
@@ -874,23 +927,20 @@ def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, val
     """flash_attn_varlen_paged, causal, with the window of flash_attn_varlen_window: the new tokens of a
     chunk against the paged cache.  bf16 or f16.  Blocks without a visible token are never read."""
     fn = "flash_attn_varlen_paged_window"
-    dev = _require_cuda(fn, q, key_cache, value_cache, seqlens_q, context_lens, block_tables)
+    index = _one_gpu(fn, (q, key_cache, value_cache, seqlens_q, context_lens, block_tables))
     num_blocks, num_kv_heads, head_size, block_size = _cache_dims(fn, key_cache, value_cache)
-    batch, out = _window_common(fn, q, seqlens_q)
-    if q.shape[2] != head_size:
+    batch = _check_prefill(fn, q, seqlens_q)
+    total_q, num_heads, q_head_size = q.shape
+    if q_head_size != head_size:
         raise AiciError("%s: head_size does not match the cache" % fn)
-    if q.dtype != key_cache.dtype or q.dtype != value_cache.dtype:
+    if q.dtype is not key_cache.dtype or q.dtype is not value_cache.dtype:
         raise AiciError("%s: query and cache dtypes differ" % fn)
-    if context_lens.dtype != torch.int32 or block_tables.dtype != torch.int32 or \
-            not context_lens.is_contiguous() or not block_tables.is_contiguous():
-        raise AiciError("%s: context_lens and block_tables must be contiguous int32" % fn)
-    if context_lens.numel() != batch or block_tables.dim() != 2 or block_tables.shape[0] != batch:
-        raise AiciError("%s: context_lens must be [batch] and block_tables [batch, max_blocks]" % fn)
-    with _on_device(dev):
-        _lib.check(fn, _lib.lib().aici_mha_varlen_paged_window_fwd(
-            out.data_ptr(), q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), seqlens_q.data_ptr(),
-            context_lens.data_ptr(), block_tables.data_ptr(), batch, q.shape[0], q.shape[1], num_kv_heads, head_size,
-            block_size, max_seqlen_q, max_context_len, block_tables.shape[1], num_blocks, _int32(window),
-            _int32(sinks), q.stride(0), q.stride(1), out.stride(0), out.stride(1), key_cache.stride(0), key_cache.stride(1), softmax_scale,
-            _dtype(fn, q), _raw_stream(dev)))
+    _check_table(fn, block_tables, context_lens, batch)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_tok, q_head, _ = q.stride()
+    _call(fn, "aici_mha_varlen_paged_window_fwd", index, out.data_ptr(), q.data_ptr(), key_cache.data_ptr(),
+          value_cache.data_ptr(), seqlens_q.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), batch,
+          total_q, num_heads, num_kv_heads, head_size, block_size, max_seqlen_q, max_context_len,
+          block_tables.shape[1], num_blocks, _int32(window), _int32(sinks), q_tok, q_head, num_heads * head_size,
+          head_size, key_cache.stride(0), key_cache.stride(1), softmax_scale, _dtype(fn, q))
     return out
