@@ -217,13 +217,12 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     if len(table) != 2 or table[0] != n or rows[1] != 1:
         raise AiciError("%s: block_tables must be [requests, max_blocks] with contiguous rows" % fn)
     if out is None:
-        # one allocation; the token tensors first, for their alignment
-        T4 = (max_tokens + 3) // 4 * 4
-        buf = torch.empty(3 * T4 + 3 * n + 2, dtype=torch.int32, device=query_lens.device)
-        positions, slots, seqlens, logits, context, count = buf.split_with_sizes((2 * T4, T4, n + 1, n, n, 1))
+        # one allocation; the token tensors first, each on a 16-byte boundary
+        gap = 2 * (max_tokens % 2)
+        buf = torch.empty(3 * max_tokens + gap + 3 * n + 2, dtype=torch.int32, device=query_lens.device)
+        positions, _, slots, seqlens, logits, context, count = buf.split_with_sizes(
+            (2 * max_tokens, gap, max_tokens, n + 1, n, n, 1))
         positions = positions.view(torch.int64)
-        if T4 != max_tokens:
-            positions, slots = positions[:max_tokens], slots[:max_tokens]
         out = StepTables(seqlens, positions, slots, logits, context, count)
     else:
         for t, count, dtype in ((out.seqlens_q, n + 1, torch.int32), (out.positions, max_tokens, torch.int64),

@@ -128,6 +128,14 @@ struct WindowTiles {
   __device__ __forceinline__ int tile(int i) const {
     return i < n_win ? first + n_win - 1 - i : n_sink - 1 - (i - n_win);
   }
+  // The 32-column chunks [c0, c1) of the i-th visited tile that hold every column some row sees: scores,
+  // probabilities and value rows outside them are neither computed nor read.
+  __device__ __forceinline__ void chunks(int i, int &c0, int &c1) const {
+    const int n0 = tile(i) * kBN;
+    const int hi = i < n_win ? lim : min(sinks, lo);
+    c1 = (min(hi - n0, kBN) + 31) / 32;
+    c0 = i < n_win && sinks <= n0 ? max(lo - n0, 0) / 32 : 0;
+  }
 };
 
 // Bit i: column cb + i is in [lo, hi) or [0, sinks), and below hi.
@@ -442,11 +450,31 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       else tc_commit(bar);
     };
     // S_t = Q_t K^T.  Q, K: K-major, rows of 128 B, 8-row groups 1024 B apart, two 64-column panels.
-    auto issue_s = [&](int t, int i_k) {
+    // (windowed: `ch` holds the tile's chunk range, worked out before the waits so that nothing but the
+    // instructions themselves lies between a barrier and its MMAs)
+    struct Chunks {
+      int c0 = 0, c1 = kBN / 32;
+      uint32_t idesc_s = 0;
+    };
+    auto chunks_of = [&](int j) {
+      Chunks ch;
+      if constexpr (kWindow) {
+        if (j < nmax) win.chunks(j, ch.c0, ch.c1);
+        ch.idesc_s = (idesc_s & ~(63u << 17)) | ((uint32_t)(4 * (ch.c1 - ch.c0)) << 17);  // N = 32 columns a chunk
+      }
+      return ch;
+    };
+    auto issue_s = [&](int t, int i_k, const Chunks &ch) {
       tc_fence_after();
       if (lane == 0) {
         const uint64_t qdesc = smem_desc_sw128(smem_u32(sQ + t * kTileBytes), 16, 1024);
-        const uint32_t kaddr = smem_u32(sKV + (i_k % kKvStages) * kStageBytes);
+        uint32_t kaddr = smem_u32(sKV + (i_k % kKvStages) * kStageBytes);
+        uint32_t s_col = tmem_base + t * 128;
+        const uint32_t idesc = kWindow ? ch.idesc_s : idesc_s;
+        if constexpr (kWindow) {
+          kaddr += ch.c0 * (kPaged ? 8192 : 4096);  // 32 key rows
+          s_col += 32 * ch.c0;
+        }
         const uint64_t kdesc = kPaged ? smem_desc(kaddr, 128, 2048, 0) : smem_desc_sw128(kaddr, 16, 1024);
 #pragma unroll
         for (int ks = 0; ks < kHD / 16; ++ks) {
@@ -454,7 +482,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           const uint64_t kadv = kPaged ? (uint64_t)((ks * 256) >> 4)
                                        : (uint64_t)(((ks >> 2) * kKPanel + (ks & 3) * 32) >> 4);
           if (kPair) umma_ss_pair(tmem_base + t * 128, qdesc + adv, kdesc + kadv, idesc_s, ks > 0 ? 1u : 0u);
-          else umma_ss(tmem_base + t * 128, qdesc + adv, kdesc + kadv, idesc_s, ks > 0 ? 1u : 0u);
+          else umma_ss(s_col, qdesc + adv, kdesc + kadv, idesc, ks > 0 ? 1u : 0u);
         }
         commit(&sh->s_full[t]);
       }
@@ -463,7 +491,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     // O_t += P_t V.  V as B operand: N (= d) contiguous, 64 d per swizzle atom, second atom one
     // panel further (leading offset), 8-token groups 1024 B apart (stride offset).  In a CTA pair
     // each CTA holds one atom (its 64 columns).
-    auto issue_pv = [&](int t, int i_v, bool first, bool last) {
+    auto issue_pv = [&](int t, int i_v, bool first, bool last, const Chunks &ch) {
       tc_fence_after();
       if (lane == 0) {
         const uint32_t vaddr = smem_u32(sKV + (i_v % kKvStages) * kStageBytes);
@@ -471,14 +499,20 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         // rows (d) of 32 B with the 32-byte swizzle, 8-row groups 256 B apart
         const uint64_t vdesc = kPaged ? smem_desc(vaddr, 16, 256, 6) : smem_desc_sw128(vaddr, kPanelBytes, 1024);
         const uint32_t vstep = kPaged ? 4096u : 2048u;
-#pragma unroll
-        for (int ks = 0; ks < kBN / 16; ++ks) {
+        auto step = [&](int ks, bool accumulate) {
           if (kPair)
             umma_ts_pair(tmem_base + kOCol + t * 128, tmem_base + t * 128 + 8 * ks,
-                         vdesc + (uint64_t)((ks * vstep) >> 4), idesc_pv, (!first || ks > 0) ? 1u : 0u);
+                         vdesc + (uint64_t)((ks * vstep) >> 4), idesc_pv, accumulate ? 1u : 0u);
           else
             umma_ts(tmem_base + kOCol + t * 128, tmem_base + t * 128 + 8 * ks, vdesc + (uint64_t)((ks * vstep) >> 4),
-                    idesc_pv, (!first || ks > 0) ? 1u : 0u);
+                    idesc_pv, accumulate ? 1u : 0u);
+        };
+        if (!kWindow || ch.c1 - ch.c0 == kBN / 32) {
+#pragma unroll
+          for (int ks = 0; ks < kBN / 16; ++ks) step(ks, !first || ks > 0);
+        } else {
+#pragma unroll 1
+          for (int ks = 2 * ch.c0; ks < 2 * ch.c1; ++ks) step(ks, !first || ks > 2 * ch.c0);
         }
         if (last) commit(&sh->o_full[t]);
       }
@@ -489,15 +523,17 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       __syncwarp();
     };
 
+    Chunks ch = chunks_of(0);
     if (nt0 > 0) wait_q(0);
     if (nt1 > 0) wait_q(1);
     if (wait_kv(0)) {
-      if (nt0 > 0) issue_s(0, 0);
-      if (nt1 > 0) issue_s(1, 0);
+      if (nt0 > 0) issue_s(0, 0, ch);
+      if (nt1 > 0) issue_s(1, 0, ch);
       release(0);
     }
     for (int j = 0; ok && j < nmax; ++j) {
       const int i_v = 2 * j + 1, i_kn = 2 * j + 2;
+      const Chunks ch_next = chunks_of(j + 1);
       if (!wait_kv(i_v)) break;
       if constexpr (kWindow) {
         // Value rows that no row of this query tile sees -- past its last row's position, or between the
@@ -571,22 +607,23 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       }
       if (j < nt0) {
         if (!wait_p(0, j)) break;
-        issue_pv(0, i_v, j == 0, j == nt0 - 1);
+        issue_pv(0, i_v, j == 0, j == nt0 - 1, ch);
       }
       if (j + 1 < nt0) {
         if (!wait_kv(i_kn)) break;
-        issue_s(0, i_kn);
+        issue_s(0, i_kn, ch_next);
       }
       if (j < nt1) {
         if (!wait_p(1, j)) break;
-        issue_pv(1, i_v, j == 0, j == nt1 - 1);
+        issue_pv(1, i_v, j == 0, j == nt1 - 1, ch);
       }
       release(i_v);
       if (j + 1 < nt1) {
         if (!wait_kv(i_kn)) break;
-        issue_s(1, i_kn);
+        issue_s(1, i_kn, ch_next);
       }
       if (j + 1 < nmax) release(i_kn);
+      ch = ch_next;
     }
     if (!ok && lane == 0) sh->aborted = 1;
   } else {
@@ -610,12 +647,144 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     float m_used = -INFINITY, m_next = -INFINITY, l_sum = 0.f;
     bool ok = true, pending = false;
 
+    // Windowed variant of the loop body below: the probabilities of the tile at key n0, visit j.  Whole
+    // tiles take the same single pass against the running reference; where a row has none yet, or some
+    // chunks hold no column that any row of the CTA sees (the diagonal, the sinks), the maximum comes first and
+    // only the 32-column chunks that some row of the warp sees are gone over.
+    auto window_tile = [&](int j, int n0, int c0, int c1, bool single_pass, bool full) {
+      if (single_pass) {
+        uint32_t pk[64];
+        uint32_t ra[32], rb[32];
+        uint64_t acc = pack_f32x2(0.f, 0.f);
+        const float ref = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t sc2 = pack_f32x2(sc, sc), nm2 = pack_f32x2(-ref, -ref);
+        tmem_ld32(t_s, ra);
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          tmem_wait_ld();
+          uint32_t(&cur)[32] = (c4 & 1) ? rb : ra;
+          uint32_t(&nxt)[32] = (c4 & 1) ? ra : rb;
+          if (c4 < 3) tmem_ld32(t_s + 32 * (c4 + 1), nxt);
+          if (full) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])), sc2, nm2), x0, x1);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              acc = add_f32x2(acc, pack_f32x2(p0, p1));
+              pk[16 * c4 + (i >> 1)] = Half16<T16>::pack(p0, p1);
+            }
+          } else {
+            const uint32_t vis = visible_bits(n0 + 32 * c4, lo_row, lim_row, win.sinks);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])), sc2, nm2), x0, x1);
+              const float p0 = fast_exp2((vis >> i) & 1u ? x0 : -INFINITY);
+              const float p1 = fast_exp2((vis >> (i + 1)) & 1u ? x1 : -INFINITY);
+              acc = add_f32x2(acc, pack_f32x2(p0, p1));
+              pk[16 * c4 + (i >> 1)] = Half16<T16>::pack(p0, p1);
+            }
+          }
+        }
+        float a0, a1;
+        unpack_f32x2(acc, a0, a1);
+        const float l_tile = a0 + a1;
+        if (!__any_sync(0xffffffffu, !(l_tile < kDanger))) {
+#pragma unroll
+          for (int c4 = 0; c4 < 4; ++c4)
+            tmem_st16(t_s + 16 * c4, *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * c4]));
+          l_sum += l_tile;
+          if (l_tile > kRescaleSum) {
+            pending = true;
+            m_next = m_used + __log2f(l_tile);
+          }
+          return;
+        }
+      }
+      uint32_t r[32];
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c4 = c0; c4 < c1; ++c4) {
+        const uint32_t vis = visible_bits(n0 + 32 * c4, lo_row, lim_row, win.sinks);
+        if (!__any_sync(0xffffffffu, vis != 0u)) continue;
+        tmem_ld32(t_s + 32 * c4, r);
+        tmem_wait_ld();
+        if (vis == ~0u) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if ((vis >> i) & 1u) mx = fmaxf(mx, __uint_as_float(r[i]));
+        }
+      }
+      mx *= sc;  // scale > 0 keeps the order
+      if (j == 0) {
+        m_used = mx;
+      } else {
+        const bool need = mx > m_used + kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          float alpha = 1.f;
+          if (need) {
+            alpha = fast_exp2(m_used - mx);  // 0 when nothing was visible so far
+            m_used = mx;
+            l_sum *= alpha;
+          }
+#pragma unroll 1
+          for (int c4 = 0; c4 < 4; ++c4) {
+            tmem_ld32(t_o + 32 * c4, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st32(t_o + 32 * c4, r);
+          }
+          tmem_wait_st();
+        }
+      }
+      const float base = m_used == -INFINITY ? 0.f : m_used;
+      const uint64_t sc2 = pack_f32x2(sc, sc), nb2 = pack_f32x2(-base, -base);
+      uint64_t acc = pack_f32x2(0.f, 0.f);
+#pragma unroll 1
+      for (int c4 = c0; c4 < c1; ++c4) {  // ascending: P of a chunk lands on scores already read
+        const uint32_t vis = visible_bits(n0 + 32 * c4, lo_row, lim_row, win.sinks);
+        uint32_t out[16];
+        if (__any_sync(0xffffffffu, vis != 0u)) {
+          tmem_ld32(t_s + 32 * c4, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc2, nb2), x0, x1);
+            const float p0 = fast_exp2((vis >> i) & 1u ? x0 : -INFINITY);
+            const float p1 = fast_exp2((vis >> (i + 1)) & 1u ? x1 : -INFINITY);
+            acc = add_f32x2(acc, pack_f32x2(p0, p1));
+            out[i >> 1] = Half16<T16>::pack(p0, p1);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) out[i] = 0u;
+        }
+        tmem_st16(t_s + 16 * c4, out);
+      }
+      float a0, a1;
+      unpack_f32x2(acc, a0, a1);
+      l_sum += a0 + a1;
+    };
+
     for (int j = 0; j < T.n_tiles; ++j) {
+      const int n0 = tile_of(j) * kBN;
+      int c0 = 0, c1 = 0;
+      bool single_pass = false, full = false;
+      if constexpr (kWindow) {  // all that does not depend on the scores, while they are computed
+        win.chunks(j, c0, c1);
+        single_pass = c1 - c0 == kBN / 32 && !__any_sync(0xffffffffu, sees && m_used == -INFINITY);
+        full = n0 + kBN <= lim_row && (n0 >= lo_row || n0 + kBN <= win.sinks);
+      }
       ok = mbar_wait_abortable(&sh->s_full[t], (uint32_t)j & 1u, p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int n0 = tile_of(j) * kBN;
       // A rescale that the previous tile found necessary but left for now: the previous P V has
       // completed (s_full of this tile is committed after it), so O can be touched.
       if (__any_sync(0xffffffffu, pending)) {
@@ -638,14 +807,13 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         tmem_wait_st();
       }
 
-      const bool full_tile =
-          n0 + kBN <= lim_row && (!kWindow || n0 >= lo_row || n0 + kBN <= win.sinks);
+      if constexpr (kWindow) {
+        window_tile(j, n0, c0, c1, single_pass, full);
+      } else {
+      const bool full_tile = n0 + kBN <= lim_row;
       // rows that have not seen a single column so far have no reference yet: exact path, except on
       // the first tile, which takes its reference from its own first 32 columns (below)
-      // (windowed: the columns a row sees in its first tile are no prefix, so that tile is exact too, and
-      // so are the next ones while some row of the warp has seen nothing)
-      bool exact_path = kWindow ? __any_sync(0xffffffffu, sees && m_used == -INFINITY)
-                                : (j > 0) && __any_sync(0xffffffffu, m_used == -INFINITY);
+      bool exact_path = (j > 0) && __any_sync(0xffffffffu, m_used == -INFINITY);
       if (!exact_path) {
         // ---- single pass against the running reference m_used --------------------------------
         // P is computed for the whole row in registers while S is still intact; if some score
@@ -657,7 +825,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         float l0 = 0.f, l1 = 0.f;
         uint64_t acc2 = pack_f32x2(0.f, 0.f);
         tmem_ld32(t_s, ra);
-        if (!kWindow && j == 0) {
+        if (j == 0) {
           // First tile: the reference is the largest visible score among the first 32 columns (the
           // visible columns of a row are a prefix, so a row that sees nothing here sees nothing in
           // the tile).  If the rest of the tile lies far above it, the row sum says so as usual.
@@ -689,14 +857,13 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
             }
           } else {
             const int cb = n0 + 32 * c4;
-            const uint32_t vis = kWindow ? visible_bits(cb, lo_row, lim_row, win.sinks) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const uint64_t x = fma_f32x2(pack_f32x2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1])), sc2, nm2);
               float x0, x1;
               unpack_f32x2(x, x0, x1);
-              const float p0 = fast_exp2((kWindow ? (vis >> i) & 1u : cb + i < lim_row) ? x0 : -INFINITY);
-              const float p1 = fast_exp2((kWindow ? (vis >> (i + 1)) & 1u : cb + i + 1 < lim_row) ? x1 : -INFINITY);
+              const float p0 = fast_exp2((cb + i < lim_row) ? x0 : -INFINITY);
+              const float p1 = fast_exp2((cb + i + 1 < lim_row) ? x1 : -INFINITY);
               acc2 = add_f32x2(acc2, pack_f32x2(p0, p1));
               pk[16 * c4 + (i >> 1)] = Half16<T16>::pack(p0, p1);
             }
@@ -736,14 +903,9 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           tmem_ld32(t_s + 32 * c4, r);
           tmem_wait_ld();
           const int cb = n0 + 32 * c4;
-          if (full_tile || (!kWindow && cb + 32 <= lim_row)) {
+          if (cb + 32 <= lim_row) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-          } else if (kWindow) {
-            const uint32_t vis = visible_bits(cb, lo_row, lim_row, win.sinks);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((vis >> i) & 1u) mx = fmaxf(mx, __uint_as_float(r[i]));
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -784,7 +946,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           tmem_wait_ld();
           const int cb = n0 + 32 * c4;
           uint32_t pk[16];
-          if (full_tile || (!kWindow && cb + 32 <= lim_row)) {
+          if (cb + 32 <= lim_row) {
             const uint64_t sc2 = pack_f32x2(sc, sc), nb2 = pack_f32x2(-base, -base);
             uint64_t acc2 = pack_f32x2(0.f, 0.f);
 #pragma unroll
@@ -799,19 +961,17 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
             unpack_f32x2(acc2, a0, a1);
             l_sum += a0 + a1;
           } else {
-            const uint32_t vis = kWindow ? visible_bits(cb, lo_row, lim_row, win.sinks) : 0u;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const bool v0 = kWindow ? (vis >> i) & 1u : cb + i < lim_row;
-              const bool v1 = kWindow ? (vis >> (i + 1)) & 1u : cb + i + 1 < lim_row;
-              const float p0 = v0 ? fast_exp2(fmaf(__uint_as_float(r[i]), sc, -base)) : 0.f;
-              const float p1 = v1 ? fast_exp2(fmaf(__uint_as_float(r[i + 1]), sc, -base)) : 0.f;
+              const float p0 = (cb + i < lim_row) ? fast_exp2(fmaf(__uint_as_float(r[i]), sc, -base)) : 0.f;
+              const float p1 = (cb + i + 1 < lim_row) ? fast_exp2(fmaf(__uint_as_float(r[i + 1]), sc, -base)) : 0.f;
               l_sum += p0 + p1;
               pk[i >> 1] = Half16<T16>::pack(p0, p1);
             }
           }
           tmem_st16(t_s + 16 * c4, pk);
         }
+      }
       }
       tmem_wait_st();
       tc_fence_before();
@@ -1088,7 +1248,7 @@ static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk,
                                    int max_seqlen_k, cudaStream_t stream) {
   p.pair_heads = 0;
   const int64_t keys = (int64_t)p.window + p.sinks;
-  if (p.group % 2 != 0 || (keys < max_seqlen_k ? keys : max_seqlen_k) <= AICI_PREFILL_ONE_TILE_MAX_K)
+  if (p.group % 2 != 0 || (!kPaged && (keys < max_seqlen_k ? keys : max_seqlen_k) <= AICI_PREFILL_ONE_TILE_MAX_K))
     return launch_prefill_shape<kPaged, 1, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
   return launch_prefill_shape<kPaged, 2, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
 }
