@@ -45,27 +45,25 @@ EXPORTS = (
     "aici_rotary_cos_sin_cache",
     "aici_rotary_embedding",
     "aici_rotary_embedding_and_cache",
-    "aici_paged_attention_window_workspace_bytes",
     "aici_paged_attention_window",
     "aici_mha_varlen_window_fwd",
     "aici_mha_varlen_paged_window_fwd",
 )
 
 # Parameter lists of entry points whose callers hand plain Python numbers to ctypes: p = pointer,
-# i = int, l = int64_t, z = size_t, f = float, d = double.  (Short calls: converting at the call costs
+# i = int, l = int64_t, f = float, d = double.  (Short calls: converting at the call costs
 # more host time than the kernel runs.)
 _PARAMETERS = {
     "aici_step_tables": "ppppp" "ii" "l" "i" "l" "ii" "pppppp" "p",
     "aici_rotary_cos_sin_cache": "plidi" "dli" "p",
     "aici_rotary_embedding": "pppp" "iiiiii" "lll" "ii" "p",
     "aici_rotary_embedding_and_cache": "pppppppp" "iiiiiii" "l" "i" "llll" "ii" "p",
-    "aici_paged_attention_window_workspace_bytes": "iiiiii",
-    "aici_paged_attention_window": "pppp" "if" "pp" "iiiiiiii" "llll" "pzi" "p",
+    "aici_paged_attention_window": "pppp" "if" "pp" "iiiiiiii" "llll" "i" "p",
     "aici_mha_varlen_window_fwd": "pppppp" "iiiiiiiiii" "llllllll" "fi" "p",
     "aici_mha_varlen_paged_window_fwd": "ppppppp" "iiiiiiiii" "l" "ii" "llllll" "fi" "p",
 }
-_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "z": ctypes.c_size_t,
-           "f": ctypes.c_float, "d": ctypes.c_double}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float,
+           "d": ctypes.c_double}
 
 _lib = None
 
@@ -86,12 +84,10 @@ def lib() -> ctypes.CDLL:
         _lib.aici_version.restype = ctypes.c_char_p
         _lib.aici_paged_attention_workspace_bytes.restype = ctypes.c_size_t
         _lib.aici_paged_attention_chunked_workspace_bytes.restype = ctypes.c_size_t
-        _lib.aici_paged_attention_window_workspace_bytes.restype = ctypes.c_size_t
         for name in EXPORTS:
             fn = getattr(_lib, name)
             if name not in ("aici_version", "aici_paged_attention_workspace_bytes",
-                            "aici_paged_attention_chunked_workspace_bytes",
-                            "aici_paged_attention_window_workspace_bytes"):
+                            "aici_paged_attention_chunked_workspace_bytes"):
                 fn.restype = ctypes.c_void_p  # char*, released with free()
             if name in _PARAMETERS:
                 fn.argtypes = [_CTYPES[c] for c in _PARAMETERS[name]]

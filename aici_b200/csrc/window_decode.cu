@@ -14,12 +14,15 @@
 // query-head group against a tile with mma.sync (heads are the rows of the fragment; 16 rows when a kv
 // head has more than 8 query heads) and keeps the softmax state in registers.
 //
-// Two ways of dealing out the work:
-//   cluster   few rows: 1 to 8 CTAs of a cluster share a row, tile i going to warp i mod warps, and
-//             join their results through distributed shared memory.  One launch, no workspace.
-//   spans     many rows: all tiles of the batch laid end to end, every warp of two CTAs per SM takes an
-//             equal run, whatever the mix of context lengths; rows cut by a run's border leave fp32
-//             partials that a second kernel joins.
+// A row belongs to one CTA, or, when rows are few, to a cluster of 2, 4 or 8: tile i goes to warp
+// i mod warps, the warps join their results through shared memory and the CTAs through distributed
+// shared memory.  One launch, no workspace.  With a window rows are much alike, and the CTAs of the
+// kv heads of a sequence, started next to each other, read neighbouring 4 KB pieces of the same blocks:
+// 1024 rows of 257 tiles take 311 us (6.9 TB/s), against 340 us when all tiles of the batch are cut into
+// equal runs for resident warps and a second kernel joins the cut rows (256 rows: 88 against 94 us; 8 rows,
+// cluster of 8: 9.8 against 24 us).  What that other form is better at is a batch with one row far longer
+// than the rest: a CTA alone streams a tile in 0.19 us, so the last row to start costs at most that
+// times its tiles.
 #include "half_types.cuh"
 
 namespace aici {
@@ -31,8 +34,6 @@ constexpr int kWinStageBytes = 2 * kWinTileBytes;  // key tile and value tile
 constexpr int kWinWarps = 4;
 constexpr int kWinStages = 3;  // 72 KB of ring in flight per SM and CTA pair: enough for the bandwidth-latency product
 constexpr int kWinThreads = kWinWarps * 32;
-constexpr int kWinSeqs = 1024;     // sequences of one launch (their lengths are summed in shared memory)
-constexpr int kWinMinSpan = 4;     // tiles: fewer would make partials a large share of the traffic
 constexpr int kWinRingBytes = kWinWarps * kWinStages * kWinStageBytes;
 constexpr int kWinBarBytes = 128;  // kWinWarps * kWinStages barriers
 
@@ -44,9 +45,6 @@ struct WindowDecodeParams {
   int64_t num_blocks, q_stride, kv_block;
   float scale_log2e;
   unsigned int *status;
-  // spans
-  int *span_cum;  // [num_seqs + 2] tiles before each sequence, then the span
-  float *part_m, *part_l, *part_o;
 };
 
 // The visible part of a row.
@@ -224,7 +222,6 @@ __device__ __forceinline__ int block_id(const WindowDecodeParams &p, int seq, in
   return id;
 }
 
-// ---- cluster ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t cta) {
   uint32_t remote;
   float4 v;
@@ -241,7 +238,7 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t local, uint32_t cta) {
 }
 
 template <typename T, bool kTwo>
-__global__ void __launch_bounds__(kWinThreads, 2) window_decode_cluster_kernel(const WindowDecodeParams p) {
+__global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const WindowDecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kHeads = kTwo ? 16 : 8;
   // what a warp leaves for its CTA lies in its own ring; what the CTA leaves for the cluster behind the rings
@@ -372,198 +369,6 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_cluster_kernel(c
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// ---- spans -----------------------------------------------------------------------------------------
-// Some consecutive tiles of one row.  Row (seq, kvh) starts at tile num_kv_heads * cum[seq] + kvh *
-// tiles(seq) of the batch; a warp's span is cut into pieces at row ends.  Piece number x / span + row
-// index (x = its first tile) is unique, below warps + rows, and consecutive within a row: the joining
-// kernel finds a row's partials without a list.
-struct WindowPiece {
-  WindowRow row;
-  int seq, kvh, i0, n;
-  bool whole;   // the row has no other piece
-  int64_t part; // first head's partial
-};
-
-__device__ __forceinline__ bool next_piece(const WindowDecodeParams &p, const int *s_cum, const int *s_ctx, int span,
-                                           int &x, int end, int cap, WindowPiece &it) {
-  if (x >= end) return false;
-  const int e = x / p.num_kv_heads;
-  int lo = 0, hi = p.num_seqs;
-  while (hi - lo > 1) {  // the last sequence that begins at or before e (empty ones share their successor's start)
-    const int mid = (lo + hi) >> 1;
-    if (s_cum[mid] <= e) lo = mid;
-    else hi = mid;
-  }
-  it.row = window_row(p, s_ctx[lo]);
-  const int rem = x - p.num_kv_heads * s_cum[lo];
-  it.seq = lo;
-  it.kvh = rem / it.row.tiles;
-  it.i0 = rem - it.kvh * it.row.tiles;
-  it.n = min(min(it.row.tiles - it.i0, end - x), cap);
-  const int begin = x - it.i0;  // the row's first tile
-  it.whole = (begin + it.row.tiles - 1) / span == begin / span;
-  it.part = (int64_t)(x / span + lo * p.num_kv_heads + it.kvh) * p.group;
-  x += it.n;
-  return true;
-}
-
-template <typename T, bool kTwo>
-__global__ void __launch_bounds__(kWinThreads, 2) window_decode_spans_kernel(const WindowDecodeParams p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, tig = lane & 3;
-  uint8_t *ring = smem + warp * (kWinStages * kWinStageBytes);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kWinRingBytes) + warp * kWinStages;
-  int *s_cum = reinterpret_cast<int *>(smem + kWinRingBytes + kWinBarBytes);
-  int *s_ctx = s_cum + p.num_seqs + 1;
-  if (lane == 0) {
-#pragma unroll
-    for (int s = 0; s < kWinStages; ++s) mbar_init(&full[s], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  // tiles before each sequence: every CTA reads all lengths at once and sums them for itself
-  for (int s = threadIdx.x; s < p.num_seqs; s += kWinThreads) {
-    const int ctx = p.context_lens[s];
-    s_ctx[s] = ctx;
-    s_cum[s + 1] = window_row(p, ctx).tiles;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
-      int incl = s0 + lane < p.num_seqs ? s_cum[s0 + lane + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (s0 + lane < p.num_seqs) s_cum[s0 + lane + 1] = carry + incl;
-      carry += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (lane == 0) s_cum[0] = 0;
-  }
-  __syncthreads();
-  const int total = s_cum[p.num_seqs] * p.num_kv_heads;
-  const int warps = gridDim.x * kWinWarps;
-  const int span = max((total + warps - 1) / warps, kWinMinSpan);
-  const int64_t x0 = (int64_t)(blockIdx.x * kWinWarps + warp) * span;
-  const int begin = x0 < total ? (int)x0 : total, end = x0 + span < total ? (int)(x0 + span) : total;
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i <= p.num_seqs; i += kWinThreads) p.span_cum[i] = s_cum[i];
-    if (threadIdx.x == 0) p.span_cum[p.num_seqs + 1] = span;
-  }
-
-  // producer: runs ahead of the consumer across pieces, 32 tiles' block ids at a time
-  WindowPiece pp;
-  pp.n = 0;
-  int px = begin, pt = 0, ids = 0;
-  unsigned issued = 0;
-  bool p_done = false;
-  auto produce = [&]() {
-    if (p_done) return;
-    if (pt == pp.n) {
-      if (!next_piece(p, s_cum, s_ctx, span, px, end, 32, pp)) {
-        p_done = true;
-        return;
-      }
-      if (lane < pp.n) ids = block_id(p, pp.seq, pp.row.block(pp.i0 + lane));
-      pt = 0;
-    }
-    const int blk = __shfl_sync(0xffffffffu, ids, pt);
-    if (lane == 0) issue_tile<T>(p, ring, full, issued, blk, pp.kvh);
-    ++pt;
-    ++issued;
-  };
-#pragma unroll
-  for (int s = 0; s < kWinStages - 1; ++s) produce();
-
-  unsigned done = 0;
-  int cx = begin;
-  bool ok = true;
-  WindowPiece it;
-  while (ok && next_piece(p, s_cum, s_ctx, span, cx, end, 0x7fffffff, it)) {
-    GroupState<T, kTwo> st;
-    st.load(p, it.seq, it.kvh, g, tig);
-    for (int t = 0; t < it.n; ++t) {
-      produce();
-      const unsigned stage = done % kWinStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (done / kWinStages) & 1u, p.status));
-      if (!ok) break;
-      const uint32_t kbase = smem_u32(ring + stage * kWinStageBytes);
-      st.tile(kbase, kbase + kWinTileBytes, it.row.block(it.i0 + t) * kWinBlock, it.row, p.scale_log2e, lane, tig);
-      __syncwarp();
-      ++done;
-    }
-    if (!ok) break;
-    st.finish();
-#pragma unroll
-    for (int r = 0; r < GroupState<T, kTwo>::kRows; ++r) {
-      const int h = g + 8 * r;
-      if (h >= p.group) continue;
-      const float inv = inverse(st.l[r]);
-      if (it.whole) {
-        T *dst = static_cast<T *>(p.out) + ((int64_t)it.seq * p.num_heads + it.kvh * p.group + h) * kWinHead + 2 * tig;
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-          *reinterpret_cast<uint32_t *>(dst + 8 * n) = Half16<T>::pack(st.o[n][2 * r] * inv, st.o[n][2 * r + 1] * inv);
-      } else {
-        if (tig == 0) {
-          p.part_m[it.part + h] = st.m[r];
-          p.part_l[it.part + h] = st.l[r];
-        }
-        float *dst = p.part_o + (it.part + h) * kWinHead + 2 * tig;
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-          *reinterpret_cast<float2 *>(dst + 8 * n) = make_float2(st.o[n][2 * r], st.o[n][2 * r + 1]);
-      }
-    }
-  }
-  if (!ok)
-    for (unsigned c = done; c != issued; ++c) mbar_wait(&full[c % kWinStages], (c / kWinStages) & 1u, p.status);
-}
-
-// Joins the partials of the rows that spans cut: one warp per (sequence, head), four elements to a lane.
-template <typename T>
-__global__ void __launch_bounds__(256) window_join_kernel(const WindowDecodeParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, idx = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (idx >= p.num_seqs * p.num_heads) return;
-  const int seq = idx / p.num_heads, head = idx - seq * p.num_heads;
-  const int kvh = head / p.group, h = head - kvh * p.group;
-  const int c0 = p.span_cum[seq], tiles = p.span_cum[seq + 1] - c0, span = p.span_cum[p.num_seqs + 1];
-  T *out = static_cast<T *>(p.out) + (int64_t)idx * kWinHead + 4 * lane;
-  if (tiles == 0) {  // an empty context: no warp came by this row
-    *reinterpret_cast<uint2 *>(out) = make_uint2(0u, 0u);
-    return;
-  }
-  const int g0 = p.num_kv_heads * c0 + kvh * tiles;
-  const int n = (g0 + tiles - 1) / span - g0 / span + 1;
-  if (n == 1) return;
-  const int64_t base = (int64_t)(g0 / span + seq * p.num_kv_heads + kvh) * p.group + h;
-  float m = -INFINITY;
-  for (int j = lane; j < n; j += 32) m = fmaxf(m, p.part_m[base + (int64_t)j * p.group]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const int64_t at = base + (int64_t)j * p.group;
-    const float f = fast_exp2(p.part_m[at] - ref);
-    const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * kWinHead + 4 * lane);
-    l += f * p.part_l[at];
-    a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
-  }
-  const float inv = inverse(l);
-  *reinterpret_cast<uint2 *>(out) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
-}
-
 // ---- host side -----------------------------------------------------------------------------------------
 // Most tiles a row can have.
 static int64_t most_tiles(int64_t max_context, int64_t window, int64_t sinks) {
@@ -572,104 +377,41 @@ static int64_t most_tiles(int64_t max_context, int64_t window, int64_t sinks) {
   return seen < all ? seen : all;
 }
 
-// CTAs that share a row in the cluster form, 0 = spans.
-static int cluster_ctas(int num_seqs, int num_kv_heads, int64_t tiles) {
-  const int64_t rows = (int64_t)num_seqs * num_kv_heads, places = 2 * sm_count();
-  if (rows > places) return 0;
+// CTAs that share a row: as many as keep all rows resident at once, and no more than have tiles to
+// work on.  (64 rows of 65 tiles: 14.2, 9.7, 8.2 us with 1, 2, 4 CTAs and 12.6 with 8, two waves; 8 rows of
+// 4 tiles: 2.8 us with one CTA, 4.0 with any cluster.)
+static int ctas_per_row(int64_t rows, int64_t tiles) {
   int c = 1;
-  while (c < 8 && rows * 2 * c <= places && tiles > (int64_t)c * kWinWarps) c *= 2;
+  while (c < 8 && rows * 2 * c <= 2 * sm_count() && tiles > (int64_t)c * kWinWarps) c *= 2;
   return c;
 }
 
-// Sequences of one launch of the span form: 32-bit tile numbers, lengths in shared memory.
-static int span_seqs(int num_kv_heads, int64_t tiles) {
-  const int64_t fit = (1ll << 30) / (num_kv_heads * (tiles + 1));
-  return (int)(fit < 1 ? 1 : fit < kWinSeqs ? fit : kWinSeqs);
-}
-
-struct WindowWorkspace {
-  size_t m_off, l_off, o_off, total;
-};
-
-static WindowWorkspace window_workspace(int num_seqs, int num_heads, int num_kv_heads) {
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  const size_t pieces = (size_t)2 * sm_count() * kWinWarps + (size_t)num_seqs * num_kv_heads;
-  const size_t parts = pieces * (num_heads / num_kv_heads);
-  WindowWorkspace w;
-  w.m_off = up((size_t)(num_seqs + 2) * sizeof(int));
-  w.l_off = w.m_off + up(parts * sizeof(float));
-  w.o_off = w.l_off + up(parts * sizeof(float));
-  w.total = w.o_off + parts * kWinHead * sizeof(float);
-  return w;
-}
-
-static size_t window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int64_t tiles) {
-  if (cluster_ctas(num_seqs, num_kv_heads, tiles) > 0) return 0;
-  const int part = span_seqs(num_kv_heads, tiles);
-  return window_workspace(num_seqs < part ? num_seqs : part, num_heads, num_kv_heads).total;
-}
-
 template <typename T, bool kTwo>
-static char *launch_window_decode(WindowDecodeParams p, int64_t tiles, char *workspace, cudaStream_t stream) {
-  constexpr int kClusterSmem = kWinRingBytes + kWinBarBytes + (kTwo ? 16 : 8) * (kWinHead * 4 + 8 + kWinWarps * 8);
-  constexpr int kSpanSmem = kWinRingBytes + kWinBarBytes + (2 * kWinSeqs + 1) * (int)sizeof(int);
+static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStream_t stream) {
+  constexpr int kSmem = kWinRingBytes + kWinBarBytes + (kTwo ? 16 : 8) * (kWinHead * 4 + 8 + kWinWarps * 8);
   static OncePerDevice once;
   if (char *e = once.run([]() -> char * {
-        AICI_CUDA(cudaFuncSetAttribute(window_decode_cluster_kernel<T, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kClusterSmem));
-        AICI_CUDA(cudaFuncSetAttribute(window_decode_spans_kernel<T, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSpanSmem));
-        // the same shared-memory split for the joining kernel, so that its CTAs can start on SMs that still
-        // run the kernel before it
-        AICI_CUDA(cudaFuncSetAttribute(window_join_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                       cudaSharedmemCarveoutMaxShared));
+        AICI_CUDA(cudaFuncSetAttribute(window_decode_kernel<T, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         return nullptr;
       }))
     return e;
-  // programmatic dependents: a kernel's prologue overlaps the tail of the one before it, and each waits for
-  // it before it touches anything
+  // a programmatic dependent: its prologue overlaps the tail of the grid before it, and it waits for
+  // that grid before it touches anything
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.num_seqs * p.num_kv_heads * ctas));
+  cfg.blockDim = dim3(kWinThreads);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cfg.blockDim = dim3(kWinThreads);
-  const int ctas = cluster_ctas(p.num_seqs, p.num_kv_heads, tiles);
-  if (ctas > 0) {
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
-    cfg.gridDim = dim3(p.num_seqs * p.num_kv_heads * ctas);
-    cfg.dynamicSmemBytes = kClusterSmem;
-    AICI_CUDA(cudaLaunchKernelEx(&cfg, window_decode_cluster_kernel<T, kTwo>, p));
-    return nullptr;
-  }
-  const int all = p.num_seqs, part = span_seqs(p.num_kv_heads, tiles);
-  const WindowWorkspace w = window_workspace(all < part ? all : part, p.num_heads, p.num_kv_heads);
-  p.span_cum = reinterpret_cast<int *>(workspace);
-  p.part_m = reinterpret_cast<float *>(workspace + w.m_off);
-  p.part_l = reinterpret_cast<float *>(workspace + w.l_off);
-  p.part_o = reinterpret_cast<float *>(workspace + w.o_off);
-  for (int s0 = 0; s0 < all; s0 += part) {  // one after the other on the stream, in the same workspace
-    WindowDecodeParams c = p;
-    c.num_seqs = all - s0 < part ? all - s0 : part;
-    c.out = static_cast<T *>(p.out) + (int64_t)s0 * p.num_heads * kWinHead;
-    c.q = static_cast<const T *>(p.q) + s0 * p.q_stride;
-    c.block_tables = p.block_tables + (int64_t)s0 * p.max_blocks;
-    c.context_lens = p.context_lens + s0;
-    const int64_t most = (int64_t)c.num_seqs * c.num_kv_heads * tiles;
-    const int64_t need = (most + kWinWarps * kWinMinSpan - 1) / (kWinWarps * kWinMinSpan);
-    cfg.gridDim = dim3((unsigned)(need < 1 ? 1 : need < 2 * sm_count() ? need : 2 * sm_count()));
-    cfg.blockDim = dim3(kWinThreads);
-    cfg.dynamicSmemBytes = kWinRingBytes + kWinBarBytes + (2 * c.num_seqs + 1) * sizeof(int);
-    AICI_CUDA(cudaLaunchKernelEx(&cfg, window_decode_spans_kernel<T, kTwo>, c));
-    cfg.gridDim = dim3((c.num_seqs * c.num_heads + 7) / 8);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    AICI_CUDA(cudaLaunchKernelEx(&cfg, window_join_kernel<T>, c));
-  }
+  cfg.numAttrs = 2;
+  AICI_CUDA(cudaLaunchKernelEx(&cfg, window_decode_kernel<T, kTwo>, p));
   return nullptr;
 }
 
@@ -677,20 +419,13 @@ static char *launch_window_decode(WindowDecodeParams p, int64_t tiles, char *wor
 
 using namespace aici;
 
-extern "C" size_t aici_paged_attention_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
-                                                              int max_context_len, int window, int sinks) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0 || window < 1 || sinks < 0) return 0;
-  return window_workspace_bytes(num_seqs, num_heads, num_kv_heads, most_tiles(max_context_len, window, sinks));
-}
-
 extern "C" char *aici_paged_attention_window(void *out, const void *query, const void *key_cache,
                                              const void *value_cache, int num_kv_heads, float scale,
                                              const int32_t *block_tables, const int32_t *context_lens,
                                              int block_size, int max_context_len, int window, int sinks, int num_seqs,
                                              int num_heads, int head_size, int max_num_blocks_per_seq,
                                              int64_t num_blocks, int64_t q_stride, int64_t kv_block_stride,
-                                             int64_t kv_head_stride, void *workspace, size_t workspace_bytes,
-                                             int dtype, aici_stream_t stream) {
+                                             int64_t kv_head_stride, int dtype, aici_stream_t stream) {
   const char *fn = "aici_paged_attention_window";
   AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn, dtype);
   AICI_CHECK(head_size == kWinHead, "%s: head_size must be 128 (got %d)", fn, head_size);
@@ -715,12 +450,6 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
   AICI_CHECK(((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache) % 16 == 0,
              "%s: tensors must be 16-byte aligned", fn);
   if (char *e = check_on_current_device(fn, "query", query)) return e;
-  const int64_t tiles = most_tiles(max_context_len, window, sinks);
-  AICI_CHECK(num_kv_heads * (tiles + 1) <= (1ll << 30), "%s: max_context_len too large", fn);
-  const size_t need = window_workspace_bytes(num_seqs, num_heads, num_kv_heads, tiles);
-  AICI_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need),
-             "%s: workspace too small (%zu bytes given, %zu needed)", fn, workspace_bytes, need);
-  AICI_CHECK(need == 0 || (uintptr_t)workspace % 256 == 0, "%s: workspace must be 256-byte aligned", fn);
   unsigned int *st = status_ptr();
   AICI_CHECK(st != nullptr, "%s: no CUDA device", fn);
   WindowDecodeParams p = {};
@@ -744,9 +473,9 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
   p.scale_log2e = scale * 1.4426950408889634f;
   p.status = st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  char *ws = static_cast<char *>(workspace);
+  const int ctas = ctas_per_row((int64_t)num_seqs * num_kv_heads, most_tiles(max_context_len, window, sinks));
   return with_half_type(dtype, [&](auto t) -> char * {
     using T = decltype(t);
-    return group > 8 ? launch_window_decode<T, true>(p, tiles, ws, s) : launch_window_decode<T, false>(p, tiles, ws, s);
+    return group > 8 ? launch_window_decode<T, true>(p, ctas, s) : launch_window_decode<T, false>(p, ctas, s);
   });
 }

@@ -858,30 +858,10 @@ def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: to
         raise AiciError("%s: dtypes differ" % fn)
     num_seqs, num_heads, _ = shape
     _check_table(fn, block_tables, context_lens, num_seqs)
-    window, sinks = _int32(window), _int32(sinks)
-    nbytes = _window_workspace_bytes(index, num_seqs, num_heads, num_kv_heads, max_context_len, window, sinks)
-    ws = _window_workspace(index, nbytes) if nbytes else None
     _call(fn, "aici_paged_attention_window", index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(),
           value_cache.data_ptr(), num_kv_heads, scale, block_tables.data_ptr(), context_lens.data_ptr(), block_size,
-          max_context_len, window, sinks, num_seqs, num_heads, head_size, block_tables.shape[1], num_blocks,
-          stride[0], key_cache.stride(0), key_cache.stride(1), ws.data_ptr() if nbytes else None, nbytes,
-          _dtype(fn, query))
-
-
-def _window_workspace_bytes(index: int, *sizes) -> int:
-    # the size depends on the GPU's number of multiprocessors
-    if torch._C._cuda_getDevice() == index:
-        return _lib.lib().aici_paged_attention_window_workspace_bytes(*sizes)
-    with torch.cuda.device(index):
-        return _lib.lib().aici_paged_attention_window_workspace_bytes(*sizes)
-
-
-def _window_workspace(index: int, nbytes: int) -> torch.Tensor:
-    """The stream's scratch; a captured call gets one of its own, since graphs may run at the same time."""
-    dev = torch.device("cuda", index)
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return _workspace(dev, nbytes)
+          max_context_len, _int32(window), _int32(sinks), num_seqs, num_heads, head_size, block_tables.shape[1],
+          num_blocks, stride[0], key_cache.stride(0), key_cache.stride(1), _dtype(fn, query))
 
 
 def _check_prefill(fn, q, seqlens_q):

@@ -500,17 +500,14 @@ char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, voi
  * Decode over the paged cache, arguments as in aici_paged_attention_v1: one query per sequence at
  * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number.  Blocks that hold no
  * visible token are not read (their table entries may be anything), and tokens that are not visible
- * may hold anything, NaN included.  `workspace` as there, of the size that
- * aici_paged_attention_window_workspace_bytes gives; calls that overlap on the GPU need one each. */
-size_t aici_paged_attention_window_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
-                                                   int max_context_len, int window, int sinks);
+ * may hold anything, NaN included.  No workspace. */
 char *aici_paged_attention_window(void *out, const void *query, const void *key_cache,
                                   const void *value_cache, int num_kv_heads, float scale,
                                   const int32_t *block_tables, const int32_t *context_lens, int block_size,
                                   int max_context_len, int window, int sinks, int num_seqs, int num_heads,
                                   int head_size, int max_num_blocks_per_seq, int64_t num_blocks,
                                   int64_t q_stride, int64_t kv_block_stride, int64_t kv_head_stride,
-                                  void *workspace, size_t workspace_bytes, int dtype, aici_stream_t stream);
+                                  int dtype, aici_stream_t stream);
 
 /* Prefill over packed keys and values (arguments as in aici_mha_varlen_fwd) and over the paged cache
  * (as in aici_mha_varlen_paged_fwd); row r of a sequence is the token at position len_k - len_q + r, any

@@ -59,7 +59,7 @@ def test_table_refuses(lib, change, match):
 
 
 DEC = dict(out=P, q=P, kc=P, vc=P, Hk=2, scale=0.1, bt=P, cl=P, block=16, maxctx=64, window=8, sinks=0, n=2, H=8, D=128,
-           mb=4, nb=8, qs=1024, bs=4096, hs=2048, ws=P, wsb=1 << 30, dt=0, s=None)
+           mb=4, nb=8, qs=1024, bs=4096, hs=2048, dt=0, s=None)
 DECODE_REFUSALS = [
     (dict(dt=2), "only bf16 and f16"), (dict(D=64), "head_size"), (dict(block=32), "block_size"), (dict(H=7), "not divisible"),
     (dict(H=34, qs=8192), "at most 16"), (dict(window=0), "window"), (dict(window=-3), "window"), (dict(sinks=-1), "sinks"),
@@ -127,13 +127,6 @@ def test_python_side_refuses_cpu_tensors_and_wrong_types():
         tch_cuda.flash_attn_varlen_window(x, x, x, i[:2], i[:2], 1, 1, 0.1, 4)
     with pytest.raises(AiciError, match="no CPU path"):
         tch_cuda.flash_attn_varlen_paged_window(x, kc, vc, i[:2], i[:1], i.view(1, 4), 1, 1, 0.1, 4)
-
-
-def test_workspace_grows_with_the_batch_only_as_far_as_it_must(lib):
-    f = lib.aici_paged_attention_window_workspace_bytes
-    assert f(0, 8, 8, 100, 10, 0) >= 0
-    big = f(64, 32, 8, 1 << 20, 4096, 4)
-    assert 0 < big <= 64 << 20 and f(64, 32, 8, 1 << 20, 4096, 4) == big
 
 
 # ---- the oracle -----------------------------------------------------------------------------------------
