@@ -219,7 +219,7 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     if out is None:
         # one allocation; the token tensors first, each on a 16-byte boundary
         gap = 2 * (max_tokens % 2)
-        buf = torch.empty(3 * max_tokens + gap + 3 * n + 2, dtype=torch.int32, device=query_lens.device)
+        buf = query_lens.new_empty(3 * max_tokens + gap + 3 * n + 2)
         positions, _, slots, seqlens, logits, context, count = buf.split_with_sizes(
             (2 * max_tokens, gap, max_tokens, n + 1, n, n, 1))
         positions = positions.view(torch.int64)

@@ -156,7 +156,7 @@ __device__ __forceinline__ void copy_async16(void *dst_smem, const void *src) {
 // thread keeps its token's cosines and sines for all its heads.
 // kUnits: vectors of a key head that a thread handles (2 only for heads of more than 128 elements).
 template <typename T, typename C, bool kNeox, int kUnits>
-__global__ void __launch_bounds__(kRotThreads) rotary_cache_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache_kernel(const RotaryParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
   const int groups = (p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta;
@@ -381,7 +381,7 @@ static char *launch_rotary(RotaryParams p, bool cache, cudaStream_t stream) {
   } else {
     const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
     p.kv_heads_per_cta = 1;
-    while (p.kv_heads_per_cta < 4 && (int64_t)tiles * p.num_kv_heads >= (int64_t)8 * p.kv_heads_per_cta * sm_count())
+    while (p.kv_heads_per_cta < 8 && (int64_t)tiles * p.num_kv_heads >= (int64_t)8 * p.kv_heads_per_cta * sm_count())
       p.kv_heads_per_cta *= 2;
     const int grid = tiles * ((p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta) + p.q_plan.ctas;
     const size_t smem = 2 * kRotTok * (p.head_size + 8) * sizeof(T);

@@ -358,7 +358,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           id_cur = id_next;
         } else {
           if (lane < 16 && counts)
-            tma_load_5d(dst + bi * 4096 + (lane >> 3) * 2048, &tmap_k, 0, (lane >> 3) * 8, 0, hk, id_cur,
+            tma_load_5d(dst + bi * 4096 + (lane >> 3) * 2048, &tmap_k, 0, lane >> 3, 0, hk, id_cur,
                         &sh->kv_full[stage]);
         }
         __syncwarp();
@@ -1158,10 +1158,13 @@ static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base,
                              int64_t kv_block_stride) {
   const TmapKey key = {base, num_kv_heads, num_blocks, kv_head_stride, kv_block_stride, value ? 2 : 1};
   if (g_tmap_cache.find(key, map)) return nullptr;
-  if (!value) {  // [blk][h][c = 16][tok = 16][e = 8]: box = 8 tokens of all chunks
-    cuuint64_t dims[5] = {8, 16, 16, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
-    cuuint64_t str[4] = {16, 256, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
-    cuuint32_t box[5] = {8, 8, 16, 1, 1};
+  if (!value) {
+    // [blk][h][c = 16][tok = 16][e = 8], a chunk taken as two halves of 8 tokens x 8 elements = 128
+    // contiguous bytes: box = one half of all chunks, 16 rows of 128 bytes for the engine (the same bytes as
+    // 128 rows of 16, which it moves far slower)
+    cuuint64_t dims[5] = {64, 2, 16, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
+    cuuint64_t str[4] = {128, 256, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
+    cuuint32_t box[5] = {64, 1, 16, 1, 1};
     if (char *e = make_tmap_nd(fn, map, base, 5, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return e;
   } else {  // [blk][h][d = 128][tok = 16]: box = one block, rows of 32 bytes
     cuuint64_t dims[4] = {16, 128, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
@@ -1242,13 +1245,16 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
 
 // Windowed variant.  A query tile visits window / 128 + 1 key tiles and the sinks' tiles: by that length
 // and not the sequence's a call takes shape 1 or 2; two tiles of a CTA are two heads of one kv head.
+// Paged tiles cost the copy engine more (values move in rows of 32 bytes), so sharing them between two
+// query tiles pays earlier: 8 chunks of 512 rows, 32/8 heads, window 256: 67 us one-tile, 72 us two-tile;
+// window 1024: 129 and 122 us; packed, window 1024: 111 and 119 us.
 template <bool kPaged, typename T16>
 static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                                    const OutMaps &to, PrefillParams &p, int num_heads, int batch, int max_seqlen_q,
                                    int max_seqlen_k, cudaStream_t stream) {
   p.pair_heads = 0;
-  const int64_t keys = (int64_t)p.window + p.sinks;
-  if (p.group % 2 != 0 || (!kPaged && (keys < max_seqlen_k ? keys : max_seqlen_k) <= AICI_PREFILL_ONE_TILE_MAX_K))
+  const int64_t keys = (int64_t)p.window + p.sinks, most = kPaged ? 640 : AICI_PREFILL_ONE_TILE_MAX_K;
+  if (p.group % 2 != 0 || (keys < max_seqlen_k ? keys : max_seqlen_k) <= most)
     return launch_prefill_shape<kPaged, 1, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
   return launch_prefill_shape<kPaged, 2, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
 }
