@@ -10,6 +10,7 @@
 //   swap_blocks            (:236-243, todo!)  aici::tch::swap_blocks
 //   paged_attention_v1     (:356-391)        aici::tch::paged_attention_v1
 //   paged_attention_v2_C   (:122-137)        aici::tch::paged_attention_v2  (the crate has no pub fn)
+//   rotary_embedding       (:333-354)        aici::tch::rotary_embedding    (both pairings, part of the head)
 //
 // The crate works on tch::Tensor; without libtorch the same information (data pointer, sizes,
 // strides in elements, kind, device) travels in aici::tch::Tensor, which either views memory
@@ -549,6 +550,194 @@ inline void rotary_embedding_reshape_and_cache(const Tensor &positions, Tensor &
                                           (int)cos_sin_cache.size(1), is_neox ? 1 : 0, cos_sin_cache.size(0),
                                           c.block_size, c.num_blocks, query.stride(0), key.stride(0),
                                           value.stride(0), detail::dtype_of(fn, key), stream));
+}
+
+// ---- rotary positions in their general form -------------------------------------------------------
+namespace detail {
+// Heads per token of [num_tokens, heads * head_size] or [num_tokens, heads, head_size].
+inline int head_rows(const char *fn, const Tensor &t, int head_size) {
+  if (t.dim() == 2 && t.size(1) % head_size == 0 && (t.stride(1) == 1 || t.size(1) == 1)) return (int)(t.size(1) / head_size);
+  if (t.dim() == 3 && t.size(2) == head_size && t.stride(2) == 1 && (t.stride(1) == head_size || t.size(1) == 1))
+    return (int)t.size(1);
+  throw Error(std::string(fn) + ": query, key and value must be [num_tokens, heads * head_size] or [num_tokens, heads, "
+                                "head_size] with contiguous rows");
+}
+inline void rotary_args(const char *fn, const Tensor &positions, const Tensor &query, const Tensor &key, int head_size,
+                        const Tensor &cos_sin_cache) {
+  require(fn, head_size > 0, "head_size must be positive");
+  require(fn, positions.kind == Kind::Int64 && positions.is_contiguous() && positions.numel() == query.size(0) &&
+                  query.size(0) == key.size(0),
+          "positions must be contiguous int64 with one entry per token of query and key");
+  require(fn, cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous(), "cos_sin_cache must be contiguous [max_position, rot_dim]");
+  require(fn, query.kind == key.kind, "query and key must have the same dtype");
+}
+}  // namespace detail
+
+// Cosines and sines [max_position, rot_dim] of aici_rotary_cos_sin_cache; scaling is one of AICI_ROPE_*.
+inline Tensor rotary_cos_sin_cache(int64_t max_position, int rot_dim, double base, Kind kind, int device,
+                                   int scaling = AICI_ROPE_NONE, double factor = 1.0, int64_t original_context = 0,
+                                   cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "rotary_cos_sin_cache";
+  Tensor out = Tensor::empty({max_position, rot_dim}, kind, device);
+  detail::DeviceGuard guard(device);
+  check(fn, aici_rotary_cos_sin_cache(out.data, max_position, rot_dim, base, scaling, factor, original_context,
+                                      detail::dtype_of(fn, out), stream));
+  return out;
+}
+
+// rotary_embedding (lib.rs:333-354): query and key turned in place by the table's rows.
+inline void rotary_embedding(const Tensor &positions, Tensor &query, Tensor &key, int head_size,
+                             const Tensor &cos_sin_cache, bool is_neox, cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "rotary_embedding";
+  const int dev = detail::require_cuda(fn, {&positions, &query, &key, &cos_sin_cache});
+  detail::rotary_args(fn, positions, query, key, head_size, cos_sin_cache);
+  const int heads = detail::head_rows(fn, query, head_size), kv_heads = detail::head_rows(fn, key, head_size);
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_rotary_embedding(static_cast<const int64_t *>(positions.data), query.data, key.data, cos_sin_cache.data,
+                                  (int)query.size(0), heads, kv_heads, head_size, (int)cos_sin_cache.size(1),
+                                  is_neox ? 1 : 0, cos_sin_cache.size(0), query.stride(0), key.stride(0),
+                                  detail::dtype_of(fn, cos_sin_cache), detail::dtype_of(fn, query), stream));
+}
+
+// The same in one pass with the cache write of the turned key and the value.
+inline void rotary_embedding_and_cache(const Tensor &positions, Tensor &query, Tensor &key, const Tensor &value,
+                                       int head_size, const Tensor &cos_sin_cache, bool is_neox, Tensor &key_cache,
+                                       Tensor &value_cache, const Tensor &slot_mapping,
+                                       cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "rotary_embedding_and_cache";
+  using detail::require;
+  const int dev = detail::require_cuda(fn, {&positions, &query, &key, &value, &cos_sin_cache, &key_cache, &value_cache,
+                                            &slot_mapping});
+  const detail::CacheDims c = detail::cache_dims(fn, key_cache, value_cache);
+  detail::rotary_args(fn, positions, query, key, head_size, cos_sin_cache);
+  const int heads = detail::head_rows(fn, query, head_size);
+  require(fn, c.head_size == head_size && detail::head_rows(fn, key, head_size) == c.num_kv_heads &&
+                  detail::head_rows(fn, value, head_size) == c.num_kv_heads && value.size(0) == key.size(0),
+          "key and value do not match the cache");
+  require(fn, value.kind == query.kind && key_cache.kind == query.kind && value_cache.kind == query.kind, "dtypes differ");
+  require(fn, (slot_mapping.kind == Kind::Int || slot_mapping.kind == Kind::Int64) && slot_mapping.is_contiguous() &&
+                  slot_mapping.numel() == query.size(0),
+          "slot_mapping must be contiguous int32 or int64 with one entry per token");
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_rotary_embedding_and_cache(
+                static_cast<const int64_t *>(positions.data), query.data, key.data, value.data, cos_sin_cache.data,
+                key_cache.data, value_cache.data, slot_mapping.data, slot_mapping.kind == Kind::Int64 ? 1 : 0,
+                (int)query.size(0), heads, c.num_kv_heads, head_size, (int)cos_sin_cache.size(1), is_neox ? 1 : 0,
+                cos_sin_cache.size(0), c.block_size, c.num_blocks, query.stride(0), key.stride(0), value.stride(0),
+                detail::dtype_of(fn, cos_sin_cache), detail::dtype_of(fn, query), stream));
+}
+
+// ---- attention with a sliding window and sinks ------------------------------------------------------
+// paged_attention_v1 in which a query sees the last `window` tokens of its sequence and the first `sinks`.
+inline void paged_attention_window(Tensor &out, const Tensor &query, const Tensor &key_cache, const Tensor &value_cache,
+                                   int num_kv_heads, float scale, const Tensor &block_tables,
+                                   const Tensor &context_lens, int block_size, int max_context_len, int window,
+                                   int sinks = 0, cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "paged_attention_window";
+  const int dev = detail::require_cuda(fn, {&out, &query, &key_cache, &value_cache, &block_tables, &context_lens});
+  const detail::DecodeDims d = detail::decode_dims(fn, out, query, key_cache, value_cache, num_kv_heads, block_tables,
+                                                   context_lens, block_size);
+  detail::require(fn, value_cache.kind == query.kind, "dtypes differ");
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_paged_attention_window(out.data, query.data, key_cache.data, value_cache.data, num_kv_heads, scale,
+                                        static_cast<const int32_t *>(block_tables.data),
+                                        static_cast<const int32_t *>(context_lens.data), block_size, max_context_len,
+                                        window, sinks, d.num_seqs, d.num_heads, d.c.head_size, d.max_blocks,
+                                        d.c.num_blocks, query.stride(0), key_cache.stride(0), key_cache.stride(1),
+                                        detail::dtype_of(fn, query), stream));
+}
+
+// flash_attn_varlen, causal, with the window; returns a new tensor shaped like q.
+inline Tensor flash_attn_varlen_window(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &seqlens_q,
+                                       const Tensor &seqlens_k, size_t max_seqlen_q, size_t max_seqlen_k,
+                                       float softmax_scale, int window, int sinks = 0,
+                                       cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "flash_attn_varlen_window";
+  using detail::require;
+  const int dev = detail::require_cuda(fn, {&q, &k, &v, &seqlens_q, &seqlens_k});
+  require(fn, q.dim() == 3 && k.dim() == 3 && v.sizes == k.sizes && k.size(2) == q.size(2) && q.stride(2) == 1 &&
+                  k.stride(2) == 1 && v.stride(2) == 1,
+          "q, k, v must be [tokens, heads, head_size] with contiguous last dimension");
+  require(fn, k.kind == q.kind && v.kind == q.kind, "query, key and value must have the same dtype");
+  require(fn, seqlens_q.kind == Kind::Int && seqlens_k.kind == Kind::Int && seqlens_q.is_contiguous() &&
+                  seqlens_k.is_contiguous() && seqlens_q.numel() == seqlens_k.numel() && seqlens_q.numel() > 1,
+          "seqlens_q and seqlens_k must be contiguous int32 [batch + 1]");
+  Tensor out = Tensor::empty(q.sizes, q.kind, dev);
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_mha_varlen_window_fwd(
+                out.data, q.data, k.data, v.data, static_cast<const int32_t *>(seqlens_q.data),
+                static_cast<const int32_t *>(seqlens_k.data), (int)seqlens_q.numel() - 1, (int)q.size(0), (int)k.size(0),
+                (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)max_seqlen_q, (int)max_seqlen_k, window, sinks,
+                q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                out.stride(1), softmax_scale, detail::dtype_of(fn, q), stream));
+  return out;
+}
+
+// flash_attn_varlen_paged, causal, with the window.
+inline Tensor flash_attn_varlen_paged_window(const Tensor &q, const Tensor &key_cache, const Tensor &value_cache,
+                                             const Tensor &seqlens_q, const Tensor &context_lens,
+                                             const Tensor &block_tables, size_t max_seqlen_q, size_t max_context_len,
+                                             float softmax_scale, int window, int sinks = 0,
+                                             cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "flash_attn_varlen_paged_window";
+  using detail::require;
+  const int dev = detail::require_cuda(fn, {&q, &key_cache, &value_cache, &seqlens_q, &context_lens, &block_tables});
+  const detail::CacheDims c = detail::cache_dims(fn, key_cache, value_cache);
+  require(fn, q.dim() == 3 && q.size(2) == c.head_size && q.stride(2) == 1,
+          "q must be [total_q, num_heads, head_size] with contiguous last dimension");
+  require(fn, key_cache.kind == q.kind && value_cache.kind == q.kind, "query and cache dtypes differ");
+  require(fn, seqlens_q.kind == Kind::Int && context_lens.kind == Kind::Int && block_tables.kind == Kind::Int &&
+                  seqlens_q.is_contiguous() && context_lens.is_contiguous() && block_tables.is_contiguous(),
+          "seqlens_q, context_lens and block_tables must be contiguous int32");
+  const int batch = (int)seqlens_q.numel() - 1;
+  require(fn, batch > 0 && context_lens.numel() == batch && block_tables.dim() == 2 && block_tables.size(0) == batch,
+          "context_lens must be [batch] and block_tables [batch, max_blocks]");
+  Tensor out = Tensor::empty(q.sizes, q.kind, dev);
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_mha_varlen_paged_window_fwd(
+                out.data, q.data, key_cache.data, value_cache.data, static_cast<const int32_t *>(seqlens_q.data),
+                static_cast<const int32_t *>(context_lens.data), static_cast<const int32_t *>(block_tables.data), batch,
+                (int)q.size(0), (int)q.size(1), c.num_kv_heads, c.head_size, c.block_size, (int)max_seqlen_q,
+                (int)max_context_len, (int)block_tables.size(1), c.num_blocks, window, sinks, q.stride(0), q.stride(1),
+                out.stride(0), out.stride(1), key_cache.stride(0), key_cache.stride(1), softmax_scale,
+                detail::dtype_of(fn, q), stream));
+  return out;
+}
+
+// ---- a step's index tensors on the GPU (aici_step_tables) ---------------------------------------------
+struct StepTables {
+  Tensor seqlens_q, positions, slot_mapping, logit_idxs, context_lens, free_count;
+};
+
+// block_tables is extended in place; the returned tensors are new.
+inline StepTables step_tables(const Tensor &query_lens, const Tensor &context_lens, Tensor &block_tables,
+                              const Tensor &free_blocks, const Tensor &free_count, int64_t num_blocks, int max_tokens,
+                              int block_size = 16, cudaStream_t stream = cudaStreamPerThread) {
+  const char *fn = "step_tables";
+  using detail::require;
+  const int dev = detail::require_cuda(fn, {&query_lens, &context_lens, &block_tables, &free_blocks, &free_count});
+  for (const Tensor *t : std::initializer_list<const Tensor *>{&query_lens, &context_lens, &block_tables, &free_blocks,
+                                                               &free_count})
+    require(fn, t->kind == Kind::Int && t->is_contiguous(), "lengths, tables and free list must be contiguous int32");
+  const int n = (int)query_lens.numel();
+  require(fn, context_lens.numel() == n && block_tables.dim() == 2 && block_tables.size(0) == n && free_count.numel() == 1,
+          "query_lens and context_lens must be [requests], block_tables [requests, max_blocks], free_count [1]");
+  StepTables r;
+  r.seqlens_q = Tensor::empty({n + 1}, Kind::Int, dev);
+  r.positions = Tensor::empty({max_tokens}, Kind::Int64, dev);
+  r.slot_mapping = Tensor::empty({max_tokens}, Kind::Int, dev);
+  r.logit_idxs = Tensor::empty({n}, Kind::Int, dev);
+  r.context_lens = Tensor::empty({n}, Kind::Int, dev);
+  r.free_count = Tensor::empty({1}, Kind::Int, dev);
+  detail::DeviceGuard guard(dev);
+  check(fn, aici_step_tables(static_cast<const int32_t *>(query_lens.data), static_cast<const int32_t *>(context_lens.data),
+                             static_cast<int32_t *>(block_tables.data), static_cast<const int32_t *>(free_blocks.data),
+                             static_cast<const int32_t *>(free_count.data), n, (int)block_tables.size(1),
+                             block_tables.size(1), (int)free_blocks.numel(), num_blocks, block_size, max_tokens,
+                             static_cast<int32_t *>(r.seqlens_q.data), static_cast<int64_t *>(r.positions.data),
+                             static_cast<int32_t *>(r.slot_mapping.data), static_cast<int32_t *>(r.logit_idxs.data),
+                             static_cast<int32_t *>(r.context_lens.data), static_cast<int32_t *>(r.free_count.data), stream));
+  return r;
 }
 
 // Reads and clears the device's sticky status word (no counterpart in the crate; the reference
