@@ -354,8 +354,8 @@ static char *check_rotary(const char *fn, const RotaryParams &p, int table_dtype
                "%s: token strides must be multiples of 8 elements and cover one row", fn);
     AICI_CHECK(p.num_slots > 0, "%s: num_blocks must be positive", fn);
   }
-  const int64_t tiles = (p.num_tokens + 15) / 16;
-  AICI_CHECK(tiles * p.num_kv_heads + p.num_tokens < (1ll << 31), "%s: too many tokens and heads for one call", fn);
+  AICI_CHECK(p.num_tokens < (1 << 29) && (int64_t)(p.num_tokens / 16 + 1) * p.num_kv_heads < (1 << 30),
+             "%s: too many tokens and heads for one call", fn);
   return nullptr;
 }
 

@@ -1086,7 +1086,8 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Generic tiled map over bf16 data: dims/box innermost first, strides (bytes) for dims 1..rank-1.
+// Generic tiled map over 16-bit data (declared bf16; f16 tensors use the same maps, since the engine moves
+// the elements as they are and fills with zero): dims/box innermost first, strides (bytes) for dims 1..rank-1.
 static char *make_tmap_nd(const char *fn, CUtensorMap *map, const void *base, int rank,
                           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
                           CUtensorMapSwizzle swizzle) {

@@ -314,6 +314,34 @@ def test_prefill_with_a_covering_window_is_causal_attention(cuda_device):
     assert float((a - b).abs().max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
 
 
+@pytest.mark.parametrize("is_paged", [False, True])
+@pytest.mark.parametrize("window,sinks,offset", [(100, 0, 0), (128, 4, 37), (300, 20, 128)])
+def test_prefill_tiles_that_do_not_see_a_token_do_not_meet_it(cuda_device, window, sinks, offset, is_paged):
+    """NaN in one token: query tiles of 128 rows none of which sees it stay right."""
+    dev, dtype, n, H = cuda_device, torch.bfloat16, 520, 2
+    for bad in (0, 3, 19, 21, 130, 255, 256, 300, 511):
+        g = torch.Generator().manual_seed(bad)
+        lens_k = [n + offset]
+        kc, vc, table, ks, vs = paged(g, lens_k, 1, dtype)
+        q, k, v = normal(g, dtype, n, H, D), ks[0].clone(), vs[0].clone()
+        k[bad], v[bad] = NAN, NAN
+        kc[table[0, bad // 16], :, :, bad % 16] = NAN
+        vc[table[0, bad // 16], :, :, bad % 16] = NAN
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        if is_paged:
+            out = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc.to(dev), vc.to(dev), i32([0, n]), i32(lens_k),
+                                                          table.to(dev), n, n + offset, SCALE, window, sinks).cpu()
+        else:
+            out = tch_cuda.flash_attn_varlen_window(q.to(dev), k.to(dev), v.to(dev), i32([0, n]), i32([0, n + offset]), n,
+                                                    n + offset, SCALE, window, sinks).cpu()
+        for r0 in range(0, n, 128):
+            rows = range(r0, min(r0 + 128, n))
+            if not any(bad in W.visible(offset + r, window, sinks) for r in (rows[0], rows[-1], max(rows[0], min(rows[-1], bad - offset)))):
+                some = [rows[0], rows[len(rows) // 2], rows[-1]]
+                near(out[some], q[some], ks[0], vs[0], [offset + r for r in some], window, sinks, dtype)
+    assert _lib.last_status() == 0
+
+
 def test_prefill_of_single_tokens_is_decode(cuda_device):
     dev, dtype = cuda_device, torch.float16
     g = torch.Generator().manual_seed(14)
