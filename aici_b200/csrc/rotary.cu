@@ -151,11 +151,12 @@ __device__ __forceinline__ void copy_async16(void *dst_smem, const void *src) {
 // With the cache write.  The first CTAs take 16 tokens and some kv heads each, one head after the other:
 // the key is turned, put back and written to the cache, the value goes through shared memory because the
 // cache keeps it transposed ([d][token]).  The CTAs behind them turn the query heads.  Where a token goes
-// and how far it turns does not change what is read: the first head's keys and values are on their way
-// before slots and positions have arrived, and each head's while the one before it is worked on.  A
-// thread keeps its token's cosines and sines for all its heads.
+// and how far it turns does not change what is read, so a ring of kStages heads is filled by asynchronous
+// copies from the start: what bounds this part is bytes in flight (4 KB of keys and of values per head, 96
+// KB an SM with three heads ahead and four CTAs; with one head ahead it ran a third slower).  A thread
+// keeps its token's cosines and sines for all its heads.
 // kUnits: vectors of a key head that a thread handles (2 only for heads of more than 128 elements).
-template <typename T, typename C, bool kNeox, int kUnits>
+template <typename T, typename C, bool kNeox, int kUnits, int kStages>
 __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache_kernel(const RotaryParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
@@ -169,42 +170,26 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache
   const int t0 = blockIdx.x / groups * kRotTok;
   const int tid = threadIdx.x, D = p.head_size, pitch = D + 8;
   const int tokens = min(kRotTok, p.num_tokens - t0);
-  auto buffer = [&](int h) { return reinterpret_cast<T *>(smem) + ((h - h_begin) & 1) * (kRotTok * pitch); };  // [16][D + 8]
-  auto fetch_value = [&](int h) {
-    T *dst = buffer(h);
-    for (int i = tid; i < tokens * (D / 8); i += kRotThreads) {
-      const int tok = i / (D / 8), c = i - tok * (D / 8);
-      copy_async16(dst + tok * pitch + c * 8,
-                   static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + (int64_t)h * D + c * 8);
+  // stage of head h: keys [16][D + 8], then values
+  auto stage = [&](int h) { return reinterpret_cast<T *>(smem) + (h - h_begin) % kStages * (2 * kRotTok * pitch); };
+  auto fetch = [&](int h) {
+    if (h < h_end) {
+      T *dst = stage(h);
+      for (int i = tid; i < tokens * (D / 8); i += kRotThreads) {
+        const int tok = i / (D / 8), c = i - tok * (D / 8);
+        const int64_t from = (int64_t)h * D + c * 8;
+        copy_async16(dst + tok * pitch + c * 8, static_cast<const T *>(p.key) + (t0 + tok) * p.key_stride + from);
+        copy_async16(dst + (kRotTok + tok) * pitch + c * 8, static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + from);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // keys: 16 consecutive threads take the 16 tokens of one unit, so that the cache sees runs of 256
-  // bytes.  Units are the chunks, then the vectors behind rot_dim.
-  const int nc = p.rot_dim / 16, units = nc + (D - p.rot_dim) / 8;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) fetch(h_begin + s);
+
   const int tok = tid & (kRotTok - 1);
-  const bool mine = tok < tokens;
-  T *key = static_cast<T *>(p.key) + (t0 + tok) * p.key_stride;
-  int unit[kUnits], e0[kUnits], e1[kUnits];
-#pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    unit[i] = tid / kRotTok + i * (kRotThreads / kRotTok);
-    e0[i] = unit[i] < nc ? unit[i] * 8 : p.rot_dim + (unit[i] - nc) * 8;
-    e1[i] = e0[i] + p.rot_dim / 2;
-  }
-  uint4 xv[kUnits], yv[kUnits];
-  auto fetch_key = [&](int h) {
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i)
-      if (mine && unit[i] < units) {
-        xv[i] = *reinterpret_cast<const uint4 *>(key + (int64_t)h * D + e0[i]);
-        if (unit[i] < nc) yv[i] = *reinterpret_cast<const uint4 *>(key + (int64_t)h * D + e1[i]);
-      }
-  };
-  fetch_value(h_begin);
-  fetch_key(h_begin);
   int64_t slot = -1, pos = -1;
-  if (mine) {
+  if (tok < tokens) {
     slot = p.slot_is_int64 ? static_cast<const int64_t *>(p.slots)[t0 + tok]
                            : (int64_t) static_cast<const int32_t *>(p.slots)[t0 + tok];
     pos = p.positions[t0 + tok];
@@ -216,45 +201,48 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache
     }
   }
   if (tid < kRotTok) s_slot[tid] = slot;
+  // keys: 16 consecutive threads take the 16 tokens of one unit, so that the cache sees runs of 256
+  // bytes.  Units are the chunks, then the vectors behind rot_dim.
+  const int nc = p.rot_dim / 16, units = nc + (D - p.rot_dim) / 8;
   float co[kUnits][8], si[kUnits][8];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i)
-    if (pos >= 0 && unit[i] < nc)
-      load_turn<C, kNeox>(static_cast<const C *>(p.table) + pos * p.rot_dim, p.rot_dim, unit[i], co[i], si[i]);
+  for (int i = 0; i < kUnits; ++i) {
+    const int u = tid / kRotTok + i * (kRotThreads / kRotTok);
+    if (pos >= 0 && u < nc)
+      load_turn<C, kNeox>(static_cast<const C *>(p.table) + pos * p.rot_dim, p.rot_dim, u, co[i], si[i]);
+  }
+  T *key = static_cast<T *>(p.key) + (t0 + tok) * p.key_stride;
   T *kc = static_cast<T *>(p.key_cache) +
           (slot >= 0 ? slot / kRotBlock * p.num_kv_heads * D * kRotBlock + slot % kRotBlock * 8 : 0);
   T *vc = static_cast<T *>(p.value_cache);
   uint32_t runs = 0;
 
   for (int h = h_begin; h < h_end; ++h) {
-    uint4 x[kUnits], y[kUnits];
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      x[i] = xv[i];
-      y[i] = yv[i];
-    }
-    if (h + 1 < h_end) {
-      fetch_value(h + 1);
-      fetch_key(h + 1);
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();  // everybody's copies of this head have landed, and the stage refilled next is read
+    fetch(h + kStages - 1);
+    const T *s_k = stage(h), *s_v = s_k + kRotTok * pitch;
     if (pos >= 0) {
       T *to = kc + (int64_t)h * D * kRotBlock;  // vector e / 8 of the head: 16 tokens x 8 elements
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        if (unit[i] < nc) {
-          turn<T, kNeox>(x[i], y[i], co[i], si[i]);
-          *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e0[i]) = x[i];
-          *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e1[i]) = y[i];
-        }
-        if (slot >= 0 && unit[i] < units) {
-          *reinterpret_cast<uint4 *>(to + e0[i] * kRotBlock) = x[i];
-          if (unit[i] < nc) *reinterpret_cast<uint4 *>(to + e1[i] * kRotBlock) = y[i];
+        const int u = tid / kRotTok + i * (kRotThreads / kRotTok);
+        if (u < units) {
+          const int e0 = u < nc ? u * 8 : p.rot_dim + (u - nc) * 8, e1 = e0 + p.rot_dim / 2;
+          uint4 x = *reinterpret_cast<const uint4 *>(s_k + tok * pitch + e0), y = make_uint4(0, 0, 0, 0);
+          if (u < nc) {
+            y = *reinterpret_cast<const uint4 *>(s_k + tok * pitch + e1);
+            turn<T, kNeox>(x, y, co[i], si[i]);
+            *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e0) = x;
+            *reinterpret_cast<uint4 *>(key + (int64_t)h * D + e1) = y;
+          }
+          if (slot >= 0) {
+            *reinterpret_cast<uint4 *>(to + e0 * kRotBlock) = x;
+            if (u < nc) *reinterpret_cast<uint4 *>(to + e1 * kRotBlock) = y;
+          }
         }
       }
     }
-    if (h + 1 < h_end) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
     // values: 8 tokens whose slots are consecutive and start at a multiple of 8 leave as one vector, any
     // others element by element with consecutive threads on consecutive tokens
     if (h == h_begin) {
@@ -267,7 +255,6 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache
         runs |= (run ? 1u : 0u) << g;
       }
     }
-    const T *s_v = buffer(h);
     auto value_at = [&](int64_t s) { return vc + (s / kRotBlock * p.num_kv_heads + h) * D * kRotBlock + s % kRotBlock; };
     if (runs != 0u)
       for (int i = tid; i < 2 * D; i += kRotThreads) {  // both halves of a block's row side by side
@@ -284,7 +271,6 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache
       T *dst = value_at(slot);
       for (int d = tid / kRotTok; d < D; d += kRotThreads / kRotTok) dst[d * kRotBlock] = s_v[tok * pitch + d];
     }
-    if (h + 2 < h_end) __syncthreads();  // the next round's fetch goes into this buffer
   }
 }
 
@@ -372,6 +358,15 @@ static HeadPlan plan_heads(int tokens, int heads, int rot_dim) {
   return plan;
 }
 
+template <typename T, typename C, bool kNeox, int kUnits, int kStages>
+static char *launch_rotary_cache(const RotaryParams &p, int grid, cudaStream_t stream) {
+  // two tiles of 16 rows a stage; heads of up to 128 elements take four stages, larger ones two
+  const size_t smem = (size_t)kStages * 2 * kRotTok * (p.head_size + 8) * sizeof(T);
+  rotary_cache_kernel<T, C, kNeox, kUnits, kStages><<<grid, kRotThreads, smem, stream>>>(p);
+  AICI_CUDA(cudaGetLastError());
+  return nullptr;
+}
+
 template <typename T, typename C, bool kNeox>
 static char *launch_rotary(RotaryParams p, bool cache, cudaStream_t stream) {
   p.q_plan = plan_heads(p.num_tokens, p.num_heads, p.rot_dim);
@@ -384,11 +379,10 @@ static char *launch_rotary(RotaryParams p, bool cache, cudaStream_t stream) {
     while (p.kv_heads_per_cta < 8 && (int64_t)tiles * p.num_kv_heads >= (int64_t)8 * p.kv_heads_per_cta * sm_count())
       p.kv_heads_per_cta *= 2;
     const int grid = tiles * ((p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta) + p.q_plan.ctas;
-    const size_t smem = 2 * kRotTok * (p.head_size + 8) * sizeof(T);
-    if (p.rot_dim / 16 + (p.head_size - p.rot_dim) / 8 <= kRotThreads / kRotTok)
-      rotary_cache_kernel<T, C, kNeox, 1><<<grid, kRotThreads, smem, stream>>>(p);
-    else
-      rotary_cache_kernel<T, C, kNeox, 2><<<grid, kRotThreads, smem, stream>>>(p);
+    const bool one = p.rot_dim / 16 + (p.head_size - p.rot_dim) / 8 <= kRotThreads / kRotTok;
+    if (one && p.head_size <= 128) return launch_rotary_cache<T, C, kNeox, 1, 4>(p, grid, stream);
+    if (one) return launch_rotary_cache<T, C, kNeox, 1, 2>(p, grid, stream);
+    return launch_rotary_cache<T, C, kNeox, 2, 2>(p, grid, stream);
   }
   AICI_CUDA(cudaGetLastError());
   return nullptr;
