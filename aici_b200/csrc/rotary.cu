@@ -152,12 +152,15 @@ __device__ __forceinline__ void copy_async16(void *dst_smem, const void *src) {
 // the key is turned, put back and written to the cache, the value goes through shared memory because the
 // cache keeps it transposed ([d][token]).  The CTAs behind them turn the query heads.  Where a token goes
 // and how far it turns does not change what is read, so a ring of kStages heads is filled by asynchronous
-// copies from the start: what bounds this part is bytes in flight (4 KB of keys and of values per head, 96
-// KB an SM with three heads ahead and four CTAs; with one head ahead it ran a third slower).  A thread
-// keeps its token's cosines and sines for all its heads.
+// copies from the start: what bounds this part is bytes in flight (4 KB of keys and of values per head, 72
+// KB an SM with three heads ahead and three CTAs; with one head ahead the whole call took 85 us where it
+// takes 77, 16384 tokens, 64/8 heads, half of each head rotated).  A thread keeps its token's cosines and
+// sines for all its heads.  (A prompt that starts inside a block leaves value by value, 45 against 50 us
+// at 8/8 heads; vectors for the half blocks inside a tile, or for those that reach into the next tile with
+// the tokens they need fetched twice, were no faster.)
 // kUnits: vectors of a key head that a thread handles (2 only for heads of more than 128 elements).
 template <typename T, typename C, bool kNeox, int kUnits, int kStages>
-__global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 4 : 2) rotary_cache_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 3 : 2) rotary_cache_kernel(const RotaryParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
   const int groups = (p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta;
