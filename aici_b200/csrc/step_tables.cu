@@ -9,16 +9,17 @@
 // p % 16 == 0 begins a new one, and the k-th new block of the step, counted in token order, is
 // free_blocks[free_count - 1 - k].  slot = block * 16 + p % 16.
 //
-// The work is a handful of dependent reads and writes of at most a megabyte: latency bounds it.  One
-// cluster does it in one launch.  Every CTA reads all the lengths and computes both running sums (new
-// tokens, new blocks) for itself in shared memory -- n values, which beats a hand-over between CTAs --
-// then the CTAs share out the tokens.  The cluster barrier between "all lengths are read" and "the new
-// lengths are written" is what lets the outputs be the inputs' own buffers.
+// The work is a handful of dependent reads and writes of at most a megabyte: latency bounds it, and the
+// instructions of the longest thread.  Every CTA reads all the lengths and computes both running sums
+// (new tokens, new blocks) for itself in shared memory -- n values, which beats a hand-over between CTAs --
+// then the CTAs share out the tokens.  Where an output is an input's own buffer (state that advances in
+// place) nothing may be written before every CTA has read the lengths: then the grid is one cluster of up
+// to 8 CTAs with its barrier between the two; otherwise it has as many CTAs as have tokens to work on.
 #include "common.cuh"
 
 namespace aici {
 
-constexpr int kStepThreads = 1024;  // of a CTA at most; a quarter for small steps
+constexpr int kStepThreads = 512;   // of a CTA at most; half of them for small steps
 constexpr int kStepWarps = kStepThreads / 32;
 constexpr int kStepBatch = 4;       // lengths a thread loads at once, tokens it works on together
 constexpr int kBlockTokens = 16;
@@ -49,9 +50,7 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
   __shared__ unsigned int s_warp_tok[kStepWarps], s_warp_new[kStepWarps];
   __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
-  unsigned int rank, ctas;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  const unsigned int rank = blockIdx.x, ctas = gridDim.x;
   if (tid == 0) s_bad = 0;
   __syncthreads();
 
@@ -136,7 +135,7 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
     if (refused && rank == 0) set_status(p.status, s_bad || !no_blocks ? AICI_STATUS_BAD_BLOCK : AICI_STATUS_NO_BLOCKS);
   }
   __syncthreads();
-  // every CTA has read the lengths and the count once all have arrived here
+  // in place (the grid is a cluster): every CTA has read the lengths and the count once all have arrived here
   asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 
   // ---- tokens: four consecutive ones to a thread -----------------------------------------------------
@@ -282,14 +281,23 @@ extern "C" char *aici_step_tables(const int32_t *query_lens, const int32_t *cont
   StepParams p = {query_lens, context_lens, block_tables, free_blocks, free_count, seqlens_q, slot_mapping,
                   logit_idxs, context_lens_out, free_count_out, positions, num_requests, max_blocks_per_seq,
                   max_tokens, free_capacity, num_blocks, block_table_stride, st};
-  // one small CTA, or up to eight large ones: a thread has one batch of tokens where that is possible
+  auto meets = [](const void *a, int64_t na, const void *b, int64_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + 4 * nb && (uintptr_t)b < (uintptr_t)a + 4 * na;
+  };
+  bool in_place = false;
+  const int32_t *outs[4] = {seqlens_q, logit_idxs, context_lens_out, free_count_out};
+  const int64_t lens[4] = {num_requests + 1, num_requests, num_requests, 1};
+  for (int i = 0; i < 4; ++i)
+    in_place = in_place || meets(outs[i], lens[i], query_lens, num_requests) ||
+               meets(outs[i], lens[i], context_lens, num_requests) || meets(outs[i], lens[i], free_count, 1);
   const int64_t work = (int64_t)max_tokens + num_requests;
-  const int threads = work <= kStepThreads ? kStepThreads / 4 : kStepThreads;
+  const int threads = work <= 2 * kStepThreads ? kStepThreads / 2 : kStepThreads;
+  const int64_t most = in_place ? 8 : sm_count();
   int ctas = 1;
-  while (ctas < 8 && work > (int64_t)kStepBatch * threads * ctas) ctas *= 2;
+  while (2 * ctas <= most && work > (int64_t)kStepBatch * threads * ctas) ctas *= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.x = in_place ? ctas : 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};

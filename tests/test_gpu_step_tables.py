@@ -85,6 +85,23 @@ def test_in_place_over_several_steps_and_strided_table(cuda_device):
     assert (wide[:, 33:] == -7).all() and _lib.last_status() == 0
 
 
+@pytest.mark.parametrize("which", ["context", "count", "both"])
+def test_in_place_with_many_tokens(cuda_device, which):
+    """Large enough for several CTAs, which must all read the state before one of them writes it."""
+    dev = cuda_device
+    d = lambda x: torch.tensor(x, dtype=I32, device=dev)  # noqa: E731
+    news, ctx, tables, free, count, T, num_blocks = make(31, 700, 160, 400)
+    want = W.step_tables(news, ctx, tables, free, count, T, num_blocks)
+    for _ in range(20):
+        e = lambda k, t=I32: torch.empty(k, dtype=t, device=dev)  # noqa: E731
+        ctx_d, count_d, bt = d(ctx), d([count]), d(tables)
+        out = batch_info.StepTables(e(701), e(T, torch.int64), e(T), e(700), ctx_d if which != "count" else e(700),
+                                    count_d if which != "context" else e(1))
+        batch_info.step_tables(d(news), ctx_d, bt, d(free), count_d, num_blocks, T, out=out)
+        check(out, bt, want)
+    assert _lib.last_status() == 0
+
+
 @pytest.mark.parametrize("change,status", [
     (lambda a: a[0].__setitem__(2, -1), 1), (lambda a: a[1].__setitem__(0, -5), 1), (lambda a: a[1].__setitem__(1, 1 << 30), 1),
     (lambda a: a[0].__setitem__(1, (1 << 31) - 1), 1), (lambda a: a.__setitem__(5, a[5] - 1), 1),
