@@ -98,9 +98,23 @@ struct PrefillParams {
   int window, sinks;
 };
 
-// One tensor map per output buffer (this GPU's and, for the fused gather, every peer's).
+// One tensor map per output buffer (this GPU's and, for the fused gather, every peer's); the windowed
+// variant has one output (1 KB less of kernel arguments for the host to hand over).
 struct OutMaps {
   CUtensorMap m[8];
+};
+struct OutMap {
+  CUtensorMap m[1];
+};
+template <bool kWindow>
+struct OutMapsOf {
+  using type = OutMaps;
+  static const OutMaps &of(const OutMaps &m) { return m; }
+};
+template <>
+struct OutMapsOf<true> {
+  using type = OutMap;
+  static OutMap of(const OutMaps &m) { return {{m.m[0]}}; }
 };
 
 struct PrefillSmem {
@@ -169,7 +183,7 @@ __global__ void __launch_bounds__(PrefillCfg<kShape>::kThreads, PrefillCfg<kShap
 varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ CUtensorMap tmap_k,
                       const __grid_constant__ CUtensorMap tmap_v,
-                      const __grid_constant__ OutMaps tmap_o, const PrefillParams p) {
+                      const __grid_constant__ typename OutMapsOf<kWindow>::type tmap_o, const PrefillParams p) {
   using Cfg = PrefillCfg<kShape>;
   constexpr int kTiles = Cfg::kTiles;
   constexpr bool kPair = Cfg::kPair;
@@ -1223,7 +1237,8 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cudaError_t le = cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<kPaged, kShape, kWindow, T16>, tq, tk, tv, to, p);
+  cudaError_t le = cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<kPaged, kShape, kWindow, T16>, tq, tk, tv,
+                                      OutMapsOf<kWindow>::of(to), p);
   if (le != cudaSuccess) {
     cudaGetLastError();
     int clusters = -1, max_size = -1;

@@ -891,7 +891,7 @@ def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         raise AiciError("%s: query, key and value must have the same dtype" % fn)
     if seqlens_k.dtype is not torch.int32 or not seqlens_k.is_contiguous() or seqlens_k.numel() != batch + 1:
         raise AiciError("%s: seqlens_k must be contiguous int32 and as long as seqlens_q" % fn)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_window_fwd", index, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
           seqlens_q.data_ptr(), seqlens_k.data_ptr(), batch, total_q, k.shape[0], num_heads, k.shape[1], head_size,
@@ -916,7 +916,7 @@ def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, val
     if q.dtype is not key_cache.dtype or q.dtype is not value_cache.dtype:
         raise AiciError("%s: query and cache dtypes differ" % fn)
     _check_table(fn, block_tables, context_lens, batch)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_paged_window_fwd", index, out.data_ptr(), q.data_ptr(), key_cache.data_ptr(),
           value_cache.data_ptr(), seqlens_q.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), batch,
