@@ -144,7 +144,11 @@ struct GroupState {
       vm_lo = (vis[0] ? 0xffffu : 0u) | (vis[1] ? 0xffff0000u : 0u);
       vm_hi = (vis[2] ? 0xffffu : 0u) | (vis[3] ? 0xffff0000u : 0u);
     }
-    uint32_t pa[2][2];
+    // A probability goes in as two 16-bit numbers, the rounded value and what the rounding left: the values'
+    // product is then as exact as fp32 sums make it, and the output carries one rounding, its own.  (With
+    // the rounded value alone the error is half as large again; the second product costs nothing beside
+    // the tile's copy.)
+    uint32_t pa[2][2], pb[2][2];
     float alpha[kRows];
     bool moved = false;
 #pragma unroll
@@ -163,6 +167,9 @@ struct GroupState {
       l[r] = l[r] * alpha[r] + (p0 + p1) + (p2 + p3);
       pa[r][0] = Half16<T>::pack(p0, p1);
       pa[r][1] = Half16<T>::pack(p2, p3);
+      const float2 h01 = Half16<T>::unpack(pa[r][0]), h23 = Half16<T>::unpack(pa[r][1]);
+      pb[r][0] = Half16<T>::pack(p0 - h01.x, p1 - h01.y);
+      pb[r][1] = Half16<T>::pack(p2 - h23.x, p3 - h23.y);
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -185,6 +192,8 @@ struct GroupState {
       }
       mma_half<T>(o[2 * np], pa[0][0], kTwo ? pa[1][0] : 0u, pa[0][1], kTwo ? pa[1][1] : 0u, v00, v01);
       mma_half<T>(o[2 * np + 1], pa[0][0], kTwo ? pa[1][0] : 0u, pa[0][1], kTwo ? pa[1][1] : 0u, v10, v11);
+      mma_half<T>(o[2 * np], pb[0][0], kTwo ? pb[1][0] : 0u, pb[0][1], kTwo ? pb[1][1] : 0u, v00, v01);
+      mma_half<T>(o[2 * np + 1], pb[0][0], kTwo ? pb[1][0] : 0u, pb[0][1], kTwo ? pb[1][1] : 0u, v10, v11);
     }
   }
 

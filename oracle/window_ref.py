@@ -106,11 +106,12 @@ def attention_row(q, k, v, position, window, sinks, scale):
             len(t), size)
 
 
-def attention_bound(o, a, n, size, vmax, dtype):
+def attention_bound(o, a, n, size, vmax, dtype, split=False):
     """How far a kernel's output may be from `o`: half a step of the 16-bit type for the output and one for
     each probability, the fp32 sums over n tokens, the fp32 scores of 128 products each (which reach both
-    the probabilities and their sum), exp2 in fp32, and for f16 probabilities below its normal range."""
+    the probabilities and their sum), exp2 in fp32, and for f16 probabilities below its normal range.  With
+    `split` a probability is its rounded value plus what the rounding left, rounded: half a step squared."""
     half = torch.finfo(dtype).eps / 2
     small = n * 2.0 ** -23 + 2 * (128 * 2.0 ** -24 * size * 1.4427 + 2.0 ** -21)
     under = n * 2.0 ** -25 * vmax if dtype == torch.float16 else 0.0
-    return (half * (o.abs() + a) + small * a) * 1.01 + under + 1e-30
+    return (half * o.abs() + (half * half if split else half) * a + small * a) * 1.01 + under + 1e-30

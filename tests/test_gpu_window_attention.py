@@ -52,12 +52,12 @@ def hide_unseen(kc, vc, table, i, n, seen):
             table[i, b] = -1
 
 
-def near(got, q, k, v, positions, window, sinks, dtype, scale=SCALE):
+def near(got, q, k, v, positions, window, sinks, dtype, scale=SCALE, split=False):
     worst = 0.0
     for r, p in enumerate(positions):
         o, a, n, size = W.attention_row(q[r], k, v, p, window, sinks, scale)
         vmax = float(v[W.visible(p, window, sinks)].abs().max()) if n else 0.0
-        bound = W.attention_bound(o, a, n, size, vmax, dtype)
+        bound = W.attention_bound(o, a, n, size, vmax, dtype, split)
         d = (got[r].double() - o).abs()
         assert torch.isfinite(got[r]).all(), (r, p)
         worst = max(worst, float((d / bound).max()))
@@ -89,7 +89,7 @@ def test_decode(cuda_device, ctx, H, Hk, window, sinks, dtype):
     q = normal(g, dtype, len(ctx), H, D)
     got = decode(cuda_device, q, kc, vc, table, ctx, window, sinks)
     for i, n in enumerate(ctx):
-        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], window, sinks, dtype)
+        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], window, sinks, dtype, split=True)
     assert _lib.last_status() == 0
 
 
@@ -118,7 +118,7 @@ def test_decode_uneven_scores(cuda_device, dtype):
         W.write_cache(ks[i][t:t + 1], vs[i][t:t + 1], kc, vc, table[i, t // 16:t // 16 + 1].long() * 16 + t % 16)
     got = decode(cuda_device, q, kc, vc, table, ctx, 100, 4)
     for i in range(4):
-        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [399], 100, 4, dtype)
+        near(got[i:i + 1], q[i:i + 1], ks[i], vs[i], [399], 100, 4, dtype, split=True)
 
 
 def test_decode_strided_queries_and_infinite_masked_tokens(cuda_device):
