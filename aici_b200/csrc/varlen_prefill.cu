@@ -40,6 +40,7 @@
 // Every barrier wait is bounded; a timeout sets AICI_STATUS_WAIT_TIMEOUT and unwinds.
 #include "half_types.cuh"
 #include "tcgen05.cuh"
+#include "window_chunk.cuh"
 
 namespace aici {
 
@@ -1527,6 +1528,14 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   if (char *e = check_on_current_device(fn, "q", q)) return e;
   unsigned int *st = status_ptr();
   AICI_CHECK(st != nullptr, "%s: no CUDA device", fn);
+
+  if (win != nullptr && window_chunk_takes(batch, num_heads, num_kv_heads, max_seqlen_q)) {
+    const WindowChunk c = {out, q, key_cache, value_cache, cu_seqlens_q, context_lens, block_tables, batch, total_q, num_heads,
+                           num_kv_heads, max_seqlen_q, max_context_len, max_num_blocks_per_seq, win->window, win->sinks,
+                           num_blocks, q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
+                           softmax_scale, st};
+    return launch_window_chunk(c, dtype, static_cast<cudaStream_t>(stream));
+  }
 
   CUtensorMap tq, tk, tv;
   if (char *e = make_tmap(fn, &tq, q, total_q, num_heads, q_tok_stride, q_head_stride)) return e;

@@ -1,7 +1,10 @@
-// Decode attention with a sliding window and sinks over the paged cache (one query token per sequence).
+// Attention of few query rows with a sliding window and sinks over the paged cache: decode (one query
+// token per sequence), and short chunks (fast-forwarded tokens, drafts to be verified), whose tokens and
+// heads are dealt out to work items of 16 rows; the general prefill kernel takes 128 rows of one head to a
+// tile and walks the keys with one CTA.
 //
-// The query of a sequence stands at position ctx - 1 and sees the tokens t < ctx with t >= ctx - window
-// or t < sinks.  Only cache blocks with a visible token are touched: of the block list of a row
+// A query at position d sees the tokens t <= d with t > d - window or t < sinks; the last token of a
+// sequence stands at ctx - 1.  Only cache blocks with a visible token are touched: of the block list of a row
 // (sequence, kv head) those are the first ones (sinks) and the last ones (window), and "tile i of a
 // row" below counts through them:  block(i) = i < n_sink ? i : first + i - n_sink.
 //     o = sum_t 2^(c q.k_t - m) v_t / sum_t 2^(c q.k_t - m),   c = scale log2 e,  m = max_t c q.k_t
@@ -24,6 +27,7 @@
 // than the rest: a CTA alone streams a tile in 0.19 us, so the last row to start costs at most that
 // times its tiles.
 #include "half_types.cuh"
+#include "window_chunk.cuh"
 
 namespace aici {
 
@@ -45,16 +49,24 @@ struct WindowDecodeParams {
   int64_t num_blocks, q_stride, kv_block;
   float scale_log2e;
   unsigned int *status;
+  // chunks: first query row of each sequence [num_seqs + 1], head strides and the output's token stride
+  const int32_t *cu_q;
+  int64_t q_head, o_tok, o_head;
+  int items;    // work items of 16 rows to a (sequence, kv head)
+  int total_q;  // query rows of the tensor
 };
 
-// The visible part of a row.
+// The visible part of a work item: of a (sequence, kv head) in decode; in a chunk, what any of the item's
+// tokens sees.
 struct WindowRow {
   int ctx, lo, sinks;        // visible: t < ctx && (t >= lo || t < sinks)
+  int all_hi, all_lo;        // chunks: t < all_hi is not too late for any token, t >= all_lo not too early
   int first, n_sink, tiles;  // first block of the window, blocks of sinks before it, blocks in all
   __device__ __forceinline__ int block(int i) const { return i < n_sink ? i : first + i - n_sink; }
 };
 
-__device__ __forceinline__ WindowRow window_row(const WindowDecodeParams &p, int ctx) {
+// `tokens`: query tokens of the item, the last of them `back` positions before the sequence's last.
+__device__ __forceinline__ WindowRow window_row(const WindowDecodeParams &p, int ctx, int tokens, int back) {
   const int64_t table = (int64_t)p.max_blocks * kWinBlock;
   const int cap = table < p.max_context ? (int)table : p.max_context;
   if (ctx > cap) {
@@ -62,12 +74,14 @@ __device__ __forceinline__ WindowRow window_row(const WindowDecodeParams &p, int
     ctx = cap;
   }
   WindowRow r;
-  r.ctx = max(ctx, 0);
-  r.lo = max(r.ctx - p.window, 0);
-  r.sinks = min(p.sinks, r.ctx);
+  r.ctx = max(ctx, 0) - back;  // below 1: nothing is visible
+  r.lo = (int)max((int64_t)r.ctx - (tokens - 1) - p.window, (int64_t)0);
+  r.all_hi = r.ctx - (tokens - 1);
+  r.all_lo = max(r.ctx - p.window, 0);
+  r.sinks = max(min(p.sinks, r.ctx), 0);
   r.first = r.lo / kWinBlock;
   r.n_sink = min((r.sinks + kWinBlock - 1) / kWinBlock, r.first);
-  r.tiles = r.n_sink + (r.ctx + kWinBlock - 1) / kWinBlock - r.first;
+  r.tiles = r.ctx > 0 ? r.n_sink + (r.ctx + kWinBlock - 1) / kWinBlock - r.first : 0;
   return r;
 }
 
@@ -88,23 +102,34 @@ __device__ __forceinline__ void mma_half<__half>(float (&d)[4], uint32_t a0, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Softmax state of a query-head group against the tiles seen so far, spread over a warp as the
-// mma.sync fragments are: lane (g, tig) holds rows g and (kTwo) g + 8, columns 8 n + 2 tig, + 1.
-template <typename T, bool kTwo>
+// Softmax state of the query rows of a kv head against the tiles seen so far, spread over a warp as the
+// mma.sync fragments are: lane (g, tig) holds rows g and (kTwo) g + 8, columns 8 n + 2 tig, + 1.  Row = head
+// of the group, or in a chunk token * group + head from the item's first row on.
+template <typename T, bool kTwo, bool kChunk>
 struct GroupState {
   static constexpr int kRows = kTwo ? 2 : 1;
+  int hi[kRows], lo[kRows];  // chunks: visible to the row: t < hi && (t >= lo || t < sinks)
   uint32_t qa[8][2 * kRows];
   float o[16][4];  // [n][2..3] stay zero without the second row
   float m[kRows], l[kRows];
 
-  __device__ __forceinline__ void load(const WindowDecodeParams &p, int seq, int kvh, int g, int tig) {
+  // q0: the sequence's first query row of the tensor, pos0: its position; the item has the rows row0 ..
+  // row0 + rows - 1 of the kv head's
+  __device__ __forceinline__ void load(const WindowDecodeParams &p, int q0, int pos0, int row0, int rows, int kvh, int g, int tig) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const T *row = static_cast<const T *>(p.q) + seq * p.q_stride + (int64_t)(kvh * p.group + g + 8 * r) * kWinHead + 2 * tig;
+      const int i = row0 + g + 8 * r, token = kChunk ? i / p.group : 0, head = i - token * p.group;
+      const bool there = g + 8 * r < rows;
+      const T *row = static_cast<const T *>(p.q) + (q0 + token) * p.q_stride +
+                     (kvh * p.group + head) * (kChunk ? p.q_head : (int64_t)kWinHead) + 2 * tig;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        qa[ks][r] = g + 8 * r < p.group ? *reinterpret_cast<const uint32_t *>(row + 16 * ks) : 0u;
-        qa[ks][kRows + r] = g + 8 * r < p.group ? *reinterpret_cast<const uint32_t *>(row + 16 * ks + 8) : 0u;
+        qa[ks][r] = there ? *reinterpret_cast<const uint32_t *>(row + 16 * ks) : 0u;
+        qa[ks][kRows + r] = there ? *reinterpret_cast<const uint32_t *>(row + 16 * ks + 8) : 0u;
+      }
+      if (kChunk) {
+        hi[r] = there ? pos0 + token + 1 : 0;
+        lo[r] = (int)max((int64_t)hi[r] - p.window, (int64_t)0);
       }
       m[r] = -INFINITY;
       l[r] = 0.f;
@@ -132,17 +157,25 @@ struct GroupState {
     }
     // tokens t0 + {2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9}: scores masked by selection, values by clearing
     // (0 x NaN is NaN, and what is not visible may hold anything)
-    bool vis[4] = {true, true, true, true};
+    bool vis[kRows][4];
     uint32_t vm_lo = ~0u, vm_hi = ~0u;
-    const bool edge = t0 + kWinBlock > row.ctx || (t0 < row.lo && t0 + kWinBlock > row.sinks);
+    const bool edge = t0 + kWinBlock > (kChunk ? row.all_hi : row.ctx) ||
+                      (t0 < (kChunk ? row.all_lo : row.lo) && t0 + kWinBlock > row.sinks);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vis[r][j] = true;
     if (edge) {
+      bool any[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int t = t0 + 2 * tig + (j & 1) + 8 * (j >> 1);
-        vis[j] = t < row.ctx && (t >= row.lo || t < row.sinks);
+        any[j] = t < row.ctx && (t >= row.lo || t < row.sinks);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) vis[r][j] = kChunk ? t < hi[r] && (t >= lo[r] || t < row.sinks) : any[j];
       }
-      vm_lo = (vis[0] ? 0xffffu : 0u) | (vis[1] ? 0xffff0000u : 0u);
-      vm_hi = (vis[2] ? 0xffffu : 0u) | (vis[3] ? 0xffff0000u : 0u);
+      vm_lo = (any[0] ? 0xffffu : 0u) | (any[1] ? 0xffff0000u : 0u);
+      vm_hi = (any[2] ? 0xffffu : 0u) | (any[3] ? 0xffff0000u : 0u);
     }
     // A probability goes in as two 16-bit numbers, the rounded value and what the rounding left: the values'
     // product is then as exact as fp32 sums make it, and the output carries one rounding, its own.  (With
@@ -153,8 +186,8 @@ struct GroupState {
     bool moved = false;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const float x0 = vis[0] ? s0[2 * r] * scale : -INFINITY, x1 = vis[1] ? s0[2 * r + 1] * scale : -INFINITY;
-      const float x2 = vis[2] ? s1[2 * r] * scale : -INFINITY, x3 = vis[3] ? s1[2 * r + 1] * scale : -INFINITY;
+      const float x0 = vis[r][0] ? s0[2 * r] * scale : -INFINITY, x1 = vis[r][1] ? s0[2 * r + 1] * scale : -INFINITY;
+      const float x2 = vis[r][2] ? s1[2 * r] * scale : -INFINITY, x3 = vis[r][3] ? s1[2 * r + 1] * scale : -INFINITY;
       float mt = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
@@ -246,7 +279,7 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t local, uint32_t cta) {
   return v;
 }
 
-template <typename T, bool kTwo>
+template <typename T, bool kTwo, bool kChunk>
 __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const WindowDecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kHeads = kTwo ? 16 : 8;
@@ -270,12 +303,27 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int rowi = blockIdx.x / ctas, seq = rowi / p.num_kv_heads, kvh = rowi - seq * p.num_kv_heads;
-  const WindowRow row = window_row(p, p.context_lens[seq]);
+  int item = blockIdx.x / ctas, row0 = 0;
+  if (kChunk) {
+    row0 = item % p.items * 16;
+    item /= p.items;
+  }
+  const int seq = item / p.num_kv_heads, kvh = item - seq * p.num_kv_heads;
+  const int ctx = p.context_lens[seq];
+  int q0 = seq, rows = p.group, tokens = 1, back = 0, all_tokens = 1;
+  if (kChunk) {
+    q0 = min(max(p.cu_q[seq], 0), p.total_q);
+    all_tokens = min(max(p.cu_q[seq + 1], q0), p.total_q) - q0;
+    rows = (int)max(min((int64_t)all_tokens * p.group - row0, (int64_t)kHeads), (int64_t)0);
+    const int last = (row0 + max(rows, 1) - 1) / p.group;  // the item's last token
+    tokens = last - row0 / p.group + 1;
+    back = max(all_tokens - 1 - last, 0);
+  }
+  const WindowRow row = window_row(p, ctx, tokens, back);
   const int stride = ctas * kWinWarps, first = rank * kWinWarps + warp;
-  const int mine = row.tiles > first ? (row.tiles - first + stride - 1) / stride : 0;  // tiles first, first + stride, ...
-  GroupState<T, kTwo> st;
-  st.load(p, seq, kvh, g, tig);
+  const int mine = rows > 0 && row.tiles > first ? (row.tiles - first + stride - 1) / stride : 0;  // tiles first, first + stride, ...
+  GroupState<T, kTwo, kChunk> st;
+  st.load(p, q0, row.ctx + back - all_tokens, row0, rows, kvh, g, tig);
   int ids = 0;
   unsigned issued = 0;
   auto produce = [&]() {
@@ -306,9 +354,9 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   // ---- join the warps of the CTA ----------------------------------------------------------------------
   float *w_o = reinterpret_cast<float *>(ring);  // [kHeads][128] of this warp
 #pragma unroll
-  for (int r = 0; r < GroupState<T, kTwo>::kRows; ++r) {
+  for (int r = 0; r < GroupState<T, kTwo, kChunk>::kRows; ++r) {
     const int h = g + 8 * r;
-    if (h < p.group) {
+    if (h < rows) {
 #pragma unroll
       for (int n = 0; n < 16; ++n)
         *reinterpret_cast<float2 *>(w_o + h * kWinHead + 8 * n + 2 * tig) = make_float2(st.o[n][2 * r], st.o[n][2 * r + 1]);
@@ -316,8 +364,12 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
     }
   }
   __syncthreads();
-  const int items = p.group * (kWinHead / 4);  // four elements of a head each
-  T *out = static_cast<T *>(p.out) + ((int64_t)seq * p.num_heads + kvh * p.group) * kWinHead;
+  const int items = rows * (kWinHead / 4);  // four elements of a row each
+  auto out = [&](int row) {
+    if (!kChunk) return static_cast<T *>(p.out) + ((int64_t)seq * p.num_heads + kvh * p.group + row) * kWinHead;
+    const int token = (row0 + row) / p.group;
+    return static_cast<T *>(p.out) + (q0 + token) * p.o_tok + (kvh * p.group + row0 + row - token * p.group) * p.o_head;
+  };
   for (int i = threadIdx.x; i < items; i += kWinThreads) {
     const int h = i >> 5, d = (i & 31) * 4;
     float m = -INFINITY;
@@ -336,7 +388,7 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
     }
     if (ctas == 1) {
       const float inv = inverse(l);
-      *reinterpret_cast<uint2 *>(out + h * kWinHead + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
+      *reinterpret_cast<uint2 *>(out(h) + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
     } else {
       *reinterpret_cast<float4 *>(s_o + h * kWinHead + d) = a;
       if ((i & 31) == 0) s_ml[h] = make_float2(m, l);
@@ -371,7 +423,7 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
         a.x += f * v[c].x; a.y += f * v[c].y; a.z += f * v[c].z; a.w += f * v[c].w;
       }
     const float inv = inverse(l);
-    *reinterpret_cast<uint2 *>(out + h * kWinHead + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
+    *reinterpret_cast<uint2 *>(out(h) + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
   }
   // nobody leaves while its shared memory may still be read
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -380,9 +432,9 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
 
 // ---- host side -----------------------------------------------------------------------------------------
 // Most tiles a row can have.
-static int64_t most_tiles(int64_t max_context, int64_t window, int64_t sinks) {
+static int64_t most_tiles(int64_t max_context, int64_t window, int64_t sinks, int64_t tokens) {
   const int64_t all = (max_context + kWinBlock - 1) / kWinBlock;
-  const int64_t seen = (window + kWinBlock - 1) / kWinBlock + 1 + (sinks + kWinBlock - 1) / kWinBlock;
+  const int64_t seen = (window + tokens - 1 + kWinBlock - 1) / kWinBlock + 1 + (sinks + kWinBlock - 1) / kWinBlock;
   return seen < all ? seen : all;
 }
 
@@ -395,12 +447,12 @@ static int ctas_per_row(int64_t rows, int64_t tiles) {
   return c;
 }
 
-template <typename T, bool kTwo>
+template <typename T, bool kTwo, bool kChunk>
 static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStream_t stream) {
   constexpr int kSmem = kWinRingBytes + kWinBarBytes + (kTwo ? 16 : 8) * (kWinHead * 4 + 8 + kWinWarps * 8);
   static OncePerDevice once;
   if (char *e = once.run([]() -> char * {
-        AICI_CUDA(cudaFuncSetAttribute(window_decode_kernel<T, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        AICI_CUDA(cudaFuncSetAttribute(window_decode_kernel<T, kTwo, kChunk>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         return nullptr;
       }))
     return e;
@@ -414,14 +466,50 @@ static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStr
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.num_seqs * p.num_kv_heads * ctas));
+  cfg.gridDim = dim3((unsigned)((int64_t)p.num_seqs * p.num_kv_heads * p.items * ctas));
   cfg.blockDim = dim3(kWinThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  AICI_CUDA(cudaLaunchKernelEx(&cfg, window_decode_kernel<T, kTwo>, p));
+  AICI_CUDA(cudaLaunchKernelEx(&cfg, window_decode_kernel<T, kTwo, kChunk>, p));
   return nullptr;
+}
+
+char *launch_window_chunk(const WindowChunk &c, int dtype, cudaStream_t stream) {
+  WindowDecodeParams p = {};
+  p.out = c.out;
+  p.q = c.q;
+  p.k = c.key_cache;
+  p.v = c.value_cache;
+  p.block_tables = c.block_tables;
+  p.context_lens = c.context_lens;
+  p.num_seqs = c.batch;
+  p.num_heads = c.num_heads;
+  p.num_kv_heads = c.num_kv_heads;
+  p.group = c.num_heads / c.num_kv_heads;
+  p.window = c.window;
+  p.sinks = c.sinks;
+  p.max_blocks = c.max_blocks;
+  p.max_context = 0x7fffffff;  // as in the general kernel the table's width alone limits a context
+  p.num_blocks = c.num_blocks;
+  p.q_stride = c.q_tok;
+  p.kv_block = c.kv_block;
+  p.scale_log2e = c.scale * 1.4426950408889634f;
+  p.status = c.status;
+  p.cu_q = c.cu_q;
+  p.q_head = c.q_head;
+  p.o_tok = c.o_tok;
+  p.o_head = c.o_head;
+  p.items = (int)window_chunk_items(c.max_tokens, p.group);
+  p.total_q = c.total_q;
+  const int ctas = ctas_per_row((int64_t)c.batch * c.num_kv_heads * p.items,
+                                most_tiles(c.max_context, c.window, c.sinks, c.max_tokens));
+  return with_half_type(dtype, [&](auto t) -> char * {
+    using T = decltype(t);
+    return c.max_tokens > 8 / p.group ? launch_window_decode<T, true, true>(p, ctas, stream)
+                                      : launch_window_decode<T, false, true>(p, ctas, stream);
+  });
 }
 
 }  // namespace aici
@@ -481,10 +569,11 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
   p.kv_block = kv_block_stride;
   p.scale_log2e = scale * 1.4426950408889634f;
   p.status = st;
+  p.items = 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int ctas = ctas_per_row((int64_t)num_seqs * num_kv_heads, most_tiles(max_context_len, window, sinks));
+  const int ctas = ctas_per_row((int64_t)num_seqs * num_kv_heads, most_tiles(max_context_len, window, sinks, 1));
   return with_half_type(dtype, [&](auto t) -> char * {
     using T = decltype(t);
-    return group > 8 ? launch_window_decode<T, true>(p, ctas, s) : launch_window_decode<T, false>(p, ctas, s);
+    return group > 8 ? launch_window_decode<T, true, false>(p, ctas, s) : launch_window_decode<T, false, false>(p, ctas, s);
   });
 }

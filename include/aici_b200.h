@@ -495,8 +495,8 @@ char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, voi
  * The query at position p of its sequence sees the tokens t <= p with t > p - window or t < sinks
  * (window >= 1, sinks >= 0; a window that covers the context gives causal attention).  bf16 or f16,
  * head_size 128, block_size 16; fp32 scores and sums.  Probabilities meet the values in the 16-bit type:
- * prefill rounds them, decode adds what the rounding left as a second product.  A row that sees nothing
- * is zero.
+ * prefill rounds them, decode and short paged chunks add what the rounding left as a second product.  A
+ * row that sees nothing is zero.
  *
  * Decode over the paged cache, arguments as in aici_paged_attention_v1: one query per sequence at
  * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number.  Blocks that hold no

@@ -270,6 +270,27 @@ def test_prefill(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype, is_pa
     assert _lib.last_status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
+    ([4], [900], 4, 1, 100, 3), ([16], [300], 2, 2, 7, 0), ([2, 0, 3, 1], [40, 50, 2, 1000], 8, 2, 64, 4), ([8], [8], 2, 1, 3, 1),
+    ([16, 5], [700, 3], 1, 1, 10, 0), ([1] * 90, [70 + i for i in range(90)], 16, 1, 33, 17), ([3] * 40, [3 + 7 * i for i in range(40)], 5, 1, 90, 0),
+    ([7, 8], [2000, 1990], 4, 2, 1 << 40, 0), ([2], [17], 16, 2, 16, 16), ([9, 16, 1], [500, 20, 800], 15, 3, 64, 5),
+    ([300], [1500], 4, 2, 200, 33), ([40, 0, 61], [40, 9, 333], 28, 4, 50, 1), ([16] * 40, [30 + 9 * i for i in range(40)], 24, 8, 75, 2),
+    ([33], [2222], 48, 1, 1000, 130), ([2048], [2048], 2, 1, 64, 0)])
+def test_prefill_few_rows(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype):
+    """Chunks of at most 16 tokens, or with all items of 16 rows (tokens x heads of a kv head) resident at once,
+    have a form of their own, which carries what rounding a probability left; the others round it."""
+    items = len(lens_q) * Hk * -(-max(lens_q) * (H // Hk) // 16)
+    split = max(lens_q) <= 16 or items <= 2 * torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    g = torch.Generator().manual_seed(sum(lens_k) + window % 1000)
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, True)
+    at = 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        near(out[at:at + lq], q[at:at + lq], ks[i], vs[i], range(lk - lq, lk), window, sinks, dtype, split=split)
+        at += lq
+    assert _lib.last_status() == 0
+
+
 @pytest.mark.parametrize("is_paged", [False, True])
 @pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
     ([2500], [2500], 4, 2, 700, 4), ([300, 900], [3500, 900], 8, 1, 2300, 200), ([700], [4400], 6, 6, 4096, 0),
