@@ -216,6 +216,8 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     table, rows = block_tables.shape, block_tables.stride()
     if len(table) != 2 or table[0] != n or rows[1] != 1:
         raise AiciError("%s: block_tables must be [requests, max_blocks] with contiguous rows" % fn)
+    if not 0 <= max_tokens < 1 << 30:
+        raise AiciError("%s: bad max_tokens %d" % (fn, max_tokens))
     if out is None:
         # one allocation; the token tensors first, each on a 16-byte boundary
         gap = 2 * (max_tokens % 2)

@@ -17,8 +17,8 @@ inline int64_t window_chunk_items(int64_t max_tokens, int64_t group) { return (m
 // heads over 8, window 4096: 4 tokens 14 and 115, 64 tokens 41 and 85, 128 tokens = 256 items 71 and 81,
 // 256 tokens = 512 items 140 and 81).
 inline bool window_chunk_takes(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t max_tokens) {
-  return max_tokens <= 16 ||
-         batch * num_kv_heads * window_chunk_items(max_tokens, num_heads / num_kv_heads) <= 2 * sm_count();
+  const int64_t items = batch * num_kv_heads * window_chunk_items(max_tokens, num_heads / num_kv_heads);
+  return max_tokens <= 16 ? items < (1ll << 31) /* a grid's width */ : items <= 2 * sm_count();
 }
 
 struct WindowChunk {

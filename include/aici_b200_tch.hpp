@@ -722,6 +722,7 @@ inline StepTables step_tables(const Tensor &query_lens, const Tensor &context_le
   const int n = (int)query_lens.numel();
   require(fn, context_lens.numel() == n && block_tables.dim() == 2 && block_tables.size(0) == n && free_count.numel() == 1,
           "query_lens and context_lens must be [requests], block_tables [requests, max_blocks], free_count [1]");
+  require(fn, max_tokens >= 0, "bad max_tokens");
   StepTables r;
   r.seqlens_q = Tensor::empty({n + 1}, Kind::Int, dev);
   r.positions = Tensor::empty({max_tokens}, Kind::Int64, dev);

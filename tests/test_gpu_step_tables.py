@@ -161,3 +161,6 @@ def test_refuses_out_of_another_shape(cuda_device):
     res, bt = call(cuda_device, *args)
     with pytest.raises(_lib.AiciError, match="out does not match"):
         call(cuda_device, *args[:5], args[5] + 1, args[6], out=res)
+    for tokens in (-1, 1 << 30, 1 << 32):
+        with pytest.raises(_lib.AiciError, match="max_tokens"):
+            call(cuda_device, *args[:5], tokens, args[6])

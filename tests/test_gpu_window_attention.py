@@ -291,6 +291,24 @@ def test_prefill_few_rows(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dty
     assert _lib.last_status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
+    ([130, 1, 17, 0, 64], [130, 900, 17, 50, 333], 16, 8, 100, 3), ([300], [300], 24, 24, 1, 0), ([257, 3], [700, 2], 20, 10, 64, 130),
+    ([129], [1400], 64, 2, 300, 33), ([140], [1200], 40, 40, 1000, 0), ([200, 150], [900, 2000], 32, 4, 800, 5),
+    ([0, 128, 256], [3, 128, 255], 28, 28, 1 << 40, 2), ([60] * 20, [60 + 13 * i for i in range(20)], 8, 4, 129, 1)])
+def test_prefill_paged_tiles(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype):
+    """Chunks too many for the form above: tiles of 128 rows over the paged cache."""
+    assert max(lens_q) > 16 and len(lens_q) * Hk * -(-max(lens_q) * (H // Hk) // 16) > 2 * 148
+    g = torch.Generator().manual_seed(sum(lens_k) + H)
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, True)
+    at = 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        rows = range(0, lq, 1 if lq < 70 else 3)
+        near(out[at:at + lq][list(rows)], q[at:at + lq][list(rows)], ks[i], vs[i], [lk - lq + r for r in rows], window, sinks, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
 @pytest.mark.parametrize("is_paged", [False, True])
 @pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
     ([2500], [2500], 4, 2, 700, 4), ([300, 900], [3500, 900], 8, 1, 2300, 200), ([700], [4400], 6, 6, 4096, 0),
@@ -392,6 +410,16 @@ def test_rows_behind_the_last_sequence_stay(cuda_device):
     assert (out[130:] == 7.0).all()
 
 
+def test_sizes_as_other_integers(cuda_device):
+    """Sizes that come out of a tensor or an array."""
+    dev, g = cuda_device, torch.Generator().manual_seed(16)
+    q, k = normal(g, torch.bfloat16, 40, 2, D), normal(g, torch.bfloat16, 40, 2, D)
+    cu = torch.tensor([0, 40], dtype=torch.int32, device=dev)
+    out = tch_cuda.flash_attn_varlen_window(q.to(dev), k.to(dev), k.to(dev), cu, cu, cu.max(), cu[-1], SCALE, torch.tensor(9),
+                                            torch.tensor(2)).cpu()
+    near(out, q, k, k, range(40), 9, 2, torch.bfloat16)
+
+
 def test_refuses_mismatched_tensors(cuda_device):
     dev = cuda_device
     q, i = torch.zeros(4, 2, D, dtype=torch.bfloat16, device=dev), torch.tensor([0, 4], dtype=torch.int32, device=dev)
@@ -399,7 +427,8 @@ def test_refuses_mismatched_tensors(cuda_device):
         q=q, k=q, v=q, seqlens_q=i, seqlens_k=i, max_seqlen_q=4, max_seqlen_k=4, softmax_scale=1.0, window=4), **c})
     for change, match in ((dict(k=q.half()), "same dtype"), (dict(v=q[:3]), "k and v"), (dict(seqlens_q=i.long()), "seqlens_q"),
                           (dict(seqlens_k=i[:1]), "seqlens_k"), (dict(q=q.float(), k=q.float(), v=q.float()), "only bf16 and f16"),
-                          (dict(q=q.transpose(1, 2)), "contiguous last"), (dict(window=0), "window"), (dict(sinks=-1), "sinks")):
+                          (dict(q=q.transpose(1, 2)), "contiguous last"), (dict(window=0), "window"), (dict(sinks=-1), "sinks"),
+                          (dict(window=5 - (1 << 32)), "window"), (dict(sinks=-(1 << 40)), "sinks")):
         with pytest.raises(_lib.AiciError, match=match):
             f(**change)
     f()
