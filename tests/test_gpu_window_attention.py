@@ -410,6 +410,25 @@ def test_rows_behind_the_last_sequence_stay(cuda_device):
     assert (out[130:] == 7.0).all()
 
 
+@pytest.mark.parametrize("is_paged", [False, True])
+@pytest.mark.parametrize("lens_q", [
+    [3] * 40 + [700] + [0] * 5, [0, 0, 290] + [1, 0, 130] * 12, [900] + [17] * 31, [128] * 3 + [5] * 70 + [513] + [0] * 1000 + [129],
+    [0] * 31 + [400]], ids=["long_in_the_middle", "empty_ones", "long_first", "a_thousand_empty", "long_last"])
+def test_prefill_ragged_batches(cuda_device, lens_q, is_paged):
+    """Batches in which one sequence has many more tiles than the others; the rows at the tiles' ends."""
+    dtype, H, Hk, window, sinks = torch.bfloat16, 12, 6, 70, 3
+    g = torch.Generator().manual_seed(len(lens_q))
+    lens_k = [lq + i % 50 for i, lq in enumerate(lens_q)]
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged)
+    at = 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        rows = [r for r in range(lq) if r % 128 in (0, 1, 40, 127) or r == lq - 1]
+        if rows:
+            near(out[at:at + lq][rows], q[at:at + lq][rows], ks[i], vs[i], [lk - lq + r for r in rows], window, sinks, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
 def test_sizes_as_other_integers(cuda_device):
     """Sizes that come out of a tensor or an array."""
     dev, g = cuda_device, torch.Generator().manual_seed(16)
