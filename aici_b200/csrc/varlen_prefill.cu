@@ -107,6 +107,7 @@ struct PrefillParams {
   int64_t num_blocks;
   // windowed variant: a row at position d sees the keys t <= d with t > d - window or t < sinks
   int window, sinks;
+  int longer_than;        // sequences of at most so many tokens are another launch's
   int batch, grid_heads;  // grid_heads > 0: its grid is (tile, head), heads fastest, and batch_tile finds the tile
 };
 
@@ -184,7 +185,7 @@ __device__ __forceinline__ BatchTile batch_tile(const PrefillParams &p, int idx,
     const int i = min(lane, p.batch - 1);
     const int q0 = p.cu_q[i], q1 = p.cu_q[i + 1];
     const int k0 = kPaged ? 0 : p.cu_k[i], k1 = kPaged ? p.k_lens[i] : p.cu_k[i + 1];
-    const int n = lane < p.batch ? max(q1 - q0 + kBM - 1, 0) / kBM : 0;
+    const int n = lane < p.batch && q1 - q0 > p.longer_than ? (q1 - q0 + kBM - 1) / kBM : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -217,7 +218,7 @@ __device__ __forceinline__ BatchTile batch_tile(const PrefillParams &p, int idx,
   t.mb = idx - start(lo);
   t.q0 = p.cu_q[lo];
   t.lq = p.cu_q[lo + 1] - t.q0;
-  if (t.mb < 0 || t.mb >= (t.lq + kBM - 1) / kBM) return t;
+  if (t.lq <= p.longer_than || t.mb < 0 || t.mb >= (t.lq + kBM - 1) / kBM) return t;
   t.b = lo;
   t.k0 = kPaged ? 0 : p.cu_k[lo];
   t.lk = kPaged ? p.k_lens[lo] : p.cu_k[lo + 1] - t.k0;
@@ -273,11 +274,16 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // The grid is ordered (head, sequence, row tile) with the row tile as the slowest index: all the
   // longest tiles of the batch start first and the CTAs with one key tile fill the tail.  (Windowed: see
   // BatchTile.)
+  // Beside a launch for the short sequences (longer_than > 0) this grid starts while that one runs, whose
+  // CTAs have waited for everything before them; CTA 0 leaves after it, so that this grid ends last.
+  auto leave = [&]() {
+    if (kWindow && p.longer_than > 0 && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
   int b, q0, lq, k0 = 0, lk = 0, win_mb = 0, win_head = 0;
   if (kWindow && p.grid_heads > 0) {
     const int tile = (int)blockIdx.x / p.grid_heads;
     const BatchTile t = batch_tile<kPaged>(p, tile, lane);
-    if (t.b < 0) return;
+    if (t.b < 0) return leave();
     b = t.b, q0 = t.q0, lq = t.lq, k0 = t.k0, lk = t.lk, win_mb = t.mb;
     win_head = (int)blockIdx.x - tile * p.grid_heads;
   } else {
@@ -339,7 +345,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
       T.n_tiles = (T.rows > 0 && lim > 0) ? (lim + kBN - 1) / kBN : 0;
     }
   }
-  if (tiles[0].rows == 0 && tiles[1].rows == 0) return;
+  if (tiles[0].rows == 0 && tiles[1].rows == 0) return leave();
   const int hk = tiles[1].rows > 0 ? tiles[1].h / p.group : tiles[0].h / p.group;
   // tiles that see no key at all are zero rows (flash_fwd_kernel.h:1056)
   if (tiles[0].rows > 0 && tiles[0].n_tiles == 0) zero_rows(p, q0, tiles[0], tid, kPrefillThreads);
@@ -359,7 +365,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   }
   const int nt0 = tiles[0].n_tiles, nt1 = tiles[1].n_tiles;
   const int nmax = max(nt0, nt1);
-  if (nmax == 0) return;
+  if (nmax == 0) return leave();
   auto tile_of = [&](int j) { return kWindow ? win.tile(j) : j; };  // key tile of the j-th visit
   // end of the keys that count for this CTA, and whether any key of a 16-token block does
   const int k_end = kWindow ? win.lim : lk;
@@ -1169,6 +1175,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     if (kPair) tmem_dealloc_pair(tmem_base, kTmemCols);
     else tmem_dealloc(tmem_base, kTmemCols);
   }
+  leave();
 }
 
 // ---- host side -------------------------------------------------------------------------------------
@@ -1308,9 +1315,9 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
     const int heads = Cfg::kTiles == 1 ? num_heads : num_heads / 2;
     const int64_t room = (int64_t)p.total_q / kBM + batch, most = (int64_t)batch * mblocks;
     p.pair_heads = Cfg::kTiles == 1 ? 0 : 1;
-    p.grid_heads = most > room ? heads : 0;
+    p.grid_heads = most > room || p.longer_than > 0 ? heads : 0;
     AICI_CHECK(room * heads < (1ll << 31), "prefill: too many tiles for one call");
-    grid = most > room ? dim3((unsigned)(room * heads)) : dim3(heads, batch, mblocks);
+    grid = p.grid_heads > 0 ? dim3((unsigned)(room * heads)) : dim3(heads, batch, mblocks);
   } else if (Cfg::kTiles == 1) {
     grid = dim3(num_heads, batch, mblocks);
   } else {
@@ -1326,6 +1333,12 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
   cfg.dynamicSmemBytes = Cfg::kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
+  if (kWindow && p.longer_than > 0) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
   if (Cfg::kPair) {
     // clusters of two CTAs along x: the pair works on four query heads of one kv head
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1496,6 +1509,7 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   p.num_blocks = 0;
   p.window = win ? win->window : 0;
   p.sinks = win ? win->sinks : 0;
+  p.longer_than = 0;
   p.batch = batch;
   p.grid_heads = 0;
   // every output buffer gets a tensor map like the query's; this rank's heads start at out_head0
@@ -1618,12 +1632,15 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   unsigned int *st = status_ptr();
   AICI_CHECK(st != nullptr, "%s: no CUDA device", fn);
 
-  if (win != nullptr && window_chunk_takes(batch, num_heads, num_kv_heads, max_seqlen_q)) {
+  const bool all_short = win != nullptr && window_chunk_takes(batch, num_heads, num_kv_heads, max_seqlen_q);
+  const bool some_short = win != nullptr && !all_short && window_chunk_mixed(batch, total_q, max_seqlen_q);
+  if (all_short || some_short) {
     const WindowChunk c = {out, q, key_cache, value_cache, cu_seqlens_q, context_lens, block_tables, batch, total_q, num_heads,
-                           num_kv_heads, max_seqlen_q, max_context_len, max_num_blocks_per_seq, win->window, win->sinks,
+                           num_kv_heads, all_short ? max_seqlen_q : kWindowChunkTokens, max_context_len, max_num_blocks_per_seq, win->window, win->sinks,
                            num_blocks, q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
                            softmax_scale, st};
-    return launch_window_chunk(c, dtype, static_cast<cudaStream_t>(stream));
+    char *e = launch_window_chunk(c, dtype, static_cast<cudaStream_t>(stream));
+    if (e != nullptr || all_short) return e;
   }
 
   CUtensorMap tq, tk, tv;
@@ -1652,6 +1669,7 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   p.num_blocks = num_blocks;
   p.window = win ? win->window : 0;
   p.sinks = win ? win->sinks : 0;
+  p.longer_than = some_short ? kWindowChunkTokens : 0;
   p.batch = batch;
   p.grid_heads = 0;
   OutMaps to = {};

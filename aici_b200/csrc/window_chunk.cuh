@@ -9,6 +9,8 @@ namespace aici {
 // Work items of 16 rows (tokens x heads of a kv head) to a (sequence, kv head).
 inline int64_t window_chunk_items(int64_t max_tokens, int64_t group) { return (max_tokens * group + 15) / 16; }
 
+constexpr int kWindowChunkTokens = 16;
+
 // Whether a call takes this form: chunks of at most 16 tokens, where an item does at least the work of a
 // query head (64 sequences at context 8192, window 4096, us here and in the general kernel's 128-row tiles:
 // 32 heads over 8, 4 tokens 166 and 807, 16 tokens 490 and 800, 32 tokens 973 and 630; 8 heads over 8, 16
@@ -18,14 +20,24 @@ inline int64_t window_chunk_items(int64_t max_tokens, int64_t group) { return (m
 // 256 tokens = 512 items 140 and 81).
 inline bool window_chunk_takes(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t max_tokens) {
   const int64_t items = batch * num_kv_heads * window_chunk_items(max_tokens, num_heads / num_kv_heads);
-  return max_tokens <= 16 ? items < (1ll << 31) /* a grid's width */ : items <= 2 * sm_count();
+  return max_tokens <= kWindowChunkTokens ? items < (1ll << 31) /* a grid's width */ : items <= 2 * sm_count();
+}
+
+// Whether, in a call that does not, the sequences of at most kWindowChunkTokens tokens get a launch of this
+// form beside the general kernel's (a step of single tokens and some chunks).  The host knows no lengths: it
+// does so where the mean is below half the longest, or no other sum is possible.  In us, with and without, at
+// 32 heads over 8: 63 single tokens and a chunk of 512, context 6000: 44 and 141 (window 128), 240 and 886
+// (4096); 3 and a chunk: 20 and 30, 89 and 119; 4 chunks of 64 to 512, for which there is nothing to gain: 21
+// and 33 (its tiles are also found by batch_tile), 94 and 93.
+inline bool window_chunk_mixed(int64_t batch, int64_t total_q, int64_t max_tokens) {
+  return 2 * total_q < batch * max_tokens || total_q < (kWindowChunkTokens + 1) * (batch - 1) + max_tokens;
 }
 
 struct WindowChunk {
   void *out;
   const void *q, *key_cache, *value_cache;
   const int32_t *cu_q, *context_lens, *block_tables;
-  int batch, total_q, num_heads, num_kv_heads, max_tokens, max_context, max_blocks, window, sinks;
+  int batch, total_q, num_heads, num_kv_heads, max_tokens /* sequences with more are left out */, max_context, max_blocks, window, sinks;
   int64_t num_blocks, q_tok, q_head, o_tok, o_head, kv_block;
   float scale;
   unsigned int *status;

@@ -54,6 +54,7 @@ struct WindowDecodeParams {
   int64_t q_head, o_tok, o_head;
   int items;    // work items of 16 rows to a (sequence, kv head)
   int total_q;  // query rows of the tensor
+  int max_tokens;
 };
 
 // The visible part of a work item: of a (sequence, kv head) in decode; in a chunk, what any of the item's
@@ -314,6 +315,7 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   if (kChunk) {
     q0 = min(max(p.cu_q[seq], 0), p.total_q);
     all_tokens = min(max(p.cu_q[seq + 1], q0), p.total_q) - q0;
+    if (all_tokens > p.max_tokens) all_tokens = 0;
     rows = (int)max(min((int64_t)all_tokens * p.group - row0, (int64_t)kHeads), (int64_t)0);
     const int last = (row0 + max(rows, 1) - 1) / p.group;  // the item's last token
     tokens = last - row0 / p.group + 1;
@@ -503,6 +505,7 @@ char *launch_window_chunk(const WindowChunk &c, int dtype, cudaStream_t stream) 
   p.o_head = c.o_head;
   p.items = (int)window_chunk_items(c.max_tokens, p.group);
   p.total_q = c.total_q;
+  p.max_tokens = c.max_tokens;
   const int ctas = ctas_per_row((int64_t)c.batch * c.num_kv_heads * p.items,
                                 most_tiles(c.max_context, c.window, c.sinks, c.max_tokens));
   return with_half_type(dtype, [&](auto t) -> char * {

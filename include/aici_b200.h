@@ -512,7 +512,8 @@ char *aici_paged_attention_window(void *out, const void *query, const void *key_
 
 /* Prefill over packed keys and values (arguments as in aici_mha_varlen_fwd) and over the paged cache
  * (as in aici_mha_varlen_paged_fwd); row r of a sequence is the token at position len_k - len_q + r, any
- * number of query heads per kv head.  Tokens that none of the 128 rows of a query tile (rows
+ * number of query heads per kv head.  Over the paged cache a step may mix single tokens and chunks: sequences
+ * of at most 16 tokens are worked on beside the others in a second launch.  Tokens that none of the 128 rows of a query tile (rows
  * 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token that one of
  * them sees are not read. */
 char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,

@@ -429,6 +429,63 @@ def test_prefill_ragged_batches(cuda_device, lens_q, is_paged):
     assert _lib.last_status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
+    ([1] * 20 + [300], [37 * i + 1 for i in range(20)] + [900], 16, 4, 90, 2), ([0, 16, 17, 1, 600], [9, 500, 17, 1, 640], 24, 12, 130, 0),
+    ([257] + [1] * 40, [257] + [11 * i + 3 for i in range(40)], 8, 8, 1 << 40, 0), ([2] * 7 + [400, 0], [3000 + i for i in range(7)] + [400, 7], 40, 8, 1000, 9),
+    ([500, 3, 16, 0, 1], [2, 3, 10, 5, 1], 64, 4, 20, 1)])
+def test_prefill_mixed_batches(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype):
+    """Steps of single tokens and chunks: sequences of at most 16 tokens take one form, the others another."""
+    assert 2 * sum(lens_q) < len(lens_q) * max(lens_q) or sum(lens_q) < 17 * (len(lens_q) - 1) + max(lens_q)
+    assert len(lens_q) * Hk * -(-max(lens_q) * (H // Hk) // 16) > 2 * 148
+    g = torch.Generator().manual_seed(sum(lens_k) + H)
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, True)
+    at = 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        rows = [r for r in range(lq) if lq < 20 or r % 7 == 0 or r % 128 in (0, 127) or r == lq - 1]
+        if rows:
+            near(out[at:at + lq][rows], q[at:at + lq][rows], ks[i], vs[i], [lk - lq + r for r in rows], window, sinks, dtype,
+                 split=lq <= 16)
+        at += lq
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("lens_q", [[1] * 50 + [900], [1] * 50 + [0]])
+def test_mixed_batches_end_before_what_follows(cuda_device, lens_q):
+    """The two launches of a mixed step overlap: what comes behind them, on the stream or in a captured graph, sees
+    the rows of both, and the inputs may be written again.  (The second batch leaves the later launch nothing.)"""
+    dev, dtype, H, Hk = cuda_device, torch.bfloat16, 8, 2
+    g = torch.Generator().manual_seed(21)
+    lens_k = [2500 if lq < 2 else lq for lq in lens_q]
+    kc, vc, table, _, _ = (x.to(dev) if torch.is_tensor(x) else x for x in paged(g, lens_k, Hk, dtype))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cu, ctx, total = i32([sum(lens_q[:i]) for i in range(len(lens_q) + 1)]), i32(lens_k), sum(lens_q)
+    qs = [normal(g, dtype, total, H, D).to(dev) for _ in range(4)]
+    q, got = qs[0].clone(), torch.zeros(4, total, H, D, dtype=dtype, device=dev)
+    call = lambda x: tch_cuda.flash_attn_varlen_paged_window(x, kc, vc, cu, ctx, table, 900, 2500, SCALE, 2000, 4)  # noqa: E731
+    want = []
+    for x in qs:
+        want.append(call(x))
+        torch.cuda.synchronize()
+    def steps():
+        for i, x in enumerate(qs):
+            q.copy_(x)
+            got[i].copy_(call(q))
+            q.fill_(NAN)
+    for _ in range(5):
+        got.zero_()
+        steps()
+        assert torch.equal(got, torch.stack(want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps()
+    for _ in range(5):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, torch.stack(want))
+    assert torch.isfinite(got).all() and _lib.last_status() == 0
+
+
 def test_sizes_as_other_integers(cuda_device):
     """Sizes that come out of a tensor or an array."""
     dev, g = cuda_device, torch.Generator().manual_seed(16)
