@@ -38,6 +38,7 @@
 // visible pairs; 4 x 4096, 32/8 heads, window 1024: 331 us = 729, window 128: 171 us = 204, where a CTA's
 // fixed cost (fill 4300 clk, epilogue 2700) and the diagonal's two passes weigh as much as the MMAs.
 // Every barrier wait is bounded; a timeout sets AICI_STATUS_WAIT_TIMEOUT and unwinds.
+#include "dependent.cuh"
 #include "half_types.cuh"
 #include "tcgen05.cuh"
 #include "window_chunk.cuh"
@@ -279,6 +280,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   auto leave = [&]() {
     if (kWindow && p.longer_than > 0 && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
+  if (kWindow && p.longer_than == 0) dependent_start();
   int b, q0, lq, k0 = 0, lk = 0, win_mb = 0, win_head = 0;
   if (kWindow && p.grid_heads > 0) {
     const int tile = (int)blockIdx.x / p.grid_heads;
@@ -1333,9 +1335,8 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
   cfg.dynamicSmemBytes = Cfg::kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
-  if (kWindow && p.longer_than > 0) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  if (kWindow) {
+    attr[0] = dependent_launch();
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }

@@ -26,6 +26,7 @@
 // cluster of 8: 9.8 against 24 us).  What that other form is better at is a batch with one row far longer
 // than the rest: a CTA alone streams a tile in 0.19 us, so the last row to start costs at most that
 // times its tiles.
+#include "dependent.cuh"
 #include "half_types.cuh"
 #include "window_chunk.cuh"
 
@@ -301,8 +302,7 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
     fence_mbar_init();
   }
   __syncwarp();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  dependent_start();
 
   int item = blockIdx.x / ctas, row0 = 0;
   if (kChunk) {
@@ -458,11 +458,8 @@ static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStr
         return nullptr;
       }))
     return e;
-  // a programmatic dependent: its prologue overlaps the tail of the grid before it, and it waits for
-  // that grid before it touches anything
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0] = dependent_launch();
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = 1;
