@@ -203,11 +203,11 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     Returns a StepTables."""
     fn = "step_tables"
     given = (query_lens, context_lens, block_tables, free_blocks, free_count)
-    index = _one_gpu(fn, given)
+    index, int32 = _one_gpu(fn, given), torch.int32
     for t in given:
-        if t.dtype is not torch.int32:
+        if t.dtype is not int32:
             raise AiciError("%s: lengths, tables and free list must be int32" % fn)
-        if not t.is_contiguous() and t is not block_tables:
+        if t is not block_tables and not t.is_contiguous():
             raise AiciError("%s: lengths and free list must be contiguous" % fn)
     n = query_lens.numel()
     if query_lens.dim() != 1 or context_lens.shape != query_lens.shape or free_blocks.dim() != 1 or \
@@ -219,11 +219,13 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     if not 0 <= max_tokens < 1 << 30:
         raise AiciError("%s: bad max_tokens %d" % (fn, max_tokens))
     if out is None:
-        # one allocation; the token tensors first, each on a 16-byte boundary
-        gap = 2 * (max_tokens % 2)
-        buf = query_lens.new_empty(3 * max_tokens + gap + 3 * n + 2)
-        positions, _, slots, seqlens, logits, context, count = buf.split_with_sizes(
-            (2 * max_tokens, gap, max_tokens, n + 1, n, n, 1))
+        # one allocation; the token tensors first, each on a 16-byte boundary (a piece costs the host 0.9 us)
+        if max_tokens % 2 == 0:
+            positions, slots, seqlens, logits, context, count = query_lens.new_empty(
+                3 * max_tokens + 3 * n + 2).split_with_sizes((2 * max_tokens, max_tokens, n + 1, n, n, 1))
+        else:
+            positions, _, slots, seqlens, logits, context, count = query_lens.new_empty(
+                3 * max_tokens + 3 * n + 4).split_with_sizes((2 * max_tokens, 2, max_tokens, n + 1, n, n, 1))
         positions = positions.view(torch.int64)
         out = StepTables(seqlens, positions, slots, logits, context, count)
     else:
