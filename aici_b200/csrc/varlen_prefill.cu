@@ -34,8 +34,8 @@
 // multiplied (N of the S MMA, K steps of the P V MMAs), so four sinks cost a quarter of a tile.  What bounds
 // long calls is what bounds the kernel without a window, the tensor pipe with its operand reads: 3650 clk for
 // a step of two tiles where the MMAs alone would take 3136 (in-kernel time stamps, 1.75 GHz under load), of
-// which the issuing warp waits 590.  2 x 32768 tokens, 64/8 heads, window 4096: 8.4 ms = 980 TFLOP/s of
-// visible pairs; 4 x 4096, 32/8 heads, window 1024: 331 us = 729, window 128: 171 us = 204, where a CTA's
+// which the issuing warp waits 590.  2 x 32768 tokens, 64/8 heads, window 4096: 8.6 ms = 957 TFLOP/s of
+// visible pairs; 4 x 4096, 32/8 heads, window 1024: 332 us = 725, window 128: 170 us = 205, where a CTA's
 // fixed cost (fill 4300 clk, epilogue 2700) and the diagonal's two passes weigh as much as the MMAs.
 // Every barrier wait is bounded; a timeout sets AICI_STATUS_WAIT_TIMEOUT and unwinds.
 #include "dependent.cuh"
