@@ -275,8 +275,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // The grid is ordered (head, sequence, row tile) with the row tile as the slowest index: all the
   // longest tiles of the batch start first and the CTAs with one key tile fill the tail.  (Windowed: see
   // BatchTile.)
-  // Beside a launch for the short sequences (longer_than > 0) this grid starts while that one runs, whose
-  // CTAs have waited for everything before them; CTA 0 leaves after it, so that this grid ends last.
+  // Beside a launch for the short sequences (longer_than > 0) this grid starts while that one runs, which
+  // began only when everything before it had ended; CTA 0 leaves after it, so that this grid ends last.
   auto leave = [&]() {
     if (kWindow && p.longer_than > 0 && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
@@ -1639,7 +1639,7 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
     const WindowChunk c = {out, q, key_cache, value_cache, cu_seqlens_q, context_lens, block_tables, batch, total_q, num_heads,
                            num_kv_heads, all_short ? max_seqlen_q : kWindowChunkTokens, max_context_len, max_num_blocks_per_seq, win->window, win->sinks,
                            num_blocks, q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
-                           softmax_scale, st};
+                           softmax_scale, st, !all_short};
     char *e = launch_window_chunk(c, dtype, static_cast<cudaStream_t>(stream));
     if (e != nullptr || all_short) return e;
   }

@@ -41,6 +41,7 @@ struct WindowChunk {
   int64_t num_blocks, q_tok, q_head, o_tok, o_head, kv_block;
   float scale;
   unsigned int *status;
+  bool beside;  // the general kernel's launch follows and starts with it: begin behind all that came before
 };
 
 char *launch_window_chunk(const WindowChunk &c, int dtype, cudaStream_t stream);

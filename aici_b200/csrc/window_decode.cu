@@ -450,7 +450,7 @@ static int ctas_per_row(int64_t rows, int64_t tiles) {
 }
 
 template <typename T, bool kTwo, bool kChunk>
-static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStream_t stream) {
+static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStream_t stream, bool overlap = true) {
   constexpr int kSmem = kWinRingBytes + kWinBarBytes + (kTwo ? 16 : 8) * (kWinHead * 4 + 8 + kWinWarps * 8);
   static OncePerDevice once;
   if (char *e = once.run([]() -> char * {
@@ -460,6 +460,7 @@ static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStr
     return e;
   cudaLaunchAttribute attr[2];
   attr[0] = dependent_launch();
+  attr[0].val.programmaticStreamSerializationAllowed = overlap;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = 1;
@@ -507,8 +508,8 @@ char *launch_window_chunk(const WindowChunk &c, int dtype, cudaStream_t stream) 
                                 most_tiles(c.max_context, c.window, c.sinks, c.max_tokens));
   return with_half_type(dtype, [&](auto t) -> char * {
     using T = decltype(t);
-    return c.max_tokens > 8 / p.group ? launch_window_decode<T, true, true>(p, ctas, stream)
-                                      : launch_window_decode<T, false, true>(p, ctas, stream);
+    return c.max_tokens > 8 / p.group ? launch_window_decode<T, true, true>(p, ctas, stream, !c.beside)
+                                      : launch_window_decode<T, false, true>(p, ctas, stream, !c.beside);
   });
 }
 

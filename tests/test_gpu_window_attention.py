@@ -486,6 +486,47 @@ def test_mixed_batches_end_before_what_follows(cuda_device, lens_q):
     assert torch.isfinite(got).all() and _lib.last_status() == 0
 
 
+def test_mixed_batches_see_what_came_before(cuda_device):
+    """Lengths, block tables, queries and caches written by the kernels right before the call, at the same addresses
+    with other contents each time."""
+    dev, dtype, H, Hk, B = cuda_device, torch.bfloat16, 8, 2, 40
+    g = torch.Generator().manual_seed(22)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    sets = []
+    for s in range(4):
+        lens_q = [1] * B
+        lens_q[7 * s] = 700 - s
+        lens_k = [900 + 13 * s + i for i in range(B)]
+        kc, vc, table, _, _ = paged(g, [1000] * B, Hk, dtype)
+        cu = i32([sum(lens_q[:i]) for i in range(B + 1)])
+        sets.append([x.to(dev) for x in (normal(g, dtype, 739, H, D), kc, vc, cu, i32(lens_k), table)])
+    call = lambda x: tch_cuda.flash_attn_varlen_paged_window(*x, 700, 1000, SCALE, 500, 4)  # noqa: E731
+    want = []
+    for x in sets:
+        want.append(call(x)[:int(x[3][-1])].clone())
+        torch.cuda.synchronize()
+    now, got = [x.clone() for x in sets[0]], torch.zeros(4, 739, H, D, dtype=dtype, device=dev)
+    def steps():
+        for i, x in enumerate(sets):
+            for a, b in zip(now, x):
+                a.copy_(b)
+            got[i].copy_(call(now))
+    def check():
+        for i, w in enumerate(want):
+            assert torch.equal(got[i, :len(w)], w), i
+    for _ in range(5):
+        steps()
+        check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps()
+    for _ in range(10):
+        got.zero_()
+        graph.replay()
+        check()
+    assert _lib.last_status() == 0
+
+
 def test_sizes_as_other_integers(cuda_device):
     """Sizes that come out of a tensor or an array."""
     dev, g = cuda_device, torch.Generator().manual_seed(16)
