@@ -246,8 +246,8 @@ __device__ __forceinline__ void zero_rows(const PrefillParams &p, int q0, const 
 // kPaged = true : K and V come from the paged cache.  A key tile is 16 half-blocks of
 //   [16 chunks][8 tokens][8 elements] (2 KB each, no swizzle: exactly the 8-row x 16-byte core
 //   matrices the MMA wants, leading offset 128 B between the two chunks of a K step, stride offset
-//   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] loaded with the
-//   32-byte swizzle, one K = 16 MMA per block.  Value columns past the sequence end are zeroed in
+//   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] in the
+//   32-byte swizzle, d reordered in groups of four, one K = 16 MMA per block.  Value columns past the sequence end are zeroed in
 //   shared memory before P V (cache slots there may hold anything, NaN included).
 //
 // kWindow = true: sliding window and sinks (always causal); the CTA's tiles share their rows (one tile, or
@@ -1115,10 +1115,11 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 v;
-          v.x = Half16<T16>::pack(__uint_as_float(r[8 * q + 0]) * inv, __uint_as_float(r[8 * q + 1]) * inv);
-          v.y = Half16<T16>::pack(__uint_as_float(r[8 * q + 2]) * inv, __uint_as_float(r[8 * q + 3]) * inv);
-          v.z = Half16<T16>::pack(__uint_as_float(r[8 * q + 4]) * inv, __uint_as_float(r[8 * q + 5]) * inv);
-          v.w = Half16<T16>::pack(__uint_as_float(r[8 * q + 6]) * inv, __uint_as_float(r[8 * q + 7]) * inv);
+          const int f = kPaged ? q : 0;  // cache V: see make_cache_tmap
+          v.x = Half16<T16>::pack(__uint_as_float(r[8 * q + (0 ^ f)]) * inv, __uint_as_float(r[8 * q + (1 ^ f)]) * inv);
+          v.y = Half16<T16>::pack(__uint_as_float(r[8 * q + (2 ^ f)]) * inv, __uint_as_float(r[8 * q + (3 ^ f)]) * inv);
+          v.z = Half16<T16>::pack(__uint_as_float(r[8 * q + (4 ^ f)]) * inv, __uint_as_float(r[8 * q + (5 ^ f)]) * inv);
+          v.w = Half16<T16>::pack(__uint_as_float(r[8 * q + (6 ^ f)]) * inv, __uint_as_float(r[8 * q + (7 ^ f)]) * inv);
           const int chunk = 4 * c4 + q;
           *reinterpret_cast<uint4 *>(stage + (chunk >> 3) * kPanelBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
         }
@@ -1267,7 +1268,7 @@ static char *make_tmap(const char *fn, CUtensorMap *map, const void *base, int64
 }
 
 // Paged caches: kind 1 = key cache (5-D, one half block per box), kind 2 = value cache (4-D, one
-// block per box, 32-byte swizzle).
+// block per box).
 static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base, bool value,
                              int num_kv_heads, int64_t num_blocks, int64_t kv_head_stride,
                              int64_t kv_block_stride, bool keep) {
@@ -1281,11 +1282,15 @@ static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base,
     cuuint64_t str[4] = {128, 256, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
     cuuint32_t box[5] = {64, 1, 16, 1, 1};
     if (char *e = make_tmap_nd(fn, map, base, 5, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return e;
-  } else {  // [blk][h][d = 128][tok = 16]: box = one block, rows of 32 bytes
-    cuuint64_t dims[4] = {16, 128, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
-    cuuint64_t str[3] = {32, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
-    cuuint32_t box[4] = {16, 128, 1, 1};
-    if (char *e = make_tmap_nd(fn, map, base, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_32B)) return e;
+  } else {
+    // [blk][h][d = 128][tok = 16]: box = one block, four d to a row of 128 bytes (as rows of 32 bytes the engine
+    // moves it far slower).  The MMA reads it as rows of 32 bytes with the 32-byte swizzle, address bit 4 ^= bit
+    // 7; the 128-byte swizzle of the copy does that and bits 5, 6 ^= bits 8, 9 besides, which only reorders the
+    // d in groups of four: column d of the output arrives as column d ^ (d / 8 % 4), and the epilogue knows.
+    cuuint64_t dims[4] = {64, 32, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
+    cuuint64_t str[3] = {128, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
+    cuuint32_t box[4] = {64, 32, 1, 1};
+    if (char *e = make_tmap_nd(fn, map, base, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
   }
   if (keep) g_tmap_cache.put(key, *map);
   return nullptr;
@@ -1373,15 +1378,16 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
 
 // Windowed variant.  A query tile visits window / 128 + 1 key tiles and the sinks' tiles: by that length
 // and not the sequence's a call takes shape 1 or 2; two tiles of a CTA are two heads of one kv head.
-// Paged tiles cost the copy engine more (values move in rows of 32 bytes), so sharing them between two
-// query tiles pays earlier: 8 chunks of 512 rows, 32/8 heads, window 256: 67 us one-tile, 72 us two-tile;
-// window 1024: 129 and 122 us; packed, window 1024: 111 and 119 us.
+// A paged tile is 24 copies where a packed one is 4, and the one-tile shape's two stages hide less of them, so
+// sharing tiles between two query tiles pays earlier: paged, 4 x 4096, 32/8 heads, window 640: 286 us one-tile
+// and 304 two-tile, 1024: 353 and 365, 1536: 432 and 434, 2048: 495 and 490; 8 chunks of 512 with 8192 cached:
+// 93.6 and 96.6, 122.0 and 121.4, 160.8 and 155.7, 207 and 189; packed, chunks, window 1024: 110 and 119.
 template <bool kPaged, typename T16>
 static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                                    const OutMaps &to, PrefillParams &p, int num_heads, int batch, int max_seqlen_q,
                                    int max_seqlen_k, cudaStream_t stream) {
   p.pair_heads = 0;
-  const int64_t keys = (int64_t)p.window + p.sinks, most = kPaged ? 640 : AICI_PREFILL_ONE_TILE_MAX_K;
+  const int64_t keys = (int64_t)p.window + p.sinks, most = kPaged ? 1280 : AICI_PREFILL_ONE_TILE_MAX_K;
   if (p.group % 2 != 0 || (keys < max_seqlen_k ? keys : max_seqlen_k) <= most)
     return launch_prefill_shape<kPaged, 1, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
   return launch_prefill_shape<kPaged, 2, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
