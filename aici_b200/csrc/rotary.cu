@@ -306,10 +306,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_
   double s, c, ds, dc;
   sincos((double)pos0 * p.freq[j], &s, &c);
   sincos(p.freq[j], &ds, &dc);
+  c *= p.by;  // the turns keep the length
+  s *= p.by;
   C *row = static_cast<C *>(p.out) + pos0 * p.rot_dim + j;
   for (int k = 0; k < n; ++k) {
-    put(row, c * p.by);
-    put(row + half, s * p.by);
+    put(row, c);
+    put(row + half, s);
     const double t = c * dc - s * ds;
     s = s * dc + c * ds;
     c = t;
