@@ -1381,13 +1381,14 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
 // A paged tile is 24 copies where a packed one is 4, and the one-tile shape's two stages hide less of them, so
 // sharing tiles between two query tiles pays earlier: paged, 4 x 4096, 32/8 heads, window 640: 286 us one-tile
 // and 304 two-tile, 1024: 353 and 365, 1536: 432 and 434, 2048: 495 and 490; 8 chunks of 512 with 8192 cached:
-// 93.6 and 96.6, 122.0 and 121.4, 160.8 and 155.7, 207 and 189; packed, chunks, window 1024: 110 and 119.
+// 93.6 and 96.6, 122.0 and 121.4, 160.8 and 155.7, 207 and 189.  Packed, 4 x 4096, 2048: 472 and 490, 4096: 585
+// and 572; chunks, 1024: 110 and 119, 2048: 188 and 195, 4096: 326 and 320.
 template <bool kPaged, typename T16>
 static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                                    const OutMaps &to, PrefillParams &p, int num_heads, int batch, int max_seqlen_q,
                                    int max_seqlen_k, cudaStream_t stream) {
   p.pair_heads = 0;
-  const int64_t keys = (int64_t)p.window + p.sinks, most = kPaged ? 1280 : AICI_PREFILL_ONE_TILE_MAX_K;
+  const int64_t keys = (int64_t)p.window + p.sinks, most = kPaged ? 1280 : 2560;
   if (p.group % 2 != 0 || (keys < max_seqlen_k ? keys : max_seqlen_k) <= most)
     return launch_prefill_shape<kPaged, 1, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);
   return launch_prefill_shape<kPaged, 2, true, T16>(tq, tk, tv, to, p, num_heads, batch, max_seqlen_q, stream);

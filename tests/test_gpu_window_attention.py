@@ -326,6 +326,24 @@ def test_prefill_long(cuda_device, lens_q, lens_k, H, Hk, window, sinks, is_page
     assert _lib.last_status() == 0
 
 
+@pytest.mark.parametrize("is_paged", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,window,sinks", [
+    ([2800, 1], [2900, 2900], 8, 4, 2650, 130), ([700, 90], [3300, 2700], 16, 4, 1 << 40, 0), ([640], [5000], 12, 6, 2560, 1)])
+def test_prefill_two_tile_shape(cuda_device, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged):
+    """Windows of more than 2560 keys and an even number of heads to a kv head: two heads' tiles to a CTA."""
+    assert min(window + sinks, max(lens_k)) > 2560 and H // Hk % 2 == 0
+    assert len(lens_q) * Hk * -(-max(lens_q) * (H // Hk) // 16) > 2 * 148
+    g = torch.Generator().manual_seed(sum(lens_k) + H)
+    out, q, ks, vs = run_prefill(cuda_device, g, lens_q, lens_k, H, Hk, window, sinks, dtype, is_paged, hide=len(lens_q) == 1)
+    r, at = random.Random(2), 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        rows = sorted(set(r.sample(range(lq), min(lq, 30)) + [x for x in (0, 1, 127, 128, lq - 129, lq - 2, lq - 1) if 0 <= x < lq]))
+        near(out[at:at + lq][rows], q[at:at + lq][rows], ks[i], vs[i], [lk - lq + x for x in rows], window, sinks, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window,sinks", [(60, 0), (200, 3), (1000, 0)])
 def test_prefill_uneven_scores(cuda_device, dtype, window, sinks):
