@@ -243,8 +243,8 @@ __device__ __forceinline__ void zero_rows(const PrefillParams &p, int q0, const 
 }
 
 // kPaged = false: K and V are packed [total_k, Hkv, 128] tensors (tensor maps as for Q).
-// kPaged = true : K and V come from the paged cache.  A key tile is 16 half-blocks of
-//   [16 chunks][8 tokens][8 elements] (2 KB each, no swizzle: exactly the 8-row x 16-byte core
+// kPaged = true : K and V come from the paged cache.  A key tile is 8 blocks of two halves,
+//   [16 chunks][8 tokens][8 elements] each (2 KB, no swizzle: exactly the 8-row x 16-byte core
 //   matrices the MMA wants, leading offset 128 B between the two chunks of a K step, stride offset
 //   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] in the
 //   32-byte swizzle, d reordered in groups of four, one K = 16 MMA per block.  Value columns past the sequence end are zeroed in
@@ -436,8 +436,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     }
     if (kPaged) {
       // All lanes take part: lane l < 8 owns cache block l of the tile (its id is read once per
-      // tile, one tile ahead), lanes 0-15 each issue one half-block key copy, lanes 0-7 one value
-      // copy; lane 0 posts the expected byte count.
+      // tile, one tile ahead), lanes 0-7 each issue one key copy or one value copy; lane 0 posts the expected byte count.
       const int32_t *bt_row = p.block_tables + (int64_t)b * p.max_blocks;
       auto load_id = [&](int j) {
         int id = 0;
@@ -469,9 +468,7 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
           if (lane < 8 && counts) tma_load_4d(dst + bi * 4096, &tmap_v, 0, 0, hk, id_cur, &sh->kv_full[stage]);
           id_cur = id_next;
         } else {
-          if (lane < 16 && counts)
-            tma_load_5d(dst + bi * 4096 + (lane >> 3) * 2048, &tmap_k, 0, lane >> 3, 0, hk, id_cur,
-                        &sh->kv_full[stage]);
+          if (lane < 8 && counts) tma_load_5d(dst + bi * 4096, &tmap_k, 0, 0, 0, hk, id_cur, &sh->kv_full[stage]);
         }
         __syncwarp();
       }
@@ -1267,8 +1264,9 @@ static char *make_tmap(const char *fn, CUtensorMap *map, const void *base, int64
   return nullptr;
 }
 
-// Paged caches: kind 1 = key cache (5-D, one half block per box), kind 2 = value cache (4-D, one
-// block per box).
+// Paged caches: kind 1 = key cache (5-D), kind 2 = value cache (4-D), one block per box.
+// What a copy costs the engine is some 20 clk and its rows of 128 bytes: with 16 key and 8 value copies a tile
+// 8 chunks of 512, window 1024, take 121.8 us, with 8 and 8 119.2, and packed keys (4 copies) 110.
 static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base, bool value,
                              int num_kv_heads, int64_t num_blocks, int64_t kv_head_stride,
                              int64_t kv_block_stride, bool keep) {
@@ -1276,11 +1274,11 @@ static char *make_cache_tmap(const char *fn, CUtensorMap *map, const void *base,
   if (keep && g_tmap_cache.find(key, map)) return nullptr;
   if (!value) {
     // [blk][h][c = 16][tok = 16][e = 8], a chunk taken as two halves of 8 tokens x 8 elements = 128
-    // contiguous bytes: box = one half of all chunks, 16 rows of 128 bytes for the engine (the same bytes as
-    // 128 rows of 16, which it moves far slower)
-    cuuint64_t dims[5] = {64, 2, 16, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
-    cuuint64_t str[4] = {128, 256, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
-    cuuint32_t box[5] = {64, 1, 16, 1, 1};
+    // contiguous bytes (as rows of 16 bytes the engine moves it far slower); the map's order is chunk, then
+    // half, so that one copy of a block leaves its halves one behind the other
+    cuuint64_t dims[5] = {64, 16, 2, (cuuint64_t)num_kv_heads, (cuuint64_t)num_blocks};
+    cuuint64_t str[4] = {256, 128, (cuuint64_t)kv_head_stride * 2, (cuuint64_t)kv_block_stride * 2};
+    cuuint32_t box[5] = {64, 16, 2, 1, 1};
     if (char *e = make_tmap_nd(fn, map, base, 5, dims, str, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return e;
   } else {
     // [blk][h][d = 128][tok = 16]: box = one block, four d to a row of 128 bytes (as rows of 32 bytes the engine
@@ -1378,7 +1376,7 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
 
 // Windowed variant.  A query tile visits window / 128 + 1 key tiles and the sinks' tiles: by that length
 // and not the sequence's a call takes shape 1 or 2; two tiles of a CTA are two heads of one kv head.
-// A paged tile is 24 copies where a packed one is 4, and the one-tile shape's two stages hide less of them, so
+// A paged tile is 16 copies where a packed one is 4, and the one-tile shape's two stages hide less of them, so
 // sharing tiles between two query tiles pays earlier: paged, 4 x 4096, 32/8 heads, window 640: 286 us one-tile
 // and 304 two-tile, 1024: 353 and 365, 1536: 432 and 434, 2048: 495 and 490; 8 chunks of 512 with 8192 cached:
 // 93.6 and 96.6, 122.0 and 121.4, 160.8 and 155.7, 207 and 189.  Packed, 4 x 4096, 2048: 472 and 490, 4096: 585
