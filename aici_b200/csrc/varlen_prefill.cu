@@ -246,9 +246,9 @@ __device__ __forceinline__ void zero_rows(const PrefillParams &p, int q0, const 
 // kPaged = true : K and V come from the paged cache.  A key tile is 8 blocks of two halves,
 //   [16 chunks][8 tokens][8 elements] each (2 KB, no swizzle: exactly the 8-row x 16-byte core
 //   matrices the MMA wants, leading offset 128 B between the two chunks of a K step, stride offset
-//   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] in the
-//   32-byte swizzle, d reordered in groups of four, one K = 16 MMA per block.  Value columns past the sequence end are zeroed in
-//   shared memory before P V (cache slots there may hold anything, NaN included).
+//   2 KB between 8-token groups); a value tile is 8 blocks of [128 d][16 tokens] in the 32-byte swizzle,
+//   d reordered in groups of four, one K = 16 MMA per block.  Value columns past the sequence end
+//   are zeroed in shared memory before P V (cache slots there may hold anything, NaN included).
 //
 // kWindow = true: sliding window and sinks (always causal); the CTA's tiles share their rows (one tile, or
 // two heads of one kv head).  T: bf16, or f16 in the windowed variant.
