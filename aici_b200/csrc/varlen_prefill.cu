@@ -109,6 +109,7 @@ struct PrefillParams {
   // windowed variant: a row at position d sees the keys t <= d with t > d - window or t < sinks
   int window, sinks;
   int longer_than;        // sequences of at most so many tokens are another launch's
+  int max_q;              // sequences of more are refused: zero rows and a status
   int batch, grid_heads;  // grid_heads > 0: its grid is (tile, head), heads fastest, and batch_tile finds the tile
 };
 
@@ -307,6 +308,16 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     if (lk < 0) lk = 0;
   }
   const int n_mblocks = (lq + kBM - 1) / kBM;
+  if (kWindow && lq > p.max_q) {
+    // Longer than the caller stated: the plain grid has no CTA for some of its tiles, so none is worked on
+    // (in the ragged grid neither: what a call gives does not depend on the other sequences' lengths).
+    if (tid == 0) set_status(p.status, AICI_STATUS_BAD_BLOCK);
+    const int first = p.grid_heads > 0 ? win_mb : (int)blockIdx.z, step = p.grid_heads > 0 ? n_mblocks : (int)gridDim.z;
+    for (int mb = first; mb < n_mblocks; mb += step)
+      for (int t = 0; t < kTiles; ++t)
+        zero_rows(p, q0, TileInfo{kTiles * win_head + t, mb * kBM, min(kBM, lq - mb * kBM), 0}, tid, kPrefillThreads);
+    return leave();
+  }
   if (kWindow && p.grid_heads == 0) win_mb = n_mblocks - 1 - (int)blockIdx.z;
 
   // ---- which two tiles does this CTA own? (longest causal tiles are scheduled first) ----------
@@ -1516,6 +1527,7 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   p.window = win ? win->window : 0;
   p.sinks = win ? win->sinks : 0;
   p.longer_than = 0;
+  p.max_q = max_seqlen_q;
   p.batch = batch;
   p.grid_heads = 0;
   // every output buffer gets a tensor map like the query's; this rank's heads start at out_head0
@@ -1676,6 +1688,7 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   p.window = win ? win->window : 0;
   p.sinks = win ? win->sinks : 0;
   p.longer_than = some_short ? kWindowChunkTokens : 0;
+  p.max_q = max_seqlen_q;
   p.batch = batch;
   p.grid_heads = 0;
   OutMaps to = {};

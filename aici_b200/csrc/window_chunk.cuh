@@ -37,7 +37,9 @@ struct WindowChunk {
   void *out;
   const void *q, *key_cache, *value_cache;
   const int32_t *cu_q, *context_lens, *block_tables;
-  int batch, total_q, num_heads, num_kv_heads, max_tokens /* sequences with more are left out */, max_context, max_blocks, window, sinks;
+  int batch, total_q, num_heads, num_kv_heads;
+  int max_tokens;  // sequences with more are refused, or (beside) left out
+  int max_context, max_blocks, window, sinks;
   int64_t num_blocks, q_tok, q_head, o_tok, o_head, kv_block;
   float scale;
   unsigned int *status;

@@ -56,6 +56,7 @@ struct WindowDecodeParams {
   int items;    // work items of 16 rows to a (sequence, kv head)
   int total_q;  // query rows of the tensor
   int max_tokens;
+  int refuse;   // sequences of more than max_tokens tokens: 1 = zero rows and a status, 0 = another launch's
 };
 
 // The visible part of a work item: of a (sequence, kv head) in decode; in a chunk, what any of the item's
@@ -315,7 +316,19 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   if (kChunk) {
     q0 = min(max(p.cu_q[seq], 0), p.total_q);
     all_tokens = min(max(p.cu_q[seq + 1], q0), p.total_q) - q0;
-    if (all_tokens > p.max_tokens) all_tokens = 0;
+    if (all_tokens > p.max_tokens) {
+      if (p.refuse) {
+        if (threadIdx.x == 0) set_status(p.status, AICI_STATUS_BAD_BLOCK);
+        // its rows are dealt out to the CTAs that it has
+        const int width = p.group * (kWinHead / 8), parts = p.items * (int)ctas;
+        for (int token = row0 / 16 * (int)ctas + (int)rank; token < all_tokens; token += parts)
+          for (int i = threadIdx.x; i < width; i += kWinThreads)
+            *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + (q0 + token) * p.o_tok +
+                                       (kvh * p.group + i / (kWinHead / 8)) * p.o_head + i % (kWinHead / 8) * 8) =
+                make_uint4(0, 0, 0, 0);
+      }
+      all_tokens = 0;
+    }
     rows = (int)max(min((int64_t)all_tokens * p.group - row0, (int64_t)kHeads), (int64_t)0);
     const int last = (row0 + max(rows, 1) - 1) / p.group;  // the item's last token
     tokens = last - row0 / p.group + 1;
@@ -504,6 +517,7 @@ char *launch_window_chunk(const WindowChunk &c, int dtype, cudaStream_t stream) 
   p.items = (int)window_chunk_items(c.max_tokens, p.group);
   p.total_q = c.total_q;
   p.max_tokens = c.max_tokens;
+  p.refuse = c.beside ? 0 : 1;
   const int ctas = ctas_per_row((int64_t)c.batch * c.num_kv_heads * p.items,
                                 most_tiles(c.max_context, c.window, c.sinks, c.max_tokens));
   return with_half_type(dtype, [&](auto t) -> char * {

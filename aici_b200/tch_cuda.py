@@ -879,7 +879,9 @@ def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
                              seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float,
                              window: int, sinks: int = 0) -> torch.Tensor:
     """flash_attn_varlen, causal, with a sliding window: a query at position p of its sequence sees the
-    tokens t <= p with t > p - window or t < sinks.  bf16 or f16.  Returns [total_q, num_heads, head_size]."""
+    tokens t <= p with t > p - window or t < sinks.  bf16 or f16.  Returns [total_q, num_heads, head_size].
+    A sequence with more than `max_seqlen_q` tokens gives zero rows and sets a status bit (see
+    _lib.last_status)."""
     fn = "flash_attn_varlen_window"
     index = _one_gpu(fn, (q, k, v, seqlens_q, seqlens_k))
     batch = _check_prefill(fn, q, seqlens_q)
@@ -891,11 +893,12 @@ def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         raise AiciError("%s: query, key and value must have the same dtype" % fn)
     if seqlens_k.dtype is not torch.int32 or not seqlens_k.is_contiguous() or seqlens_k.numel() != batch + 1:
         raise AiciError("%s: seqlens_k must be contiguous int32 and as long as seqlens_q" % fn)
-    out = q.new_empty(q.shape)
+    max_seqlen_q = int(max_seqlen_q)
+    out = q.new_empty(q.shape) if max_seqlen_q else q.new_zeros(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_window_fwd", index, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
           seqlens_q.data_ptr(), seqlens_k.data_ptr(), batch, total_q, k.shape[0], num_heads, k.shape[1], head_size,
-          int(max_seqlen_q), int(max_seqlen_k), _int32(window), _int32(sinks), q_tok, q_head, ks[0], ks[1], vs[0], vs[1],
+          max_seqlen_q, int(max_seqlen_k), _int32(window), _int32(sinks), q_tok, q_head, ks[0], ks[1], vs[0], vs[1],
           num_heads * head_size, head_size, softmax_scale, _dtype(fn, q))
     return out
 
@@ -905,7 +908,8 @@ def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, val
                                    max_seqlen_q: int, max_context_len: int, softmax_scale: float, window: int,
                                    sinks: int = 0) -> torch.Tensor:
     """flash_attn_varlen_paged, causal, with the window of flash_attn_varlen_window: the new tokens of a
-    chunk against the paged cache.  bf16 or f16.  Blocks without a visible token are never read."""
+    chunk against the paged cache.  bf16 or f16.  Blocks without a visible token are never read.  A sequence
+    with more than `max_seqlen_q` tokens gives zero rows and sets a status bit (see _lib.last_status)."""
     fn = "flash_attn_varlen_paged_window"
     index = _one_gpu(fn, (q, key_cache, value_cache, seqlens_q, context_lens, block_tables))
     num_blocks, num_kv_heads, head_size, block_size = _cache_dims(fn, key_cache, value_cache)
@@ -916,11 +920,12 @@ def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, val
     if q.dtype is not key_cache.dtype or q.dtype is not value_cache.dtype:
         raise AiciError("%s: query and cache dtypes differ" % fn)
     _check_table(fn, block_tables, context_lens, batch)
-    out = q.new_empty(q.shape)
+    max_seqlen_q = int(max_seqlen_q)
+    out = q.new_empty(q.shape) if max_seqlen_q else q.new_zeros(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_paged_window_fwd", index, out.data_ptr(), q.data_ptr(), key_cache.data_ptr(),
           value_cache.data_ptr(), seqlens_q.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), batch,
-          total_q, num_heads, num_kv_heads, head_size, block_size, int(max_seqlen_q), int(max_context_len),
+          total_q, num_heads, num_kv_heads, head_size, block_size, max_seqlen_q, int(max_context_len),
           block_tables.shape[1], num_blocks, _int32(window), _int32(sinks), q_tok, q_head, num_heads * head_size,
           head_size, key_cache.stride(0), key_cache.stride(1), softmax_scale, _dtype(fn, q))
     return out

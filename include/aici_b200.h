@@ -43,7 +43,8 @@ enum { AICI_DTYPE_BF16 = 0, AICI_DTYPE_F16 = 1, AICI_DTYPE_F32 = 2 };
 /* Sticky device-side status bits, read with aici_last_status(). */
 enum {
   AICI_STATUS_OK = 0,
-  AICI_STATUS_BAD_BLOCK = 1,   /* a block-table entry was outside [0, num_blocks)        */
+  AICI_STATUS_BAD_BLOCK = 1,   /* a block-table entry was outside [0, num_blocks), or a sequence did
+                                  not fit the lengths of the call                         */
   AICI_STATUS_BAD_SLOT = 2,    /* a slot index was outside the cache                      */
   AICI_STATUS_WAIT_TIMEOUT = 4, /* a bounded wait on a shared-memory barrier gave up      */
   AICI_STATUS_PEER_TIMEOUT = 8, /* a peer GPU did not reach a barrier within its bounded wait */
@@ -515,7 +516,8 @@ char *aici_paged_attention_window(void *out, const void *query, const void *key_
  * number of query heads per kv head.  Over the paged cache a step may mix single tokens and chunks: sequences
  * of at most 16 tokens are worked on beside the others in a second launch.  Tokens that none of the 128 rows of a query tile (rows
  * 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token that one of
- * them sees are not read. */
+ * them sees are not read.  The rows of a sequence with more than max_seqlen_q tokens are zero and the status
+ * says AICI_STATUS_BAD_BLOCK; max_seqlen_q = 0 says that there are no query tokens, and nothing is written. */
 char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
                                  const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
                                  int total_q, int total_k, int num_heads, int num_heads_k, int head_size,

@@ -647,7 +647,18 @@ inline void paged_attention_window(Tensor &out, const Tensor &query, const Tenso
                                         detail::dtype_of(fn, query), stream));
 }
 
-// flash_attn_varlen, causal, with the window; returns a new tensor shaped like q.
+namespace detail {
+// What a windowed prefill returns: zeros where the call says that there are no query tokens.
+inline Tensor rows_like(const char *fn, const Tensor &q, int dev, size_t max_seqlen_q, cudaStream_t stream) {
+  Tensor out = Tensor::empty(q.sizes, q.kind, dev);
+  DeviceGuard guard(dev);
+  if (max_seqlen_q == 0) cuda_check(fn, cudaMemsetAsync(out.data, 0, (size_t)out.numel() * element_size(q.kind), stream));
+  return out;
+}
+}  // namespace detail
+
+// flash_attn_varlen, causal, with the window; returns a new tensor shaped like q.  A sequence with more than
+// max_seqlen_q tokens gives zero rows and sets a status bit (last_status).
 inline Tensor flash_attn_varlen_window(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &seqlens_q,
                                        const Tensor &seqlens_k, size_t max_seqlen_q, size_t max_seqlen_k,
                                        float softmax_scale, int window, int sinks = 0,
@@ -662,7 +673,7 @@ inline Tensor flash_attn_varlen_window(const Tensor &q, const Tensor &k, const T
   require(fn, seqlens_q.kind == Kind::Int && seqlens_k.kind == Kind::Int && seqlens_q.is_contiguous() &&
                   seqlens_k.is_contiguous() && seqlens_q.numel() == seqlens_k.numel() && seqlens_q.numel() > 1,
           "seqlens_q and seqlens_k must be contiguous int32 [batch + 1]");
-  Tensor out = Tensor::empty(q.sizes, q.kind, dev);
+  Tensor out = detail::rows_like(fn, q, dev, max_seqlen_q, stream);
   detail::DeviceGuard guard(dev);
   check(fn, aici_mha_varlen_window_fwd(
                 out.data, q.data, k.data, v.data, static_cast<const int32_t *>(seqlens_q.data),
@@ -692,7 +703,7 @@ inline Tensor flash_attn_varlen_paged_window(const Tensor &q, const Tensor &key_
   const int batch = (int)seqlens_q.numel() - 1;
   require(fn, batch > 0 && context_lens.numel() == batch && block_tables.dim() == 2 && block_tables.size(0) == batch,
           "context_lens must be [batch] and block_tables [batch, max_blocks]");
-  Tensor out = Tensor::empty(q.sizes, q.kind, dev);
+  Tensor out = detail::rows_like(fn, q, dev, max_seqlen_q, stream);
   detail::DeviceGuard guard(dev);
   check(fn, aici_mha_varlen_paged_window_fwd(
                 out.data, q.data, key_cache.data, value_cache.data, static_cast<const int32_t *>(seqlens_q.data),

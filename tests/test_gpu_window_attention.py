@@ -567,3 +567,70 @@ def test_refuses_mismatched_tensors(cuda_device):
         with pytest.raises(_lib.AiciError, match=match):
             f(**change)
     f()
+
+
+def into(out, dev, q, kv, lens_q, lens_k, max_q, window, sinks, table=None, total=None, cu_q=None):
+    """A windowed prefill through the C ABI into a buffer that is there before: `kv` is (keys, values) of the
+    packed form, or the caches where there is a table."""
+    p = lambda t: t.data_ptr()  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    sums = lambda lens: [sum(lens[:i]) for i in range(len(lens) + 1)]  # noqa: E731
+    L, H, (a, b) = _lib.lib(), q.shape[1], kv
+    cu = i32(cu_q or sums(lens_q))
+    total, dt, s = total or q.shape[0], 0 if q.dtype == torch.bfloat16 else 1, torch.cuda.current_stream().cuda_stream
+    if table is None:
+        ck, Hk = i32(sums(lens_k)), a.shape[1]
+        _lib.check("x", L.aici_mha_varlen_window_fwd(
+            p(out), p(q), p(a), p(b), p(cu), p(ck), len(lens_q), total, a.shape[0], H, Hk, D, max_q, max(lens_k), window, sinks,
+            H * D, D, Hk * D, D, Hk * D, D, H * D, D, SCALE, dt, s))
+    else:
+        ck, Hk = i32(lens_k), a.shape[1]
+        _lib.check("x", L.aici_mha_varlen_paged_window_fwd(
+            p(out), p(q), p(a), p(b), p(cu), p(ck), p(table), len(lens_q), total, H, Hk, D, 16, max_q, max(lens_k),
+            table.shape[1], a.shape[0], window, sinks, H * D, D, H * D, D, a.stride(0), a.stride(1), SCALE, dt, s))
+    torch.cuda.synchronize()
+
+
+LIES = [  # paged, query lengths, the stated longest, heads, kv heads
+    (False, [40, 300, 64], 130, 4, 2), (False, [300] + [5] * 9, 140, 4, 2), (False, [200] + [5] * 40, 140, 2, 2),
+    (True, [3, 20, 1], 8, 4, 2), (True, [50, 90], 60, 2, 1), (True, [9, 2], 1, 24, 1), (True, [40, 300, 64], 130, 32, 32),
+    (True, [1] * 20 + [300, 400], 300, 16, 4), (True, [17] + [1] * 40, 16, 8, 8)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("is_paged,lens_q,stated,H,Hk", LIES)
+def test_prefill_of_a_sequence_longer_than_stated(cuda_device, is_paged, lens_q, stated, H, Hk, dtype):
+    """Whatever form the call takes, the sequence's rows are zero and the status says so; the others are right."""
+    dev, g = cuda_device, torch.Generator().manual_seed(sum(lens_q) + H)
+    lens_k = [lq + 11 for lq in lens_q]
+    q = normal(g, dtype, sum(lens_q), H, D)
+    if is_paged:
+        kc, vc, table, ks, vs = paged(g, lens_k, Hk, dtype)
+        kv, table = (kc.to(dev), vc.to(dev)), table.to(dev)
+    else:
+        ks, vs = ([normal(g, dtype, n, Hk, D) for n in lens_k] for _ in range(2))
+        kv, table = (torch.cat(ks).to(dev), torch.cat(vs).to(dev)), None
+    out = torch.full_like(q, 7.0).to(dev)
+    into(out, dev, q.to(dev), kv, lens_q, lens_k, stated, 50, 2, table)
+    out, at = out.cpu(), 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        if lq > stated:
+            assert not out[at:at + lq].any(), i
+        else:
+            near(out[at:at + lq], q[at:at + lq], ks[i], vs[i], range(lk - lq, lk), 50, 2, dtype)
+        at += lq
+    assert _lib.last_status() == 1
+
+
+def test_prefill_of_no_tokens_gives_zeros(cuda_device):
+    """A longest length of 0 over a padded tensor of rows: nobody's rows come back as zeros, not as what the memory held."""
+    dev = cuda_device
+    q = torch.full((40, 4, D), 7.0, dtype=torch.bfloat16, device=dev)
+    cu, ctx, table = (torch.zeros(*s, dtype=torch.int32, device=dev) for s in ((3,), (2,), (2, 4)))
+    kc, vc = torch.zeros(4, 2, 16, 16, 8, dtype=q.dtype, device=dev), torch.zeros(4, 2, D, 16, dtype=q.dtype, device=dev)
+    for _ in range(3):
+        junk = torch.full_like(q, 7.0)
+        del junk
+        assert not tch_cuda.flash_attn_varlen_window(q, q[:, :2], q[:, :2], cu, cu, 0, 0, SCALE, 9).any()
+        assert not tch_cuda.flash_attn_varlen_paged_window(q, kc, vc, cu, ctx, table, 0, 0, SCALE, 9).any()
+    assert _lib.last_status() == 0
