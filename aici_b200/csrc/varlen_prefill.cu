@@ -174,18 +174,22 @@ struct WindowTiles {
 // the others, and real ones behind them: one prompt of 4096 and 63 of 20 tokens, 8/2 heads, window 512: 114
 // and 37 us; 4 prompts of 64 to 512, 32 heads, window 128: 15.1 and 13.4 us; 200 of 1 to 400, 8/2 heads: 135
 // and 139 us.  Where all sequences are as long as the longest the finding alone would cost 0.4 us a CTA.)
-// Sequences and their tiles are counted from the last.  All lanes of a warp take part.
+// Sequences and their tiles are counted from the last.  All lanes of a warp take part.  (Clamped sums: with them
+// no more tiles exist than the grid has places, whatever they hold.)
 struct BatchTile {
   int b, mb;  // sequence (-1: no tile) and row tile
   int q0, lq, k0, lk;
 };
+// A running sum of query lengths: rows outside the query tensor are nobody's.
+__device__ __forceinline__ int row_sum(const PrefillParams &p, int i) { return min(max(p.cu_q[i], 0), p.total_q); }
+
 template <bool kPaged>
 __device__ __forceinline__ BatchTile batch_tile(const PrefillParams &p, int idx, int lane) {
   BatchTile t = {-1, 0, 0, 0, 0, 0};
   if (p.batch <= 32) {
     // a sequence to a lane
     const int i = min(lane, p.batch - 1);
-    const int q0 = p.cu_q[i], q1 = p.cu_q[i + 1];
+    const int q0 = row_sum(p, i), q1 = row_sum(p, i + 1);
     const int k0 = kPaged ? 0 : p.cu_k[i], k1 = kPaged ? p.k_lens[i] : p.cu_k[i + 1];
     const int n = lane < p.batch && q1 - q0 > p.longer_than ? (q1 - q0 + kBM - 1) / kBM : 0;
     int upto = n;
@@ -206,8 +210,8 @@ __device__ __forceinline__ BatchTile batch_tile(const PrefillParams &p, int idx,
   }
   // Many sequences: tiles are numbered as if sequence i began at cu[i] / 128 + i, which leaves room for all
   // of its tiles, and the sequence is found by a search with 32 probes a round.
-  const int origin = p.cu_q[0];
-  auto start = [&](int i) { return (p.cu_q[i] - origin) / kBM + i; };
+  const int origin = row_sum(p, 0);
+  auto start = [&](int i) { return (row_sum(p, i) - origin) / kBM + i; };
   idx = start(p.batch) - 1 - idx;
   if (idx < 0) return t;
   int lo = 0;
@@ -218,8 +222,8 @@ __device__ __forceinline__ BatchTile batch_tile(const PrefillParams &p, int idx,
     n = min(step, n - skip);
   }
   t.mb = idx - start(lo);
-  t.q0 = p.cu_q[lo];
-  t.lq = p.cu_q[lo + 1] - t.q0;
+  t.q0 = row_sum(p, lo);
+  t.lq = row_sum(p, lo + 1) - t.q0;
   if (t.lq <= p.longer_than || t.mb < 0 || t.mb >= (t.lq + kBM - 1) / kBM) return t;
   t.b = lo;
   t.k0 = kPaged ? 0 : p.cu_k[lo];
@@ -278,8 +282,11 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // BatchTile.)
   // Beside a launch for the short sequences (longer_than > 0) this grid starts while that one runs, which
   // began only when everything before it had ended; CTA 0 leaves after it, so that this grid ends last.
+  // CTA 0 also reports running sums that leave the query tensor (windowed: row_sum).
   auto leave = [&]() {
-    if (kWindow && p.longer_than > 0 && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!kWindow || blockIdx.x + blockIdx.y + blockIdx.z != 0) return;
+    if (tid == 0 && (p.cu_q[0] < 0 || p.cu_q[p.batch] > p.total_q)) set_status(p.status, AICI_STATUS_BAD_BLOCK);
+    if (p.longer_than > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
   if (kWindow && p.longer_than == 0) dependent_start();
   int b, q0, lq, k0 = 0, lk = 0, win_mb = 0, win_head = 0;
@@ -292,7 +299,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
   } else {
     b = blockIdx.y;
     win_head = (int)blockIdx.x;
-    q0 = p.cu_q[b], lq = p.cu_q[b + 1] - q0;
+    if (kWindow) q0 = row_sum(p, b), lq = row_sum(p, b + 1) - q0;
+    else q0 = p.cu_q[b], lq = p.cu_q[b + 1] - q0;
     if (kPaged) {
       lk = p.k_lens[b];
     } else {

@@ -314,8 +314,10 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   const int ctx = p.context_lens[seq];
   int q0 = seq, rows = p.group, tokens = 1, back = 0, all_tokens = 1;
   if (kChunk) {
-    q0 = min(max(p.cu_q[seq], 0), p.total_q);
-    all_tokens = min(max(p.cu_q[seq + 1], q0), p.total_q) - q0;
+    const int from = p.cu_q[seq], upto = p.cu_q[seq + 1];  // rows outside the query tensor are nobody's
+    q0 = min(max(from, 0), p.total_q);
+    all_tokens = min(max(upto, q0), p.total_q) - q0;
+    if ((from < 0 || upto > p.total_q) && threadIdx.x == 0) set_status(p.status, AICI_STATUS_BAD_BLOCK);
     if (all_tokens > p.max_tokens) {
       if (p.refuse) {
         if (threadIdx.x == 0) set_status(p.status, AICI_STATUS_BAD_BLOCK);

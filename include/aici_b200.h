@@ -517,7 +517,8 @@ char *aici_paged_attention_window(void *out, const void *query, const void *key_
  * of at most 16 tokens are worked on beside the others in a second launch.  Tokens that none of the 128 rows of a query tile (rows
  * 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token that one of
  * them sees are not read.  The rows of a sequence with more than max_seqlen_q tokens are zero and the status
- * says AICI_STATUS_BAD_BLOCK; max_seqlen_q = 0 says that there are no query tokens, and nothing is written. */
+ * says AICI_STATUS_BAD_BLOCK, as it does for running sums outside 0 .. total_q, whose rows outside the tensor are
+ * left out; max_seqlen_q = 0 says that there are no query tokens, and nothing is written. */
 char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
                                  const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
                                  int total_q, int total_k, int num_heads, int num_heads_k, int head_size,

@@ -634,3 +634,36 @@ def test_prefill_of_no_tokens_gives_zeros(cuda_device):
         assert not tch_cuda.flash_attn_varlen_window(q, q[:, :2], q[:, :2], cu, cu, 0, 0, SCALE, 9).any()
         assert not tch_cuda.flash_attn_varlen_paged_window(q, kc, vc, cu, ctx, table, 0, 0, SCALE, 9).any()
     assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("ends", ["behind", "before", "both"])
+@pytest.mark.parametrize("is_paged,lens_q,H,Hk", [
+    (False, [40, 90], 4, 2), (False, [140] + [3] * 12 + [90], 4, 2), (False, [140] + [3] * 45 + [90], 2, 2), (True, [3, 12], 4, 2),
+    (True, [40, 90], 32, 32), (True, [1] * 20 + [300, 90], 16, 4)])
+def test_prefill_rows_outside_the_query_tensor_are_not_touched(cuda_device, is_paged, lens_q, H, Hk, ends):
+    """Running sums that begin before the tensor's first row or end behind its last: the buffer around the
+    output stays, the status says so, and the sequences inside are right."""
+    dev, dtype, around = cuda_device, torch.bfloat16, 200
+    g = torch.Generator().manual_seed(sum(lens_q) + H)
+    lens_k = [lq + 11 for lq in lens_q]
+    cut0, cut1 = (0 if ends == "behind" else 2), (0 if ends == "before" else 5)
+    if cut0:
+        lens_q, lens_k = [30] + lens_q, [41] + lens_k
+    cu = [sum(lens_q[:i]) - cut0 for i in range(len(lens_q) + 1)]
+    total = cu[-1] - cut1
+    q = normal(g, dtype, around + total + around, H, D)
+    if is_paged:
+        kc, vc, table, ks, vs = paged(g, lens_k, Hk, dtype)
+        kv, table = (kc.to(dev), vc.to(dev)), table.to(dev)
+    else:
+        ks, vs = ([normal(g, dtype, n, Hk, D) for n in lens_k] for _ in range(2))
+        kv, table = (torch.cat(ks).to(dev), torch.cat(vs).to(dev)), None
+    out, qd = torch.full_like(q, 7.0).to(dev), q.to(dev)
+    into(out[around:], dev, qd[around:], kv, lens_q, lens_k, max(lens_q), 50, 2, table, total=total, cu_q=cu)
+    out = out.cpu()
+    assert (out[:around] == 7).all() and (out[around + total:] == 7).all()
+    out, q = out[around:around + total], q[around:around + total]
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        if cu[i] >= 0 and cu[i + 1] <= total:
+            near(out[cu[i]:cu[i + 1]], q[cu[i]:cu[i + 1]], ks[i], vs[i], range(lk - lq, lk), 50, 2, dtype)
+    assert _lib.last_status() == 1
