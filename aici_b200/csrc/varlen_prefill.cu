@@ -1486,6 +1486,7 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   AICI_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", fn);
   AICI_CHECK(batch <= 65535 && num_heads <= 65535, "%s: batch and num_heads must fit a grid dimension", fn);
   if (total_q == 0 || max_seqlen_q == 0) return nullptr;
+  if (win != nullptr && max_seqlen_q > total_q) max_seqlen_q = total_q;  // any bound will do
   AICI_CHECK(out && q && cu_seqlens_q && cu_seqlens_k, "%s: NULL pointer", fn);
   AICI_CHECK(total_k == 0 || (k && v), "%s: NULL pointer", fn);
   AICI_CHECK(((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0,
@@ -1642,6 +1643,7 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   AICI_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", fn);
   AICI_CHECK(batch <= 65535 && num_heads <= 65535, "%s: batch and num_heads must fit a grid dimension", fn);
   if (total_q == 0 || max_seqlen_q == 0) return nullptr;
+  if (win != nullptr && max_seqlen_q > total_q) max_seqlen_q = total_q;  // any bound will do
   AICI_CHECK(out && q && key_cache && value_cache && cu_seqlens_q && context_lens && block_tables,
              "%s: NULL pointer", fn);
   AICI_CHECK(num_blocks > 0, "%s: num_blocks must be positive", fn);

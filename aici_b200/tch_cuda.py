@@ -823,7 +823,8 @@ def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key
 
 # ---- attention with a sliding window and sinks ----------------------------------------------------------
 def _int32(x: int) -> int:
-    """A window or sink count as the C ABI takes it: what is longer than any sequence means the same."""
+    """A window, a sink count or a stated longest length as the C ABI takes it: what is longer than any sequence
+    means the same."""
     return min(max(int(x), -1), 0x7fffffff)
 
 
@@ -860,8 +861,8 @@ def paged_attention_window(out: torch.Tensor, query: torch.Tensor, key_cache: to
     _check_table(fn, block_tables, context_lens, num_seqs)
     _call(fn, "aici_paged_attention_window", index, out.data_ptr(), query.data_ptr(), key_cache.data_ptr(),
           value_cache.data_ptr(), int(num_kv_heads), scale, block_tables.data_ptr(), context_lens.data_ptr(),
-          int(block_size), int(max_context_len), _int32(window), _int32(sinks), num_seqs, num_heads, head_size, block_tables.shape[1],
-          num_blocks, stride[0], key_cache.stride(0), key_cache.stride(1), _dtype(fn, query))
+          int(block_size), _int32(max_context_len), _int32(window), _int32(sinks), num_seqs, num_heads, head_size,
+          block_tables.shape[1], num_blocks, stride[0], key_cache.stride(0), key_cache.stride(1), _dtype(fn, query))
 
 
 def _check_prefill(fn, q, seqlens_q):
@@ -893,12 +894,12 @@ def flash_attn_varlen_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         raise AiciError("%s: query, key and value must have the same dtype" % fn)
     if seqlens_k.dtype is not torch.int32 or not seqlens_k.is_contiguous() or seqlens_k.numel() != batch + 1:
         raise AiciError("%s: seqlens_k must be contiguous int32 and as long as seqlens_q" % fn)
-    max_seqlen_q = int(max_seqlen_q)
+    max_seqlen_q = _int32(max_seqlen_q)
     out = q.new_empty(q.shape) if max_seqlen_q else q.new_zeros(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_window_fwd", index, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
           seqlens_q.data_ptr(), seqlens_k.data_ptr(), batch, total_q, k.shape[0], num_heads, k.shape[1], head_size,
-          max_seqlen_q, int(max_seqlen_k), _int32(window), _int32(sinks), q_tok, q_head, ks[0], ks[1], vs[0], vs[1],
+          max_seqlen_q, _int32(max_seqlen_k), _int32(window), _int32(sinks), q_tok, q_head, ks[0], ks[1], vs[0], vs[1],
           num_heads * head_size, head_size, softmax_scale, _dtype(fn, q))
     return out
 
@@ -920,12 +921,12 @@ def flash_attn_varlen_paged_window(q: torch.Tensor, key_cache: torch.Tensor, val
     if q.dtype is not key_cache.dtype or q.dtype is not value_cache.dtype:
         raise AiciError("%s: query and cache dtypes differ" % fn)
     _check_table(fn, block_tables, context_lens, batch)
-    max_seqlen_q = int(max_seqlen_q)
+    max_seqlen_q = _int32(max_seqlen_q)
     out = q.new_empty(q.shape) if max_seqlen_q else q.new_zeros(q.shape)
     q_tok, q_head, _ = q.stride()
     _call(fn, "aici_mha_varlen_paged_window_fwd", index, out.data_ptr(), q.data_ptr(), key_cache.data_ptr(),
           value_cache.data_ptr(), seqlens_q.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), batch,
-          total_q, num_heads, num_kv_heads, head_size, block_size, max_seqlen_q, int(max_context_len),
+          total_q, num_heads, num_kv_heads, head_size, block_size, max_seqlen_q, _int32(max_context_len),
           block_tables.shape[1], num_blocks, _int32(window), _int32(sinks), q_tok, q_head, num_heads * head_size,
           head_size, key_cache.stride(0), key_cache.stride(1), softmax_scale, _dtype(fn, q))
     return out

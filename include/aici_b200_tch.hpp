@@ -648,6 +648,8 @@ inline void paged_attention_window(Tensor &out, const Tensor &query, const Tenso
 }
 
 namespace detail {
+// A stated longest length as the C ABI takes it: what is longer than any sequence means the same.
+inline int at_most_int(size_t x) { return x < 0x7fffffff ? (int)x : 0x7fffffff; }
 // What a windowed prefill returns: zeros where the call says that there are no query tokens.
 inline Tensor rows_like(const char *fn, const Tensor &q, int dev, size_t max_seqlen_q, cudaStream_t stream) {
   Tensor out = Tensor::empty(q.sizes, q.kind, dev);
@@ -678,8 +680,8 @@ inline Tensor flash_attn_varlen_window(const Tensor &q, const Tensor &k, const T
   check(fn, aici_mha_varlen_window_fwd(
                 out.data, q.data, k.data, v.data, static_cast<const int32_t *>(seqlens_q.data),
                 static_cast<const int32_t *>(seqlens_k.data), (int)seqlens_q.numel() - 1, (int)q.size(0), (int)k.size(0),
-                (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)max_seqlen_q, (int)max_seqlen_k, window, sinks,
-                q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                (int)q.size(1), (int)k.size(1), (int)q.size(2), detail::at_most_int(max_seqlen_q),
+                detail::at_most_int(max_seqlen_k), window, sinks, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
                 out.stride(1), softmax_scale, detail::dtype_of(fn, q), stream));
   return out;
 }
@@ -708,9 +710,9 @@ inline Tensor flash_attn_varlen_paged_window(const Tensor &q, const Tensor &key_
   check(fn, aici_mha_varlen_paged_window_fwd(
                 out.data, q.data, key_cache.data, value_cache.data, static_cast<const int32_t *>(seqlens_q.data),
                 static_cast<const int32_t *>(context_lens.data), static_cast<const int32_t *>(block_tables.data), batch,
-                (int)q.size(0), (int)q.size(1), c.num_kv_heads, c.head_size, c.block_size, (int)max_seqlen_q,
-                (int)max_context_len, (int)block_tables.size(1), c.num_blocks, window, sinks, q.stride(0), q.stride(1),
-                out.stride(0), out.stride(1), key_cache.stride(0), key_cache.stride(1), softmax_scale,
+                (int)q.size(0), (int)q.size(1), c.num_kv_heads, c.head_size, c.block_size, detail::at_most_int(max_seqlen_q),
+                detail::at_most_int(max_context_len), (int)block_tables.size(1), c.num_blocks, window, sinks, q.stride(0),
+                q.stride(1), out.stride(0), out.stride(1), key_cache.stride(0), key_cache.stride(1), softmax_scale,
                 detail::dtype_of(fn, q), stream));
   return out;
 }

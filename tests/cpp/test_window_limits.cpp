@@ -70,6 +70,10 @@ static void stated_lengths(const Batch &b) {
     auto call = [&](size_t max_q, size_t max_k) { return form == 0 ? b.packed(max_q, max_k) : b.paged(max_q, max_k); };
     std::vector<uint16_t> o = call(40, 40);
     expect(rows_are(o, 0, 40, kOne) && rows_are(o, 40, 50, kTwo) && t::last_status() == 0, "lengths as they are");
+    for (size_t most : {(size_t)1 << 31, (size_t)1 << 32, ((size_t)1 << 32) + 5}) {
+      o = call(most, most);
+      expect(rows_are(o, 0, 40, kOne) && rows_are(o, 40, 50, kTwo) && t::last_status() == 0, "lengths beyond 32 bits");
+    }
     o = call(12, 40);
     expect(rows_are(o, 0, 40, 0) && rows_are(o, 40, 50, kTwo), "a sequence longer than stated");
     expect(t::last_status() == AICI_STATUS_BAD_BLOCK, "its status");

@@ -667,3 +667,25 @@ def test_prefill_rows_outside_the_query_tensor_are_not_touched(cuda_device, is_p
         if cu[i] >= 0 and cu[i + 1] <= total:
             near(out[cu[i]:cu[i + 1]], q[cu[i]:cu[i + 1]], ks[i], vs[i], range(lk - lq, lk), 50, 2, dtype)
     assert _lib.last_status() == 1
+
+
+@pytest.mark.parametrize("most", [1 << 31, 1 << 32, (1 << 32) + 5, 1 << 40])
+def test_longest_lengths_beyond_32_bits(cuda_device, most):
+    """A stated longest length may be any bound."""
+    dev, dtype = cuda_device, torch.bfloat16
+    g = torch.Generator().manual_seed(17)
+    lens = [70, 200, 16]
+    kc, vc, table, ks, vs = paged(g, lens, 2, dtype)
+    q = normal(g, dtype, 286, 4, D)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cu, ctx, qd, k, v = i32([0, 70, 270, 286]), i32(lens), q.to(dev), torch.cat(ks).to(dev), torch.cat(vs).to(dev)
+    outs = [tch_cuda.flash_attn_varlen_window(qd, k, v, cu, cu, most, most, SCALE, 30, 2).cpu(),
+            tch_cuda.flash_attn_varlen_paged_window(qd, kc.to(dev), vc.to(dev), cu, ctx, table.to(dev), most, most, SCALE, 30, 2).cpu()]
+    for i, (a, b) in enumerate(((0, 70), (70, 270), (270, 286))):
+        for out in outs:
+            near(out[a:b], q[a:b], ks[i], vs[i], range(b - a), 30, 2, dtype)
+    out = torch.empty(3, 4, D, dtype=dtype, device=dev)
+    tch_cuda.paged_attention_window(out, qd[:3], kc.to(dev), vc.to(dev), 2, SCALE, table.to(dev), ctx, 16, most, 30, 2)
+    for i, n in enumerate(lens):
+        near(out.cpu()[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 30, 2, dtype)
+    assert _lib.last_status() == 0
