@@ -395,6 +395,10 @@ static char *launch_rotary(RotaryParams p, bool cache, cudaStream_t stream) {
 
 static char *rotary_impl(const char *fn, RotaryParams p, int is_neox, int table_dtype, int dtype, bool cache,
                          aici_stream_t stream) {
+  if (p.num_tokens <= 1) {  // the stride of a single token is never used and may be whatever a layout left there
+    p.query_stride = (int64_t)p.num_heads * p.head_size;
+    p.key_stride = p.value_stride = (int64_t)p.num_kv_heads * p.head_size;
+  }
   if (char *e = check_rotary(fn, p, table_dtype, dtype, cache)) return e;
   if (p.num_tokens == 0) return nullptr;
   if (char *e = check_on_current_device(fn, "query", p.query)) return e;

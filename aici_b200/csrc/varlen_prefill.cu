@@ -1491,6 +1491,12 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   AICI_CHECK(total_k == 0 || (k && v), "%s: NULL pointer", fn);
   AICI_CHECK(((uintptr_t)out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0,
              "%s: tensors must be 16-byte aligned", fn);
+  if (win != nullptr) {  // a stride over a dimension of one is never used and may be whatever a layout left there
+    if (total_q == 1) q_tok_stride = kHD;
+    if (num_heads == 1) q_head_stride = kHD;
+    if (total_k == 1) k_tok_stride = v_tok_stride = kHD;
+    if (num_heads_k == 1) k_head_stride = v_head_stride = kHD;
+  }
   const int64_t strides[8] = {q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
                               v_tok_stride, v_head_stride, o_tok_stride, o_head_stride};
   for (int i = 0; i < 8; ++i)
@@ -1649,6 +1655,8 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   AICI_CHECK(num_blocks > 0, "%s: num_blocks must be positive", fn);
   AICI_CHECK(((uintptr_t)out | (uintptr_t)q | (uintptr_t)key_cache | (uintptr_t)value_cache) % 16 == 0,
              "%s: tensors must be 16-byte aligned", fn);
+  if (win != nullptr && total_q == 1) q_tok_stride = kHD;  // never used
+  if (win != nullptr && num_heads == 1) q_head_stride = kHD;
   const int64_t strides[4] = {q_tok_stride, q_head_stride, o_tok_stride, o_head_stride};
   for (int i = 0; i < 4; ++i)
     AICI_CHECK(strides[i] >= kHD && strides[i] % 8 == 0,

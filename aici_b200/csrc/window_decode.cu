@@ -554,6 +554,7 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
   AICI_CHECK(num_seqs >= 0 && max_context_len >= 0 && max_num_blocks_per_seq >= 0, "%s: negative size", fn);
   AICI_CHECK((int64_t)num_seqs * num_heads < (1ll << 31), "%s: too many sequences and heads for one call", fn);
   AICI_CHECK(num_blocks > 0, "%s: num_blocks must be positive", fn);
+  if (num_seqs <= 1) q_stride = (int64_t)num_heads * head_size;  // never used
   AICI_CHECK(q_stride % 8 == 0 && q_stride >= (int64_t)num_heads * head_size,
              "%s: q_stride must be a multiple of 8 elements and cover one row", fn);
   AICI_CHECK(kv_head_stride == kWinHead * kWinBlock && kv_block_stride % 8 == 0 &&

@@ -470,7 +470,7 @@ char *aici_rotary_cos_sin_cache(void *out, int64_t max_position, int rot_dim, do
 
 /* Replaces rotary_embedding_C (lib.rs:139-146; kernels/vllm/pos_encoding_kernels.cu:40-128) in its
  * general form: query [num_tokens, num_heads, head_size] and key [num_tokens, num_kv_heads, head_size]
- * (token strides in elements, multiples of 8) are turned in place, is_neox != 0: element j with
+ * (token strides in elements, multiples of 8; any for a single token) are turned in place, is_neox != 0: element j with
  * j + rot_dim / 2, else 2 j with 2 j + 1; elements from rot_dim on stay.  bf16 or f16; cos_sin_cache
  * [max_position, rot_dim] of f32 (table_dtype AICI_DTYPE_F32) or the query's type.  head_size and
  * rot_dim are multiples of 16 up to 256.  Arithmetic in fp32, rounded once (the reference rounds every
@@ -497,7 +497,7 @@ char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, voi
  * (window >= 1, sinks >= 0; a window that covers the context gives causal attention).  bf16 or f16,
  * head_size 128, block_size 16; fp32 scores and sums.  Probabilities meet the values in the 16-bit type:
  * prefill rounds them, decode and short paged chunks add what the rounding left as a second product.  A
- * row that sees nothing is zero.
+ * row that sees nothing is zero.  The strides of a single query row, key row or head may be anything.
  *
  * Decode over the paged cache, arguments as in aici_paged_attention_v1: one query per sequence at
  * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number.  Blocks that hold no

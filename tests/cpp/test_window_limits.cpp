@@ -1,5 +1,5 @@
 // Calls at the limits of what the windowed operators' C++ host side (include/aici_b200_tch.hpp) is told:
-// stated lengths that do not cover the sequences.  Exit code = number of failures.
+// stated lengths that do not cover the sequences, strides of a single row.  Exit code = number of failures.
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -82,11 +82,40 @@ static void stated_lengths(const Batch &b) {
   }
 }
 
+// One query token of one sequence, its first stride left from another layout.
+static void single_rows(const Batch &b) {
+  std::vector<int32_t> one = {0, 1}, len = {10};
+  Tensor cu = up(one, {2}, Kind::Int), ctx = up(len, {1}, Kind::Int), bt = up(std::vector<int32_t>{3}, {1, 1}, Kind::Int);
+  for (int64_t stride : {1, 128, 1001}) {
+    Tensor q = Tensor::view(b.q.data, {1, H, D}, Kind::BFloat16, 0, {stride, D, 1});
+    Tensor v = Tensor::view(b.v.data, {1, H, D}, Kind::BFloat16, 0, {stride, D, 1});
+    Tensor o = Tensor::empty({1, H, D}, Kind::BFloat16, 0);
+    t::paged_attention_window(o, q, b.kc, b.vc, H, 0.01f, bt, ctx, 16, 10, 4);
+    expect(rows_are(down(o), 0, 1, kTwo), "decode of a single row");
+    expect(rows_are(down(t::flash_attn_varlen_paged_window(q, b.kc, b.vc, cu, ctx, bt, 1, 10, 0.01f, 4)), 0, 1, kTwo), "paged");
+    expect(rows_are(down(t::flash_attn_varlen_window(q, q, v, cu, cu, 1, 1, 0.01f, 4)), 0, 1, kOne), "packed");
+    Tensor table = t::rotary_cos_sin_cache(4, D, 10000.0, Kind::Float, 0);
+    Tensor pos = up(std::vector<int64_t>{0}, {1}, Kind::Int64), slot = up(std::vector<int64_t>{5}, {1}, Kind::Int64);
+    const std::vector<uint16_t> twos(H * D, kTwo);
+    Tensor q1 = up(twos, {1, H, D}, Kind::BFloat16), k1 = up(twos, {1, H, D}, Kind::BFloat16);
+    Tensor kc = Tensor::empty({1, H, D / 8, 16, 8}, Kind::BFloat16, 0), vc = Tensor::empty({1, H, D, 16}, Kind::BFloat16, 0);
+    q1.strides[0] = k1.strides[0] = stride;
+    t::rotary_embedding(pos, q1, k1, D, table, true);
+    t::rotary_embedding_and_cache(pos, q1, k1, v, D, table, true, kc, vc, slot);  // position 0 turns nothing
+    expect(rows_are(down(q1), 0, 1, kTwo) && rows_are(down(k1), 0, 1, kTwo), "rotation of a single token");
+    std::vector<uint16_t> keys = down(kc), values = down(vc);
+    for (int e = 0; e < H * D; ++e)
+      expect(keys[e / 8 * 128 + 5 * 8 + e % 8] == kTwo && values[e * 16 + 5] == kOne, "cache write of a single token");
+  }
+  expect(t::last_status() == 0, "status");
+}
+
 int main() {
   t::cuda_check("cudaSetDevice", cudaSetDevice(0));
   try {
     Batch b;
     stated_lengths(b);
+    single_rows(b);
   } catch (const std::exception &e) {
     std::printf("[ FAIL ] exception: %s\n", e.what());
     ++fails;

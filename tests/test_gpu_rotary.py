@@ -147,3 +147,24 @@ def test_refuses_mismatched_tensors(cuda_device):
         args[i] = bad
         with pytest.raises(_lib.AiciError, match=match):
             tch_cuda.rotary_embedding_and_cache(*args)
+
+
+@pytest.mark.parametrize("stride", [1, 128, 1001])
+def test_a_single_token_has_no_stride(cuda_device, stride):
+    """One token whose first stride is what is left of another layout."""
+    dev, H, Hk, D, dtype = cuda_device, 4, 2, 128, torch.bfloat16
+    wide, cs, pos, slots, kc, vc = inputs(8, 1, H, Hk, D, 128, dtype, torch.float32)
+    x = wide.to(dev)
+    odd = lambda lo, n: x.flatten()[lo * D:].as_strided((1, n * D), (stride, 1))  # noqa: E731
+    q, k, v = odd(0, H), odd(H, Hk), odd(H + Hk, Hk)
+    assert q.is_contiguous() and q.stride(0) == stride
+    alone = x.clone()
+    kc_d, vc_d = kc.to(dev), vc.to(dev)
+    tch_cuda.rotary_embedding_and_cache(pos.to(dev), q, k, v, D, cs.to(dev), True, kc_d, vc_d, slots.to(dev))
+    close(x[:, :H * D].reshape(1, H, D), *W.rotate(wide[:, :H * D].view(1, H, D), cs[pos], True), dtype)
+    W.write_cache(x[:, H * D:(H + Hk) * D].reshape(1, Hk, D).cpu(), wide[:, (H + Hk) * D:].reshape(1, Hk, D), kc, vc, slots)
+    assert torch.equal(kc_d.cpu(), kc) and torch.equal(vc_d.cpu(), vc)
+    flat = alone.flatten()
+    tch_cuda.rotary_embedding(pos.to(dev), flat.as_strided((1, H, D), (stride, D, 1)),
+                              flat[H * D:].as_strided((1, Hk, D), (stride, D, 1)), D, cs.to(dev), True)
+    assert torch.equal(alone, x) and _lib.last_status() == 0

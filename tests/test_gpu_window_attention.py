@@ -689,3 +689,24 @@ def test_longest_lengths_beyond_32_bits(cuda_device, most):
     for i, n in enumerate(lens):
         near(out.cpu()[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 30, 2, dtype)
     assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("stride", [1, 128, 1001])
+def test_a_single_row_has_no_stride(cuda_device, stride):
+    """One query token (or one key) whose first stride is what is left of another layout."""
+    dev, dtype, H, Hk = cuda_device, torch.float16, 6, 2
+    g = torch.Generator().manual_seed(18)
+    kc, vc, table, ks, vs = paged(g, [50], Hk, dtype)
+    q, k1, v1 = normal(g, dtype, 1, H, D), ks[0][-1:], vs[0][-1:]
+    odd = lambda x: x.to(dev).as_strided(x.shape, (stride, D, 1))  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    assert odd(q).is_contiguous() and odd(q).stride(0) == stride
+    out = torch.empty(1, H, D, dtype=dtype, device=dev)
+    tch_cuda.paged_attention_window(out, odd(q), kc.to(dev), vc.to(dev), Hk, SCALE, table.to(dev), i32([50]), 16, 50, 20, 2)
+    near(out.cpu(), q, ks[0], vs[0], [49], 20, 2, dtype)
+    out = tch_cuda.flash_attn_varlen_paged_window(odd(q), kc.to(dev), vc.to(dev), i32([0, 1]), i32([50]), table.to(dev), 1, 50,
+                                                  SCALE, 20, 2).cpu()
+    near(out, q, ks[0], vs[0], [49], 20, 2, dtype)
+    out = tch_cuda.flash_attn_varlen_window(odd(q), odd(k1), odd(v1), i32([0, 1]), i32([0, 1]), 1, 1, SCALE, 20, 2).cpu()
+    near(out, q, k1, v1, [0], 20, 2, dtype)
+    assert _lib.last_status() == 0
