@@ -199,8 +199,8 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
     tensors (at least the number of new tokens; a captured step takes its largest).  With `out` the
     tensors of an earlier result are written again; out.context_lens may be `context_lens` and
     out.free_count may be `free_count`, which advances the state in place.  A step that does not fit
-    (lengths, tokens, free blocks) changes nothing and sets a status bit (see _lib.last_status).
-    Returns a StepTables."""
+    (lengths, tokens, free blocks) changes nothing and sets a status bit (see _lib.last_status).  Tokens of a
+    block whose id is outside the pool get slot -1, and the bit is set too.  Returns a StepTables."""
     fn = "step_tables"
     given = (query_lens, context_lens, block_tables, free_blocks, free_count)
     index, int32 = _one_gpu(fn, given), torch.int32

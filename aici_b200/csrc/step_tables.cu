@@ -151,7 +151,9 @@ __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(const StepPar
     set_status(p.status, AICI_STATUS_BAD_BLOCK);
     return -1;
   };
-  auto enter = [&](int req, int at, int id) {  // a token that begins a block enters it in the table
+  // a token that begins a block enters it in the table, a bad id too: what the entry held before may be a block
+  // of another request by now
+  auto enter = [&](int req, int at, int id) {
     if (at % kBlockTokens == 0) p.block_tables[req * p.table_stride + at / kBlockTokens] = id;
   };
   for (int64_t t64 = (int64_t)kStepBatch * gid; t64 < p.max_tokens; t64 += (int64_t)kStepBatch * threads) {

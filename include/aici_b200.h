@@ -447,7 +447,9 @@ char *aici_batch_info_build(const aici_batch_entry *entries, int num_entries, in
  * more than max_tokens new tokens (AICI_STATUS_BAD_BLOCK), or free_count is below what the step needs
  * (AICI_STATUS_NO_BLOCKS), the status bit is set and the outputs are those of a step without new
  * tokens; tables, lengths and count keep their values.  A block id outside [0, num_blocks) gives slot
- * -1 and AICI_STATUS_BAD_BLOCK.  At most 16384 requests; positions and slot_mapping 16-byte aligned. */
+ * -1 and AICI_STATUS_BAD_BLOCK; one from the free list is entered in the table all the same, so that later
+ * tokens of the block meet it again and not the block that the entry named before.  At most 16384
+ * requests; positions and slot_mapping 16-byte aligned. */
 char *aici_step_tables(const int32_t *query_lens, const int32_t *context_lens, int32_t *block_tables,
                        const int32_t *free_blocks, const int32_t *free_count, int num_requests,
                        int max_blocks_per_seq, int64_t block_table_stride, int free_capacity,

@@ -164,3 +164,18 @@ def test_refuses_out_of_another_shape(cuda_device):
     for tokens in (-1, 1 << 30, 1 << 32):
         with pytest.raises(_lib.AiciError, match="max_tokens"):
             call(cuda_device, *args[:5], tokens, args[6])
+
+
+def test_a_bad_id_of_the_free_list_stays_bad(cuda_device):
+    """A block id outside the pool that the free list hands out is entered in the table: later tokens of that block
+    meet it again, and none of them is written to the block that the entry named before."""
+    dev = cuda_device
+    args = [[3, 2], [16, 4], [[1, 6], [2, 6]], [5, 777], 2, 8, 10]
+    res, bt = call(dev, *args)
+    want = W.step_tables(*args)
+    check(res, bt, want)
+    assert bt.tolist()[0] == [1, 777] and res.slot_mapping[:3].tolist() == [-1] * 3 and _lib.last_status() == 1
+    args = [[1, 0], want[4], want[6], [5, 777], want[5], 8, 10]
+    res, bt = call(dev, *args)
+    check(res, bt, W.step_tables(*args))
+    assert res.slot_mapping[0].item() == -1 and _lib.last_status() == 1
