@@ -728,7 +728,9 @@ def rotary_cos_sin_cache(max_position: int, rot_dim: int, base: float, dtype: to
     """Cosines and sines [max_position, rot_dim] = [cos | sin] for the rotary functions, the table that
     rLLM's RotaryEmbedding keeps (rllm-cuda/src/llm/mod.rs:62-129).  Pair j turns by base^(-2 j / rot_dim)
     per position; `scaling` stretches it by `factor` for longer contexts: "linear", "ntk", or "yarn" (by
-    wavelength, against `original_context`, the trained length).  dtype float32, bfloat16 or float16."""
+    wavelength, against `original_context`, the trained length: the paper's mix, linear in a pair's number of turns
+    between 1 and 32.  Checkpoints trained with another mix, such as linear in the pair's number, need a table made by
+    the caller, which the rotary functions take as well).  dtype float32, bfloat16 or float16."""
     fn = "rotary_cos_sin_cache"
     if scaling not in _SCALINGS:
         raise AiciError("%s: unknown scaling %r" % (fn, scaling))

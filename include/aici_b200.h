@@ -462,9 +462,14 @@ char *aici_step_tables(const int32_t *query_lens, const int32_t *context_lens, i
  * pair j turns by base^(-2 j / rot_dim) per position, scaled for contexts longer than the trained one:
  *   AICI_ROPE_LINEAR  positions divided by factor
  *   AICI_ROPE_NTK     base multiplied by factor^(rot_dim / (rot_dim - 2))
- *   AICI_ROPE_YARN    pairs with fewer than one turn in original_context positions are slowed down by
- *                     factor, those with more than 32 keep their speed, the ones between are mixed; cosine
- *                     and sine are multiplied by 0.1 ln(factor) + 1
+ *   AICI_ROPE_YARN    as the paper has it (Peng et al., "YaRN", 2023: NTK-by-parts, alpha 1, beta 32): pairs
+ *                     with fewer than one turn in original_context positions are slowed down by factor,
+ *                     those with more than 32 keep their speed, the ones between are mixed linearly in their
+ *                     number of turns; cosine and sine are multiplied by 0.1 ln(factor) + 1.  Released
+ *                     checkpoints are often trained with another mix, linear in the pair's number between
+ *                     the pairs that turn 32 times and once, or with other bounds: up to 2.3 times other
+ *                     speeds in between (base 500000, 16384 positions, factor 8).  Their table is the
+ *                     caller's to make; the rotary calls take any.
  * Angles are computed in 64 bits.  rot_dim even, at most 256; factor >= 1. */
 enum { AICI_ROPE_NONE = 0, AICI_ROPE_LINEAR = 1, AICI_ROPE_NTK = 2, AICI_ROPE_YARN = 3 };
 char *aici_rotary_cos_sin_cache(void *out, int64_t max_position, int rot_dim, double base, int scaling,

@@ -573,7 +573,8 @@ inline void rotary_args(const char *fn, const Tensor &positions, const Tensor &q
 }
 }  // namespace detail
 
-// Cosines and sines [max_position, rot_dim] of aici_rotary_cos_sin_cache; scaling is one of AICI_ROPE_*.
+// Cosines and sines [max_position, rot_dim] of aici_rotary_cos_sin_cache; scaling is one of AICI_ROPE_* (which
+// mix of speeds AICI_ROPE_YARN is: see there).
 inline Tensor rotary_cos_sin_cache(int64_t max_position, int rot_dim, double base, Kind kind, int device,
                                    int scaling = AICI_ROPE_NONE, double factor = 1.0, int64_t original_context = 0,
                                    cudaStream_t stream = cudaStreamPerThread) {

@@ -1,5 +1,7 @@
 """Rotary positions: the table, both pairings, part of the head, both 16-bit types, with and without the
 cache write, against the definition in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -168,3 +170,17 @@ def test_a_single_token_has_no_stride(cuda_device, stride):
     tch_cuda.rotary_embedding(pos.to(dev), flat.as_strided((1, H, D), (stride, D, 1)),
                               flat[H * D:].as_strided((1, Hk, D), (stride, D, 1)), D, cs.to(dev), True)
     assert torch.equal(alone, x) and _lib.last_status() == 0
+
+
+def test_yarn_mixes_by_turns(cuda_device):
+    """Angles per position from the paper's NTK-by-parts formula worked out in 40 decimal digits: base 500000, trained length
+    16384, factor 8.  (A mix linear in the pair's number, as some models are trained with, gives other angles between
+    the two ends: pair 30 turns by 1.199e-3 there.)"""
+    got = tch_cuda.rotary_cos_sin_cache(2, 128, 5e5, torch.float32, cuda_device, scaling="yarn", factor=8.0,
+                                        original_context=16384).cpu().double()
+    for j, angle in ((0, 1.0), (20, 1.656044008099e-02), (21, 1.349041989023e-02), (22, 9.952331774935e-03),
+                     (25, 3.172472539041e-03), (30, 5.405109533618e-04), (35, 1.170003683811e-04), (38, 5.256482028508e-05),
+                     (39, 4.208236768726e-05), (50, 4.411534674558e-06), (63, 3.068925988915e-07)):
+        # cosine and sine are off by half a step of f32 each: together by less than 2^-23 of the angle
+        assert abs(math.atan2(got[1, 64 + j], got[1, j]) - angle) <= 2.0 ** -23 * angle + 1e-12 * angle, j
+        assert abs(got[0, j] - (0.1 * math.log(8.0) + 1)) <= 2.0 ** -24 * 1.3
