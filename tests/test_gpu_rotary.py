@@ -184,3 +184,67 @@ def test_yarn_mixes_by_turns(cuda_device):
         # cosine and sine are off by half a step of f32 each: together by less than 2^-23 of the angle
         assert abs(math.atan2(got[1, 64 + j], got[1, j]) - angle) <= 2.0 ** -23 * angle + 1e-12 * angle, j
         assert abs(got[0, j] - (0.1 * math.log(8.0) + 1)) <= 2.0 ** -24 * 1.3
+
+
+def prompt_slots(g, T, nblk, start):
+    """Slots of one long sequence in shuffled blocks from token `start` of its first block on; a few tokens of it go
+    nowhere, and its last ones to single slots of other blocks."""
+    blocks = torch.randperm(nblk - 4, generator=g)
+    at = torch.arange(T) + start
+    slots = blocks[at // 16] * 16 + at % 16
+    slots[T - 5:] = (nblk - 4) * 16 + torch.randperm(64, generator=g)[:5]
+    slots[torch.randint(0, T, (7,), generator=g)] = -1
+    return slots
+
+
+LARGE = [  # heads, kv heads, head size, rotated part, neox, kv heads of a cache-writing CTA, dtype
+    (64, 8, 128, 64, False, 8, torch.float16), (10, 5, 128, 128, True, 4, torch.bfloat16), (7, 7, 256, 256, True, 2, torch.bfloat16),
+    (7, 7, 256, 16, False, 4, torch.float16), (6, 3, 256, 240, True, 8, torch.bfloat16), (32, 13, 64, 48, True, 8, torch.float16),
+    (40, 40, 96, 96, False, 8, torch.bfloat16), (100, 2, 16, 16, True, 2, torch.float16)]
+
+
+@pytest.mark.parametrize("H,Hk,D,rot,neox,per,dtype", LARGE)
+def test_many_tokens(cuda_device, H, Hk, D, rot, neox, per, dtype):
+    """Calls whose CTAs take several kv heads one after the other through their ring of stages, and whose threads
+    take four query heads and several runs of tokens."""
+    dev, g = cuda_device, torch.Generator().manual_seed(H * D + rot)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    tiles = -(-4 * per * sms // Hk)  # 8 x (per / 2) x SMs (tile, head) pairs give a CTA `per` heads
+    if H >= 32:
+        tiles = max(tiles, -(-4 * 4 * 256 * sms * 16 // (H * rot)) // 16 + 2)
+    T = tiles * 16 - 7
+    assert tiles * Hk >= 4 * per * sms and (per == 8 or tiles * Hk < 8 * per * sms or H >= 32)
+    assert H < 32 or T * H * (rot // 16) >= 4 * 4 * 256 * sms
+    wide = torch.randn(T, (H + 2 * Hk) * D, device=dev, generator=torch.Generator(dev).manual_seed(T)).to(dtype)
+    cs = W.cos_sin(range(700), rot, 1e4, "none", 1.0, 0).to(torch.float32).to(dev)
+    pos = torch.randint(0, 700, (T,), generator=g).to(dev)
+    nblk = T // 16 + 8
+    slots = prompt_slots(g, T, nblk, H % 16)
+    kc, vc = torch.full((nblk, Hk, D // 8, 16, 8), 7.0, dtype=dtype), torch.full((nblk, Hk, D, 16), 7.0, dtype=dtype)
+    cut = lambda x: (x[:, :H * D], x[:, H * D:(H + Hk) * D], x[:, (H + Hk) * D:])  # noqa: E731
+    alone, x, kc_d, vc_d = wide.clone(), wide.clone(), kc.to(dev), vc.to(dev)
+    tch_cuda.rotary_embedding_and_cache(pos, *cut(x), D, cs, neox, kc_d, vc_d, slots.to(dev))
+    tch_cuda.rotary_embedding(pos, *cut(alone)[:2], D, cs, neox)
+    assert torch.equal(x.view(torch.int16), alone.view(torch.int16))
+    for a in range(0, T, 1000):  # the definition, some tokens at a time
+        rows = slice(a, min(a + 1000, T))
+        for got, was, h in ((cut(x)[0], cut(wide)[0], H), (cut(x)[1], cut(wide)[1], Hk)):
+            want, mag = W.rotate(was[rows].reshape(-1, h, D), cs[pos[rows]], neox)
+            close(got[rows].reshape(-1, h, D), want.cpu(), mag.cpu(), dtype)
+    assert torch.equal(cut(x)[2], cut(wide)[2])
+    W.write_cache(cut(x)[1].reshape(T, Hk, D).cpu(), cut(wide)[2].reshape(T, Hk, D).cpu(), kc, vc, slots)
+    assert torch.equal(kc_d.cpu(), kc) and torch.equal(vc_d.cpu(), vc)
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("table", [torch.float32, torch.float16])
+@pytest.mark.parametrize("T,H,Hk,D,rot,neox", CASES)
+def test_alone_in_f16(cuda_device, T, H, Hk, D, rot, neox, table):
+    dev, dtype = cuda_device, torch.float16
+    wide, cs, pos, _, _, _ = inputs(T + 5 * D, T, H, Hk, D, rot, dtype, table)
+    x = wide.to(dev)
+    q, k = x[:, :H * D], x[:, H * D:(H + Hk) * D]
+    tch_cuda.rotary_embedding(pos.to(dev), q, k, D, cs.to(dev), neox)
+    close(q.reshape(T, H, D), *W.rotate(wide[:, :H * D].view(T, H, D), cs[pos], neox), dtype)
+    close(k.reshape(T, Hk, D), *W.rotate(wide[:, H * D:(H + Hk) * D].reshape(T, Hk, D), cs[pos], neox), dtype)
+    assert torch.equal(x[:, (H + Hk) * D:].cpu(), wide[:, (H + Hk) * D:]) and _lib.last_status() == 0
