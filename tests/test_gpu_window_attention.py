@@ -710,3 +710,82 @@ def test_a_single_row_has_no_stride(cuda_device, stride):
     out = tch_cuda.flash_attn_varlen_window(odd(q), odd(k1), odd(v1), i32([0, 1]), i32([0, 1]), 1, 1, SCALE, 20, 2).cpu()
     near(out, q, k1, v1, [0], 20, 2, dtype)
     assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("H", [20, 2], ids=["tiles", "items"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks,offset", [(100, 0, 0), (128, 4, 37), (300, 20, 128)])
+def test_paged_tiles_that_do_not_see_a_token_do_not_meet_it(cuda_device, window, sinks, offset, dtype, H):
+    """NaN in one token of the cache that some rows see: with 20 heads the call takes tiles of 128 rows, with 2 items
+    of 16, and those none of whose rows sees it stay right."""
+    dev, n, rows_each = cuda_device, 520, 128 if H == 20 else 16
+    assert (H * -(-n // 16) > 2 * 148) == (H == 20)
+    for bad in (0, 3, 19, 21, 130, 255, 256, 300, 511):
+        g = torch.Generator().manual_seed(bad)
+        kc, vc, table, ks, vs = paged(g, [n + offset], H, dtype)
+        q = normal(g, dtype, n, H, D)
+        kc[table[0, bad // 16], :, :, bad % 16] = NAN
+        vc[table[0, bad // 16], :, :, bad % 16] = NAN
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        out = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc.to(dev), vc.to(dev), i32([0, n]), i32([n + offset]),
+                                                      table.to(dev), n, n + offset, SCALE, window, sinks).cpu()
+        kept = 0
+        for r0 in range(0, n, rows_each):
+            rows = range(r0, min(r0 + rows_each, n))
+            if not any(bad in W.visible(offset + r, window, sinks) for r in rows):
+                some = [rows[0], rows[len(rows) // 2], rows[-1]]
+                near(out[some], q[some], ks[0], vs[0], [offset + r for r in some], window, sinks, dtype, split=H == 2)
+                kept += 1
+        assert kept >= (0 if bad < sinks else 1)
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(60, 0), (200, 3), (1000, 0)])
+def test_paged_tiles_uneven_scores(cuda_device, dtype, window, sinks):
+    """Keys of the cache that outgrow each other along the sequence and against it, in tiles of 128 rows."""
+    dev, n, H, Hk = cuda_device, 520, 20, 10
+    assert Hk * -(-n * 2 // 16) > 2 * 148
+    for order in (1, -1):
+        g = torch.Generator().manual_seed(window + order)
+        kc, vc, table, ks, vs = paged(g, [n], Hk, dtype)
+        by = torch.linspace(0.05, 30, n).view(n, 1, 1)
+        k = (ks[0].float() * (by if order == 1 else by.flip(0))).to(dtype)
+        W.write_cache(k, vs[0], kc, vc, torch.tensor([int(table[0, t // 16]) * 16 + t % 16 for t in range(n)]))
+        q, i32 = normal(g, dtype, n, H, D), lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        out = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc.to(dev), vc.to(dev), i32([0, n]), i32([n]), table.to(dev), n, n,
+                                                      SCALE, window, sinks).cpu()
+        near(out[::9], q[::9], k, vs[0], range(0, n, 9), window, sinks, dtype)
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", ["decode", "items", "paged tiles", "packed tiles"])
+def test_the_error_is_that_of_its_roundings(cuda_device, form, dtype):
+    """Root mean square over many rows.  A rounding's error is spread evenly over half a step u either way, so its
+    square is u^2 / 3 of the value's on average at most: one for the output, and where a probability is rounded
+    once (the tiles), one for each product p v.  Five per cent for fp32 sums, exp2 and chance."""
+    dev, g, window, sinks, H, Hk = cuda_device, torch.Generator().manual_seed(30), 200, 4, 20, 10
+    lens_q = {"decode": [1] * 60, "items": [10] * 12, "paged tiles": [520], "packed tiles": [520]}[form]
+    lens_k = [lq + 190 + 7 * i for i, lq in enumerate(lens_q)]
+    if form == "decode":
+        kc, vc, table, ks, vs = paged(g, lens_k, Hk, dtype)
+        q = normal(g, dtype, 60, H, D)
+        out = decode(dev, q, kc, vc, table, lens_k, window, sinks)
+    else:
+        out, q, ks, vs = run_prefill(dev, g, lens_q, lens_k, H, Hk, window, sinks, dtype, form != "packed tiles")
+    step, at, err, size, parts, count = torch.finfo(dtype).eps / 2, 0, 0.0, 0.0, 0.0, 0
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        for r in range(0, lq, 1 if lq < 20 else 7):
+            seen = W.visible(lk - lq + r, window, sinks)
+            kk, vv = ks[i][seen].double(), vs[i][seen].double()
+            p = torch.softmax(torch.einsum("hgd,thd->hgt", q[at + r].double().view(Hk, H // Hk, D), kk) * SCALE, -1)
+            o = torch.einsum("hgt,thd->hgd", p, vv).reshape(H, D)
+            err += float((out[at + r].double() - o).square().sum())
+            size += float(o.square().sum())
+            parts += float(torch.einsum("hgt,thd->hgd", p.square(), vv.square()).sum())
+            count += o.numel()
+        at += lq
+    assert count >= 60 * H * D
+    bound = step / math.sqrt(3) * math.sqrt(size + (parts if "tiles" in form else 0.0)) * 1.05
+    assert math.sqrt(err) <= bound, math.sqrt(err) / bound
