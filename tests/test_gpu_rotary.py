@@ -248,3 +248,31 @@ def test_alone_in_f16(cuda_device, T, H, Hk, D, rot, neox, table):
     close(q.reshape(T, H, D), *W.rotate(wide[:, :H * D].view(T, H, D), cs[pos], neox), dtype)
     close(k.reshape(T, Hk, D), *W.rotate(wide[:, H * D:(H + Hk) * D].reshape(T, Hk, D), cs[pos], neox), dtype)
     assert torch.equal(x[:, (H + Hk) * D:].cpu(), wide[:, (H + Hk) * D:]) and _lib.last_status() == 0
+
+
+def test_rows_past_32_bits(cuda_device):
+    """Slices of rows so wide that the last tokens lie more than 2^31 elements behind the first."""
+    dev, dtype, H, Hk, D, width, T = cuda_device, torch.float16, 3, 2, 128, 150, 120000
+    assert (T - 1000) * width * D > 1 << 31
+    wide = torch.zeros(T, width * D, dtype=dtype, device=dev)
+    wide[:, -7 * D:] = torch.randn(T, 7 * D, device=dev, generator=torch.Generator(dev).manual_seed(9)).to(dtype)
+    was = wide[:, -7 * D:].clone()
+    cs = W.cos_sin(range(900), D, 1e4, "none", 1.0, 0).to(torch.float32).to(dev)
+    pos = torch.arange(T, device=dev) % 900
+    kc = torch.zeros(T // 16, Hk, D // 8, 16, 8, dtype=dtype, device=dev)
+    vc = torch.zeros(T // 16, Hk, D, 16, dtype=dtype, device=dev)
+    cut = lambda x: (x[:, :H * D], x[:, H * D:(H + Hk) * D], x[:, (H + Hk) * D:])  # noqa: E731
+    q, k, v = cut(wide[:, -7 * D:])
+    tch_cuda.rotary_embedding_and_cache(pos, q, k, v, D, cs, True, kc, vc, torch.arange(T, device=dev))
+    at = torch.tensor([0, 1, 60000, T - 33, T - 17, T - 2, T - 1], device=dev)
+    for got, old, h in ((q, cut(was)[0], H), (k, cut(was)[1], Hk)):
+        want, mag = W.rotate(old[at].reshape(-1, h, D), cs[pos[at]], True)
+        close(got[at].reshape(-1, h, D), want.cpu(), mag.cpu(), dtype)
+    assert torch.equal(v, cut(was)[2]) and not wide[:, :-7 * D].any()
+    assert torch.equal(kc.permute(0, 3, 1, 2, 4).reshape(T, Hk * D), k) and torch.equal(vc.permute(0, 3, 1, 2).reshape(T, Hk * D), v)
+    b = wide.clone()
+    tch_cuda.rotary_embedding(pos, *cut(b[:, -7 * D:])[:2], D, cs, True)
+    for got, old, h in ((cut(b[:, -7 * D:])[0], q, H), (cut(b[:, -7 * D:])[1], k, Hk)):
+        want, mag = W.rotate(old[at].reshape(-1, h, D), cs[pos[at]], True)
+        close(got[at].reshape(-1, h, D), want.cpu(), mag.cpu(), dtype)
+    assert _lib.last_status() == 0

@@ -179,3 +179,18 @@ def test_a_bad_id_of_the_free_list_stays_bad(cuda_device):
     res, bt = call(dev, *args)
     check(res, bt, W.step_tables(*args))
     assert res.slot_mapping[0].item() == -1 and _lib.last_status() == 1
+
+
+def test_most_requests_in_place(cuda_device):
+    """The largest call in its own buffers: one cluster of CTAs with all of their shared memory."""
+    dev = cuda_device
+    d = lambda x: torch.tensor(x, dtype=I32, device=dev)  # noqa: E731
+    e = lambda k, t=I32: torch.empty(k, dtype=t, device=dev)  # noqa: E731
+    news, ctx, tables, free, count, T, num_blocks = make(32, 16384, 5, 40)
+    want = W.step_tables(news, ctx, tables, free, count, T, num_blocks)
+    for _ in range(5):
+        ctx_d, count_d, bt = d(ctx), d([count]), d(tables)
+        out = batch_info.StepTables(e(16385), e(T, torch.int64), e(T), e(16384), ctx_d, count_d)
+        batch_info.step_tables(d(news), ctx_d, bt, d(free), count_d, num_blocks, T, out=out)
+        check(out, bt, want)
+    assert _lib.last_status() == 0

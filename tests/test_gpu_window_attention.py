@@ -789,3 +789,78 @@ def test_the_error_is_that_of_its_roundings(cuda_device, form, dtype):
     assert count >= 60 * H * D
     bound = step / math.sqrt(3) * math.sqrt(size + (parts if "tiles" in form else 0.0)) * 1.05
     assert math.sqrt(err) <= bound, math.sqrt(err) / bound
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_tiles_cache_offsets_past_32_bits(cuda_device, dtype):
+    """Tiles of 128 rows over the last blocks of a pool of more than 2^31 elements."""
+    dev, H, Hk, n = cuda_device, 16, 8, 330
+    assert Hk * -(-n * 2 // 16) > 2 * 148
+    nblk = (1 << 31) // (Hk * D * 16) + 64
+    kc = torch.empty(nblk, Hk, D // 8, 16, 8, dtype=dtype, device=dev)
+    vc = torch.empty(nblk, Hk, D, 16, dtype=dtype, device=dev)
+    g = torch.Generator().manual_seed(19)
+    k, v, q = normal(g, dtype, n, Hk, D), normal(g, dtype, n, Hk, D), normal(g, dtype, n, H, D)
+    row = torch.arange(nblk - 21, nblk, dtype=torch.int32)
+    small_k, small_v = torch.zeros(21, Hk, 16, 16, 8, dtype=dtype), torch.zeros(21, Hk, D, 16, dtype=dtype)
+    W.write_cache(k, v, small_k, small_v, torch.arange(n))
+    kc[-21:], vc[-21:] = small_k.to(dev), small_v.to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = tch_cuda.flash_attn_varlen_paged_window(q.to(dev), kc, vc, i32([0, n]), i32([n]), row.view(1, -1).to(dev), n, n, SCALE,
+                                                  90, 2).cpu()
+    near(out[::5], q[::5], k, v, range(0, n, 5), 90, 2, dtype)
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("lens_q", [[60000, 60000], [130, 119300, 570]], ids=["even", "ragged"])
+def test_prefill_rows_past_32_bits(cuda_device, lens_q):
+    """Queries, keys and values as slices of rows so wide that the last tokens lie more than 2^31 elements behind the first."""
+    dev, dtype, H, Hk, width, window, sinks = cuda_device, torch.bfloat16, 2, 1, 150, 20, 1
+    total = sum(lens_q)
+    assert (total - 1000) * width * D > 1 << 31
+    wide = torch.zeros(total, width, D, dtype=dtype, device=dev)
+    wide[:, -4:] = torch.randn(total, 4, D, device=dev, generator=torch.Generator(dev).manual_seed(20)).to(dtype)
+    q, k, v = wide[:, -4:-2], wide[:, -2:-1], wide[:, -1:]
+    cu = torch.tensor([sum(lens_q[:i]) for i in range(len(lens_q) + 1)], dtype=torch.int32, device=dev)
+    out = tch_cuda.flash_attn_varlen_window(q, k, v, cu, cu, max(lens_q), max(lens_q), SCALE, window, sinks).cpu()
+    q, k, v, at = q.cpu(), k.cpu(), v.cpu(), 0
+    for n in lens_q:
+        rows = [0, 1, n // 2, n - 130, n - 2, n - 1]
+        for r in rows:  # the definition sees the sinks and the last tokens only
+            seen = W.visible(r, window, sinks)
+            near(out[at + r:at + r + 1], q[at + r:at + r + 1], k[at:at + n][seen], v[at:at + n][seen], [len(seen) - 1], 1 << 30, 0, dtype)
+        at += n
+    assert _lib.last_status() == 0
+
+
+def test_calls_from_several_threads_on_one_stream(cuda_device):
+    """Mixed steps, whose two launches may then lie apart on the stream, and decode calls between them."""
+    import threading
+    dev, dtype, H, Hk = cuda_device, torch.bfloat16, 8, 2
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    jobs = []
+    for s in range(4):
+        g = torch.Generator().manual_seed(40 + s)
+        lens_q = [1] * 40 + [500 + s]
+        lens_k = [700 + 13 * s + i for i in range(40)] + [600]
+        kc, vc, table, _, _ = (x.to(dev) if torch.is_tensor(x) else x for x in paged(g, lens_k, Hk, dtype))
+        q, cu, ctx = normal(g, dtype, 540 + s, H, D).to(dev), i32(list(range(41)) + [540 + s]), i32(lens_k)
+        def mixed(q=q, kc=kc, vc=vc, cu=cu, ctx=ctx, table=table):
+            return tch_cuda.flash_attn_varlen_paged_window(q, kc, vc, cu, ctx, table, 510, 800, SCALE, 300, 4)
+        def single(q=q, kc=kc, vc=vc, ctx=ctx, table=table):
+            out = torch.empty(41, H, D, dtype=dtype, device=dev)
+            tch_cuda.paged_attention_window(out, q[:41], kc, vc, Hk, SCALE, table, ctx, 16, 800, 300, 4)
+            return out
+        jobs.append((mixed, mixed()) if s % 2 == 0 else (lambda a=mixed, b=single: torch.cat([a(), b()]), torch.cat([mixed(), single()])))
+    torch.cuda.synchronize()
+    wrong = []
+    def work(call, want):
+        for _ in range(60):
+            if not torch.equal(call(), want):
+                wrong.append(want.shape)
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and _lib.last_status() == 0
