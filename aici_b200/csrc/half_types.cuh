@@ -18,8 +18,6 @@ struct Half16<__nv_bfloat16> {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
-  __device__ static __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
-  __device__ static __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 
 template <>
@@ -32,8 +30,6 @@ struct Half16<__half> {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
-  __device__ static __forceinline__ __half from(float x) { return __float2half_rn(x); }
-  __device__ static __forceinline__ float to(__half x) { return __half2float(x); }
 };
 
 // Calls f with a value of the type that `dtype` (AICI_DTYPE_BF16 or AICI_DTYPE_F16) names.
