@@ -10,8 +10,12 @@
 namespace aici {
 
 // In the kernel, before its first access to global memory: waits for the grids before this one, then lets the
-// next one start its own prologue.  (Every grid's CTAs do both in this order, so that what is complete for one is
-// complete for all behind it.)
+// next one start its own prologue.  Every grid that is launched as a dependent does both in this order, so that what is
+// complete for one is complete for all behind it.  One grid is an exception: window prefill beside a launch for the
+// short sequences of the same call (window_chunk.cuh) reads its inputs without the wait and lets nobody start early.
+// That is sound only because the launch right before it is not a dependent itself (programmaticStreamSerializationAllowed
+// = 0): it began when all that came before was complete, so whatever starts behind its first CTAs may read the same
+// inputs.  CTA 0 waits before it leaves, so that both are complete for what follows.
 __device__ __forceinline__ void dependent_start() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
