@@ -92,7 +92,8 @@ static void single_rows(const Batch &b) {
     Tensor o = Tensor::empty({1, H, D}, Kind::BFloat16, 0);
     t::paged_attention_window(o, q, b.kc, b.vc, H, 0.01f, bt, ctx, 16, 10, 4);
     expect(rows_are(down(o), 0, 1, kTwo), "decode of a single row");
-    expect(rows_are(down(t::flash_attn_varlen_paged_window(q, b.kc, b.vc, cu, ctx, bt, 1, 10, 0.01f, 4)), 0, 1, kTwo), "paged");
+    o = t::flash_attn_varlen_paged_window(q, b.kc, b.vc, cu, ctx, bt, 1, 10, 0.01f, 4);
+    expect(rows_are(down(o), 0, 1, kTwo), "paged");
     expect(rows_are(down(t::flash_attn_varlen_window(q, q, v, cu, cu, 1, 1, 0.01f, 4)), 0, 1, kOne), "packed");
     Tensor table = t::rotary_cos_sin_cache(4, D, 10000.0, Kind::Float, 0);
     Tensor pos = up(std::vector<int64_t>{0}, {1}, Kind::Int64), slot = up(std::vector<int64_t>{5}, {1}, Kind::Int64);

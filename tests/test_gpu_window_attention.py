@@ -864,3 +864,14 @@ def test_calls_from_several_threads_on_one_stream(cuda_device):
     for t in threads:
         t.join()
     assert not wrong and _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hk", [(17, 1), (48, 1), (96, 2)])
+def test_single_tokens_of_larger_groups(cuda_device, H, Hk, dtype):
+    """More than 16 query heads to a kv head, which the decode call refuses: the paged prefill with one token a sequence."""
+    g, lens = torch.Generator().manual_seed(H), [1, 700, 16, 129]
+    out, q, ks, vs = run_prefill(cuda_device, g, [1] * 4, lens, H, Hk, 100, 5, dtype, True)
+    for i, n in enumerate(lens):
+        near(out[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 100, 5, dtype, split=True)
+    assert _lib.last_status() == 0
