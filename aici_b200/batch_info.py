@@ -236,6 +236,7 @@ def step_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tabl
                 raise AiciError("%s: out does not match the call (device, types or sizes)" % fn)
     _call(fn, "aici_step_tables", index, query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
           free_blocks.data_ptr(), free_count.data_ptr(), n, table[1], rows[0] if n > 1 else table[1],
-          free_blocks.numel(), num_blocks, block_size, max_tokens, out.seqlens_q.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(),
-          out.logit_idxs.data_ptr(), out.context_lens.data_ptr(), out.free_count.data_ptr())
+          free_blocks.numel(), num_blocks, block_size, max_tokens, out.seqlens_q.data_ptr(),
+          out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.logit_idxs.data_ptr(),
+          out.context_lens.data_ptr(), out.free_count.data_ptr())
     return out

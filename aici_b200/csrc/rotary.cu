@@ -165,7 +165,8 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 3 : 2) rotary_cache
   const int tiles = (p.num_tokens + kRotTok - 1) / kRotTok;
   const int groups = (p.num_kv_heads + p.kv_heads_per_cta - 1) / p.kv_heads_per_cta;
   if (blockIdx.x >= (unsigned)(tiles * groups)) {
-    turn_heads<T, C, kNeox>(static_cast<T *>(p.query), p.query_stride, p.num_heads, p.q_plan, blockIdx.x - tiles * groups, p);
+    turn_heads<T, C, kNeox>(static_cast<T *>(p.query), p.query_stride, p.num_heads, p.q_plan,
+                            blockIdx.x - tiles * groups, p);
     return;
   }
   __shared__ int64_t s_slot[kRotTok];
@@ -182,7 +183,8 @@ __global__ void __launch_bounds__(kRotThreads, kUnits == 1 ? 3 : 2) rotary_cache
         const int tok = i / (D / 8), c = i - tok * (D / 8);
         const int64_t from = (int64_t)h * D + c * 8;
         copy_async16(dst + tok * pitch + c * 8, static_cast<const T *>(p.key) + (t0 + tok) * p.key_stride + from);
-        copy_async16(dst + (kRotTok + tok) * pitch + c * 8, static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + from);
+        copy_async16(dst + (kRotTok + tok) * pitch + c * 8,
+                     static_cast<const T *>(p.value) + (t0 + tok) * p.value_stride + from);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -291,9 +293,9 @@ __device__ __forceinline__ void put(float *dst, double x) { *dst = (float)x; }
 __device__ __forceinline__ void put(__nv_bfloat16 *dst, double x) { *dst = __double2bfloat16(x); }
 __device__ __forceinline__ void put(__half *dst, double x) { *dst = __double2half(x); }
 
-// One thread walks kWalk positions of a pair: sine and cosine of the first angle and of one position's
-// turn by the library, the ones between by complex products in 64 bits (each costs a relative 2^-52, so
-// kWalk of them stay far below the 2^-24 of the result).  Computing every angle on its own costs some 100
+// One thread walks p.walk positions of a pair (64, down to 4 where the table is short): sine and cosine of the first
+// angle and of one position's turn by the library, the ones between by complex products in 64 bits (each costs a
+// relative 2^-52, so 64 of them stay far below the 2^-24 of the result).  Computing every angle on its own costs some 100
 // 64-bit operations an entry and takes seven times the store's time.
 template <typename C>
 __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_constant__ TableParams p) {
@@ -321,7 +323,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_table_kernel(const __grid_
 
 // ---- host side -----------------------------------------------------------------------------------------
 static char *check_rotary(const char *fn, const RotaryParams &p, int table_dtype, int dtype, bool cache) {
-  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn, dtype);
+  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn,
+             dtype);
   AICI_CHECK(table_dtype == AICI_DTYPE_F32 || table_dtype == dtype,
              "%s: cos_sin_cache must be f32 or of the query's type (dtype=%d)", fn, table_dtype);
   AICI_CHECK(p.head_size > 0 && p.head_size % 16 == 0 && p.head_size <= kMaxHead,

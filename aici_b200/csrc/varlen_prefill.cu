@@ -34,9 +34,14 @@
 // multiplied (N of the S MMA, K steps of the P V MMAs), so four sinks cost a quarter of a tile.  What bounds
 // long calls is what bounds the kernel without a window, the tensor pipe with its operand reads: 3650 clk for
 // a step of two tiles where the MMAs alone would take 3136 (in-kernel time stamps, 1.75 GHz under load), of
-// which the issuing warp waits 590.  2 x 32768 tokens, 64/8 heads, window 4096: 8.6 ms = 957 TFLOP/s of
-// visible pairs; 4 x 4096, 32/8 heads, window 1024: 332 us = 725, window 128: 170 us = 205, where a CTA's
-// fixed cost (fill 4300 clk, epilogue 2700) and the diagonal's two passes weigh as much as the MMAs.
+// which the issuing warp waits 590.  2 x 32768 tokens, 64/8 heads, window 4096: 8.1 to 8.9 ms = 1020 to 928
+// TFLOP/s of visible pairs; 4 x 4096, 32/8 heads, window 1024: 312 us = 771, window 128: 141 to 150 us = 247 to 232,
+// where a CTA's fixed cost (fill 4300 clk, epilogue 2700) and the diagonal's two passes weigh as much as the MMAs.
+// A probability meets the values rounded to the 16-bit type once, as in the kernel without a window: against 64
+// bits the output is off by 2.0e-3 of its size, and by the 1.4e-3 of its own rounding where probabilities are exact
+// (f16: 2.9e-4 and 2.1e-4).  What the rounding left as a second product, the way of window_decode.cu, would cost a
+// second set of P V MMAs: these alone, without the work on the softmax side, take 2 x 32768 from 8.05 to 9.7-10.1
+// ms, 8 chunks of 512 over the cache from 120 to 134 us and 4 x 4096, window 1024, from 312 to 354.
 // Every barrier wait is bounded; a timeout sets AICI_STATUS_WAIT_TIMEOUT and unwinds.
 #include "dependent.cuh"
 #include "half_types.cuh"
@@ -82,9 +87,12 @@ struct PrefillCfg {
   static constexpr int kCtasPerSm = kTiles == 2 ? 1 : 2;
 };
 constexpr float kRescaleThreshold = 8.f;  // log2 units: the running reference moves once a score exceeds it by this
-constexpr float kRescaleSum = 256.f;      // single-pass tiles: a row sum above this moves the reference (some score is 2^8 above it, or many are above it)
-constexpr float kDangerSumF16 = 3e4f;     // the same for f16 probabilities, whose range ends at 65504
-constexpr float kDangerSum = 1e30f;       // single-pass tiles: a row sum at or above this (or NaN) means the tile is redone exactly
+// Single-pass tiles: a row sum above the first moves the reference (some score is 2^8 above it, or many are above
+// it); at the second or above (or NaN) the tile is redone exactly, for f16 probabilities, whose range ends at
+// 65504, at the third.
+constexpr float kRescaleSum = 256.f;
+constexpr float kDangerSum = 1e30f;
+constexpr float kDangerSumF16 = 3e4f;
 
 struct PrefillParams {
   // output [total_q, heads, 128] (strides below) in `world` buffers -- this GPU's and, for the
@@ -547,8 +555,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
     // ---------------------------------------------------------------- MMA issuer -------------
     constexpr bool kF16 = Half16<T16>::kDtype == AICI_DTYPE_F16;
     constexpr uint32_t idesc_s = kF16 ? idesc_f16(kBM, kBN, false) : idesc_bf16(kPair ? 2 * kBM : kBM, kBN, false);
-    constexpr uint32_t idesc_pv =
-        kF16 ? idesc_f16(kBM, kHD, !kPaged) : idesc_bf16(kPair ? 2 * kBM : kBM, kHD, !kPaged);  // packed V: MN-major; cache V: K-major
+    constexpr uint32_t idesc_pv =  // packed V: MN-major; cache V: K-major
+        kF16 ? idesc_f16(kBM, kHD, !kPaged) : idesc_bf16(kPair ? 2 * kBM : kBM, kHD, !kPaged);
     constexpr int kKPanel = kPair ? kPanelBytes / 2 : kPanelBytes;  // one 64-column panel of a key (half) tile
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -668,7 +676,8 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
         // sinks and its first row's window -- are cleared: their probabilities are 0, but 0 x NaN is
         // NaN, and blocks without a visible token were not loaded at all.
         const int n0 = tile_of(j) * kBN;
-        const int hi = min(kBN, win.lim - n0), dead0 = min(max(win.sinks - n0, 0), kBN), dead1 = min(max(win.lo - n0, 0), kBN);
+        const int hi = min(kBN, win.lim - n0);
+        const int dead0 = min(max(win.sinks - n0, 0), kBN), dead1 = min(max(win.lo - n0, 0), kBN);
         if (hi < kBN || dead0 < dead1) {
           uint8_t *vt = sKV + (i_v % kKvStages) * kStageBytes;
           auto clear = [&](int a, int b) {  // tokens [a, b) of the tile
@@ -680,8 +689,10 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
                   for (int idx = lane; idx < 256; idx += 32) reinterpret_cast<uint4 *>(vb)[idx] = make_uint4(0, 0, 0, 0);
                 } else {
                   for (int tok = t0; tok < t1; ++tok)
-                    for (int d = lane; d < kHD; d += 32)
-                      *reinterpret_cast<uint16_t *>(vb + d * 32 + ((((tok >> 3) ^ ((d >> 2) & 1))) << 4) + (tok & 7) * 2) = 0;
+                    for (int d = lane; d < kHD; d += 32) {
+                      const int at = d * 32 + (((tok >> 3) ^ ((d >> 2) & 1)) << 4) + (tok & 7) * 2;
+                      *reinterpret_cast<uint16_t *>(vb + at) = 0;
+                    }
                 }
               }
             } else {
@@ -1396,10 +1407,11 @@ static char *launch_prefill_shape(const CUtensorMap &tq, const CUtensorMap &tk, 
 // Windowed variant.  A query tile visits window / 128 + 1 key tiles and the sinks' tiles: by that length
 // and not the sequence's a call takes shape 1 or 2; two tiles of a CTA are two heads of one kv head.
 // A paged tile is 16 copies where a packed one is 4, and the one-tile shape's two stages hide less of them, so
-// sharing tiles between two query tiles pays earlier: paged, 4 x 4096, 32/8 heads, window 640: 286 us one-tile
-// and 304 two-tile, 1024: 353 and 365, 1536: 432 and 434, 2048: 495 and 490; 8 chunks of 512 with 8192 cached:
-// 93.6 and 96.6, 122.0 and 121.4, 160.8 and 155.7, 207 and 189.  Packed, 4 x 4096, 2048: 472 and 490, 4096: 585
-// and 572; chunks, 1024: 110 and 119, 2048: 188 and 195, 4096: 326 and 320.
+// sharing tiles between two query tiles pays earlier.  In us one-tile and two-tile, 32/8 heads: paged, 4 x 4096,
+// window 640: 283 and 305, 1024: 348 and 366, 1280: 386 and 403, 1536: 421 and 437, 2048: 501 and 492; 8 chunks of
+// 512 on 7680 cached: 95.6 and 96.8, 122.8 and 122.2, 142 and 139, 162 and 156, 200 and 190.  Packed, 4 x 4096,
+// 2048: 468 and 482, 2560: 525 and 524, 4096: 603 and 578; chunks, 1024: 123 and 124, 2048: 195 and 192, 2560: 230
+// and 223, 4096: 334 and 320.
 template <bool kPaged, typename T16>
 static char *launch_prefill_window(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                                    const OutMaps &to, PrefillParams &p, int num_heads, int batch, int max_seqlen_q,
@@ -1450,7 +1462,8 @@ struct WindowArgs {
 };
 
 static char *check_window(const char *fn, const WindowArgs &w, int num_heads, int num_kv_heads, int dtype) {
-  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn, dtype);
+  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn,
+             dtype);
   AICI_CHECK(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,
              "%s: num_heads %d not divisible by num_kv_heads %d", fn, num_heads, num_kv_heads);
   AICI_CHECK(w.window >= 1, "%s: window must be at least 1 (got %d)", fn, w.window);
@@ -1477,7 +1490,8 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   if (win != nullptr) {
     if (char *e = check_window(fn, *win, num_heads, num_heads_k, dtype)) return e;
   }
-  AICI_CHECK(win != nullptr || dtype == AICI_DTYPE_BF16, "%s: FlashAttention only support bf16 data type (dtype=%d)", fn, dtype);
+  AICI_CHECK(win != nullptr || dtype == AICI_DTYPE_BF16, "%s: FlashAttention only support bf16 data type (dtype=%d)", fn,
+             dtype);
   AICI_CHECK(batch > 0, "%s: batch size must be positive", fn);
   AICI_CHECK(head_size == kHD, "%s: head_size must be 128 (got %d)", fn, head_size);
   AICI_CHECK(num_heads > 0 && num_heads_k > 0 && num_heads % num_heads_k == 0,
@@ -1520,7 +1534,9 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   const void *vv = total_k > 0 ? v : q;
   const int64_t tk_rows = total_k > 0 ? total_k : 1;
   // the CTA-pair shape loads key tiles in halves of 64 tokens
-  if (char *e = make_tmap(fn, &tk, kk, tk_rows, num_heads_k, k_tok_stride, k_head_stride, win == nullptr, shape == 3 ? 64 : kBM)) return e;
+  if (char *e = make_tmap(fn, &tk, kk, tk_rows, num_heads_k, k_tok_stride, k_head_stride, win == nullptr,
+                          shape == 3 ? 64 : kBM))
+    return e;
   if (char *e = make_tmap(fn, &tv, vv, tk_rows, num_heads_k, v_tok_stride, v_head_stride, win == nullptr)) return e;
 
   PrefillParams p;
@@ -1550,7 +1566,8 @@ static char *mha_varlen_fwd_impl(const char *fn, void *const *outs, int world, i
   p.total_q = total_q;
   p.tma_store = 1;
   for (int w = 0; w < world; ++w)  // the kernel reads m[w] for w < world only
-    if (char *e = make_tmap(fn, &to.m[w], outs[w], total_q, out_head0 + num_heads, o_tok_stride, o_head_stride, win == nullptr))
+    if (char *e = make_tmap(fn, &to.m[w], outs[w], total_q, out_head0 + num_heads, o_tok_stride, o_head_stride,
+                            win == nullptr))
       return e;
   if (win != nullptr)
     return with_half_type(dtype, [&](auto t) {
@@ -1671,10 +1688,10 @@ static char *mha_varlen_paged_fwd_impl(const char *fn, void *out, const void *q,
   const bool all_short = win != nullptr && window_chunk_takes(batch, num_heads, num_kv_heads, max_seqlen_q);
   const bool some_short = win != nullptr && !all_short && window_chunk_mixed(batch, total_q, max_seqlen_q);
   if (all_short || some_short) {
-    const WindowChunk c = {out, q, key_cache, value_cache, cu_seqlens_q, context_lens, block_tables, batch, total_q, num_heads,
-                           num_kv_heads, all_short ? max_seqlen_q : kWindowChunkTokens, max_context_len, max_num_blocks_per_seq, win->window, win->sinks,
-                           num_blocks, q_tok_stride, q_head_stride, o_tok_stride, o_head_stride, kv_block_stride,
-                           softmax_scale, st, !all_short};
+    const WindowChunk c = {out, q, key_cache, value_cache, cu_seqlens_q, context_lens, block_tables, batch, total_q,
+                           num_heads, num_kv_heads, all_short ? max_seqlen_q : kWindowChunkTokens, max_context_len,
+                           max_num_blocks_per_seq, win->window, win->sinks, num_blocks, q_tok_stride, q_head_stride,
+                           o_tok_stride, o_head_stride, kv_block_stride, softmax_scale, st, !all_short};
     char *e = launch_window_chunk(c, dtype, static_cast<cudaStream_t>(stream));
     if (e != nullptr || all_short) return e;
   }

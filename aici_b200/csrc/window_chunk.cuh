@@ -13,10 +13,10 @@ constexpr int kWindowChunkTokens = 16;
 
 // Whether a call takes this form: chunks of at most 16 tokens, where an item does at least the work of a
 // query head (64 sequences at context 8192, window 4096, us here and in the general kernel's 128-row tiles:
-// 32 heads over 8, 4 tokens 166 and 807, 16 tokens 490 and 800, 32 tokens 973 and 630; 8 heads over 8, 16
-// tokens 167 and 238, 32 tokens 280 and 217), or all items resident at once, two to an SM, since an item's
+// 32 heads over 8, 4 tokens 165 and 805, 16 tokens 492 and 799, 32 tokens 975 and 632; 8 heads over 8, 16
+// tokens 166 and 239, 32 tokens 282 and 205), or all items resident at once, two to an SM, since an item's
 // keys are then dealt out to a cluster while a tile of the general kernel walks them alone (1 sequence, 32
-// heads over 8, window 4096: 4 tokens 14 and 115, 64 tokens 41 and 85, 128 tokens = 256 items 71 and 81,
+// heads over 8, window 4096: 4 tokens 14 and 115, 64 tokens 41 and 84, 128 tokens = 256 items 71 and 80,
 // 256 tokens = 512 items 140 and 81).
 inline bool window_chunk_takes(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t max_tokens) {
   const int64_t items = batch * num_kv_heads * window_chunk_items(max_tokens, num_heads / num_kv_heads);
@@ -26,9 +26,9 @@ inline bool window_chunk_takes(int64_t batch, int64_t num_heads, int64_t num_kv_
 // Whether, in a call that does not, the sequences of at most kWindowChunkTokens tokens get a launch of this
 // form beside the general kernel's (a step of single tokens and some chunks).  The host knows no lengths: it
 // does so where the mean is below half the longest, or no other sum is possible.  In us, with and without, at
-// 32 heads over 8: 63 single tokens and a chunk of 512, context 6000: 44 and 141 (window 128), 240 and 886
-// (4096); 3 and a chunk: 20 and 30, 89 and 119; 4 chunks of 64 to 512, for which there is nothing to gain: 21
-// and 33 (its tiles are also found by batch_tile), 94 and 93.
+// 32 heads over 8, context 6000, windows 128 and 4096: 63 single tokens and a chunk of 512: 46 and 107, 238 and
+// 877; 15 and a chunk: 22 and 40, 96 and 310; 3 and a chunk: 19.6 and 17.4, 90 and 116; 4 chunks of 64 to 512, for
+// which there is nothing to gain: 21.1 and 18.3, 92 and 90.
 inline bool window_chunk_mixed(int64_t batch, int64_t total_q, int64_t max_tokens) {
   return 2 * total_q < batch * max_tokens || total_q < (kWindowChunkTokens + 1) * (batch - 1) + max_tokens;
 }

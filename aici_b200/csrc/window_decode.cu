@@ -23,9 +23,9 @@
 // kv heads of a sequence, started next to each other, read neighbouring 4 KB pieces of the same blocks:
 // 1024 rows of 257 tiles took 311 us (6.9 TB/s), against 340 us when all tiles of the batch are cut into
 // equal runs for resident warps and a second kernel joins the cut rows (256 rows: 88 against 94 us; 8 rows,
-// cluster of 8: 9.8 against 24 us); with probabilities in two parts, as they are now, 316, 89 and 10.3 us.  What that other form is better at is a batch with one row far longer
-// than the rest: a CTA alone streams a tile in 0.19 us, so the last row to start costs at most that
-// times its tiles.
+// cluster of 8: 9.8 against 24 us); with probabilities in two parts, as they are now, 316, 89 and 10.3 us.  What
+// that other form is better at is a batch with one row far longer than the rest: a CTA alone streams a tile in 0.19
+// us, so the last row to start costs at most that times its tiles.
 #include "dependent.cuh"
 #include "half_types.cuh"
 #include "window_chunk.cuh"
@@ -37,7 +37,8 @@ constexpr int kWinBlock = 16;
 constexpr int kWinTileBytes = kWinHead * kWinBlock * 2;
 constexpr int kWinStageBytes = 2 * kWinTileBytes;  // key tile and value tile
 constexpr int kWinWarps = 4;
-constexpr int kWinStages = 3;  // 72 KB of ring in flight per SM and CTA pair: enough for the bandwidth-latency product
+// 96 KB of ring a CTA, 192 KB an SM with two of them, and as one stage of three is being worked on, 128 KB in flight
+constexpr int kWinStages = 3;
 constexpr int kWinThreads = kWinWarps * 32;
 constexpr int kWinRingBytes = kWinWarps * kWinStages * kWinStageBytes;
 constexpr int kWinBarBytes = 128;  // kWinWarps * kWinStages barriers
@@ -118,7 +119,8 @@ struct GroupState {
 
   // q0: the sequence's first query row of the tensor, pos0: its position; the item has the rows row0 ..
   // row0 + rows - 1 of the kv head's
-  __device__ __forceinline__ void load(const WindowDecodeParams &p, int q0, int pos0, int row0, int rows, int kvh, int g, int tig) {
+  __device__ __forceinline__ void load(const WindowDecodeParams &p, int q0, int pos0, int row0, int rows, int kvh, int g,
+                                       int tig) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int i = row0 + g + 8 * r, token = kChunk ? i / p.group : 0, head = i - token * p.group;
@@ -271,7 +273,10 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t cta) {
   uint32_t remote;
   float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(cta));
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ float2 ld_cluster2(uint32_t local, uint32_t cta) {
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
   }
   const WindowRow row = window_row(p, ctx, tokens, back);
   const int stride = ctas * kWinWarps, first = rank * kWinWarps + warp;
-  const int mine = rows > 0 && row.tiles > first ? (row.tiles - first + stride - 1) / stride : 0;  // tiles first, first + stride, ...
+  // tiles first, first + stride, ...
+  const int mine = rows > 0 && row.tiles > first ? (row.tiles - first + stride - 1) / stride : 0;
   GroupState<T, kTwo, kChunk> st;
   st.load(p, q0, row.ctx + back - all_tokens, row0, rows, kvh, g, tig);
   int ids = 0;
@@ -405,7 +411,8 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
     }
     if (ctas == 1) {
       const float inv = inverse(l);
-      *reinterpret_cast<uint2 *>(out(h) + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
+      *reinterpret_cast<uint2 *>(out(h) + d) =
+          make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
     } else {
       *reinterpret_cast<float4 *>(s_o + h * kWinHead + d) = a;
       if ((i & 31) == 0) s_ml[h] = make_float2(m, l);
@@ -440,7 +447,8 @@ __global__ void __launch_bounds__(kWinThreads, 2) window_decode_kernel(const Win
         a.x += f * v[c].x; a.y += f * v[c].y; a.z += f * v[c].z; a.w += f * v[c].w;
       }
     const float inv = inverse(l);
-    *reinterpret_cast<uint2 *>(out(h) + d) = make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
+    *reinterpret_cast<uint2 *>(out(h) + d) =
+        make_uint2(Half16<T>::pack(a.x * inv, a.y * inv), Half16<T>::pack(a.z * inv, a.w * inv));
   }
   // nobody leaves while its shared memory may still be read
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -469,7 +477,8 @@ static char *launch_window_decode(const WindowDecodeParams &p, int ctas, cudaStr
   constexpr int kSmem = kWinRingBytes + kWinBarBytes + (kTwo ? 16 : 8) * (kWinHead * 4 + 8 + kWinWarps * 8);
   static OncePerDevice once;
   if (char *e = once.run([]() -> char * {
-        AICI_CUDA(cudaFuncSetAttribute(window_decode_kernel<T, kTwo, kChunk>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        AICI_CUDA(cudaFuncSetAttribute(window_decode_kernel<T, kTwo, kChunk>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         return nullptr;
       }))
     return e;
@@ -541,7 +550,8 @@ extern "C" char *aici_paged_attention_window(void *out, const void *query, const
                                              int64_t num_blocks, int64_t q_stride, int64_t kv_block_stride,
                                              int64_t kv_head_stride, int dtype, aici_stream_t stream) {
   const char *fn = "aici_paged_attention_window";
-  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn, dtype);
+  AICI_CHECK(dtype == AICI_DTYPE_BF16 || dtype == AICI_DTYPE_F16, "%s: only bf16 and f16 are supported (dtype=%d)", fn,
+             dtype);
   AICI_CHECK(head_size == kWinHead, "%s: head_size must be 128 (got %d)", fn, head_size);
   AICI_CHECK(block_size == kWinBlock, "%s: block_size must be 16 (got %d)", fn, block_size);
   AICI_CHECK(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,

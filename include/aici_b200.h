@@ -503,13 +503,15 @@ char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, voi
  * The query at position p of its sequence sees the tokens t <= p with t > p - window or t < sinks
  * (window >= 1, sinks >= 0; a window that covers the context gives causal attention).  bf16 or f16,
  * head_size 128, block_size 16; fp32 scores and sums.  Probabilities meet the values in the 16-bit type:
- * prefill rounds them, decode and short paged chunks add what the rounding left as a second product.  A
+ * prefill rounds them (its error is then about 1.4 times that of the output's own rounding), decode and
+ * paged chunks of at most 16 tokens, or of few in all, add what the rounding left as a second product.  A
  * row that sees nothing is zero.  The strides of a single query row, key row or head may be anything.
  *
  * Decode over the paged cache, arguments as in aici_paged_attention_v1: one query per sequence at
- * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number.  Blocks that hold no
- * visible token are not read (their table entries may be anything), and tokens that are not visible
- * may hold anything, NaN included.  No workspace. */
+ * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number (a call of
+ * aici_mha_varlen_paged_window_fwd with one token a sequence takes more).  Blocks that hold no visible
+ * token are not read (their table entries may be anything), and tokens that are not visible may hold
+ * anything, NaN included.  No workspace. */
 char *aici_paged_attention_window(void *out, const void *query, const void *key_cache,
                                   const void *value_cache, int num_kv_heads, float scale,
                                   const int32_t *block_tables, const int32_t *context_lens, int block_size,
@@ -521,11 +523,11 @@ char *aici_paged_attention_window(void *out, const void *query, const void *key_
 /* Prefill over packed keys and values (arguments as in aici_mha_varlen_fwd) and over the paged cache
  * (as in aici_mha_varlen_paged_fwd); row r of a sequence is the token at position len_k - len_q + r, any
  * number of query heads per kv head.  Over the paged cache a step may mix single tokens and chunks: sequences
- * of at most 16 tokens are worked on beside the others in a second launch.  Tokens that none of the 128 rows of a query tile (rows
- * 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token that one of
- * them sees are not read.  The rows of a sequence with more than max_seqlen_q tokens are zero and the status
- * says AICI_STATUS_BAD_BLOCK, as it does for running sums outside 0 .. total_q, whose rows outside the tensor are
- * left out; max_seqlen_q = 0 says that there are no query tokens, and nothing is written. */
+ * of at most 16 tokens are worked on beside the others in a second launch.  Tokens that none of the 128 rows
+ * of a query tile (rows 128 i .. 128 i + 127 of a sequence) sees may hold anything, and blocks without a token
+ * that one of them sees are not read.  The rows of a sequence with more than max_seqlen_q tokens are zero and
+ * the status says AICI_STATUS_BAD_BLOCK, as it does for running sums outside 0 .. total_q, whose rows outside
+ * the tensor are left out; max_seqlen_q = 0 says that there are no query tokens, and nothing is written. */
 char *aici_mha_varlen_window_fwd(void *out, const void *q, const void *k, const void *v,
                                  const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
                                  int total_q, int total_k, int num_heads, int num_heads_k, int head_size,

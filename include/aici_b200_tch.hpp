@@ -556,7 +556,8 @@ inline void rotary_embedding_reshape_and_cache(const Tensor &positions, Tensor &
 namespace detail {
 // Heads per token of [num_tokens, heads * head_size] or [num_tokens, heads, head_size].
 inline int head_rows(const char *fn, const Tensor &t, int head_size) {
-  if (t.dim() == 2 && t.size(1) % head_size == 0 && (t.stride(1) == 1 || t.size(1) == 1)) return (int)(t.size(1) / head_size);
+  if (t.dim() == 2 && t.size(1) % head_size == 0 && (t.stride(1) == 1 || t.size(1) == 1))
+    return (int)(t.size(1) / head_size);
   if (t.dim() == 3 && t.size(2) == head_size && t.stride(2) == 1 && (t.stride(1) == head_size || t.size(1) == 1))
     return (int)t.size(1);
   throw Error(std::string(fn) + ": query, key and value must be [num_tokens, heads * head_size] or [num_tokens, heads, "
@@ -568,7 +569,8 @@ inline void rotary_args(const char *fn, const Tensor &positions, const Tensor &q
   require(fn, positions.kind == Kind::Int64 && positions.is_contiguous() && positions.numel() == query.size(0) &&
                   query.size(0) == key.size(0),
           "positions must be contiguous int64 with one entry per token of query and key");
-  require(fn, cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous(), "cos_sin_cache must be contiguous [max_position, rot_dim]");
+  require(fn, cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous(),
+          "cos_sin_cache must be contiguous [max_position, rot_dim]");
   require(fn, query.kind == key.kind, "query and key must have the same dtype");
 }
 }  // namespace detail
@@ -682,8 +684,8 @@ inline Tensor flash_attn_varlen_window(const Tensor &q, const Tensor &k, const T
                 out.data, q.data, k.data, v.data, static_cast<const int32_t *>(seqlens_q.data),
                 static_cast<const int32_t *>(seqlens_k.data), (int)seqlens_q.numel() - 1, (int)q.size(0), (int)k.size(0),
                 (int)q.size(1), (int)k.size(1), (int)q.size(2), detail::at_most_int(max_seqlen_q),
-                detail::at_most_int(max_seqlen_k), window, sinks, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
-                out.stride(1), softmax_scale, detail::dtype_of(fn, q), stream));
+                detail::at_most_int(max_seqlen_k), window, sinks, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                v.stride(0), v.stride(1), out.stride(0), out.stride(1), softmax_scale, detail::dtype_of(fn, q), stream));
   return out;
 }
 
@@ -751,7 +753,8 @@ inline StepTables step_tables(const Tensor &query_lens, const Tensor &context_le
                              block_tables.size(1), (int)free_blocks.numel(), num_blocks, block_size, max_tokens,
                              static_cast<int32_t *>(r.seqlens_q.data), static_cast<int64_t *>(r.positions.data),
                              static_cast<int32_t *>(r.slot_mapping.data), static_cast<int32_t *>(r.logit_idxs.data),
-                             static_cast<int32_t *>(r.context_lens.data), static_cast<int32_t *>(r.free_count.data), stream));
+                             static_cast<int32_t *>(r.context_lens.data), static_cast<int32_t *>(r.free_count.data),
+                             stream));
   return r;
 }
 
