@@ -23,7 +23,7 @@
 // kv heads of a sequence, started next to each other, read neighbouring 4 KB pieces of the same blocks:
 // 1024 rows of 257 tiles took 311 us (6.9 TB/s), against 340 us when all tiles of the batch are cut into
 // equal runs for resident warps and a second kernel joins the cut rows (256 rows: 88 against 94 us; 8 rows,
-// cluster of 8: 9.8 against 24 us); with probabilities in two parts, as they are now, 316, 89 and 10.3 us.  What
+// cluster of 8: 9.8 against 24 us); with probabilities in two parts, as they are now, 314, 87 and 9.8 us.  What
 // that other form is better at is a batch with one row far longer than the rest: a CTA alone streams a tile in 0.19
 // us, so the last row to start costs at most that times its tiles.
 #include "dependent.cuh"
