@@ -511,7 +511,7 @@ char *aici_rotary_embedding_and_cache(const int64_t *positions, void *query, voi
  * position context_lens[i] - 1.  Up to 16 query heads per kv head, any number (a call of
  * aici_mha_varlen_paged_window_fwd with one token a sequence takes more).  Blocks that hold no visible
  * token are not read (their table entries may be anything), and tokens that are not visible may hold
- * anything, NaN included.  No workspace. */
+ * anything, NaN included.  `out` may be the query's own buffer.  No workspace. */
 char *aici_paged_attention_window(void *out, const void *query, const void *key_cache,
                                   const void *value_cache, int num_kv_heads, float scale,
                                   const int32_t *block_tables, const int32_t *context_lens, int block_size,

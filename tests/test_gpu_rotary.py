@@ -276,3 +276,17 @@ def test_rows_past_32_bits(cuda_device):
         want, mag = W.rotate(old[at].reshape(-1, h, D), cs[pos[at]], True)
         close(got[at].reshape(-1, h, D), want.cpu(), mag.cpu(), dtype)
     assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("T,H,Hk,D,rot,neox", [(5, 80, 1, 256, 256, True), (3, 130, 2, 256, 240, False), (9, 300, 3, 128, 128, True)])
+def test_more_heads_than_threads_take_at_once(cuda_device, T, H, Hk, D, rot, neox):
+    """Heads beyond four for every slot of a CTA: a thread goes over its token's heads more than once."""
+    assert H > 4 * (256 // (rot // 16))
+    dev, dtype = cuda_device, torch.bfloat16
+    wide, cs, pos, _, _, _ = inputs(T + H, T, H, Hk, D, rot, dtype, torch.float32)
+    x = wide.to(dev)
+    q, k = x[:, :H * D], x[:, H * D:(H + Hk) * D]
+    tch_cuda.rotary_embedding(pos.to(dev), q, k, D, cs.to(dev), neox)
+    close(q.reshape(T, H, D), *W.rotate(wide[:, :H * D].view(T, H, D), cs[pos], neox), dtype)
+    close(k.reshape(T, Hk, D), *W.rotate(wide[:, H * D:(H + Hk) * D].reshape(T, Hk, D), cs[pos], neox), dtype)
+    assert _lib.last_status() == 0

@@ -875,3 +875,73 @@ def test_single_tokens_of_larger_groups(cuda_device, H, Hk, dtype):
     for i, n in enumerate(lens):
         near(out[i:i + 1], q[i:i + 1], ks[i], vs[i], [n - 1], 100, 5, dtype, split=True)
     assert _lib.last_status() == 0
+
+
+FORMS = [(False, [40, 90], 4, 2), (False, [140] + [3] * 12 + [90], 4, 2), (True, [3, 0, 12], 4, 2), (True, [40, 90], 32, 32),
+         (True, [1] * 20 + [300, 90], 16, 4)]  # paged, query lengths, heads, kv heads: each form of a call
+
+
+def batch(g, dev, dtype, is_paged, lens_q, H, Hk, extra):
+    """Queries with `extra` rows behind the last sequence, keys and values on the device, and the tokens."""
+    lens_k = [lq + 11 for lq in lens_q]
+    q = normal(g, dtype, sum(lens_q) + extra, H, D)
+    if is_paged:
+        kc, vc, table, ks, vs = paged(g, lens_k, Hk, dtype)
+        return lens_k, q, (kc.to(dev), vc.to(dev)), table.to(dev), ks, vs
+    ks, vs = ([normal(g, dtype, n, Hk, D) for n in lens_k] for _ in range(2))
+    return lens_k, q, (torch.cat(ks).to(dev), torch.cat(vs).to(dev)), None, ks, vs
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("is_paged,lens_q,H,Hk", FORMS)
+def test_padding_rows_stay_and_do_no_harm(cuda_device, is_paged, lens_q, H, Hk, dtype):
+    """A batch padded for a captured step: NaN in the query rows that no sequence owns, whose output rows stay."""
+    dev, g, total = cuda_device, torch.Generator().manual_seed(sum(lens_q)), sum(lens_q)
+    lens_k, q, kv, table, ks, vs = batch(g, dev, dtype, is_paged, lens_q, H, Hk, 77)
+    q[total:] = NAN
+    out = torch.full_like(q, 7.0).to(dev)
+    into(out, dev, q.to(dev), kv, lens_q, lens_k, max(lens_q), 50, 2, table)
+    out, at = out.cpu(), 0
+    assert (out[total:] == 7).all()
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        near(out[at:at + lq], q[at:at + lq], ks[i], vs[i], range(lk - lq, lk), 50, 2, dtype)
+        at += lq
+    assert _lib.last_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("is_paged,lens_q,H,Hk", FORMS)
+def test_a_query_row_of_nan_stays_alone(cuda_device, is_paged, lens_q, H, Hk, dtype):
+    dev, g = cuda_device, torch.Generator().manual_seed(sum(lens_q) + 1)
+    lens_k, q, kv, table, ks, vs = batch(g, dev, dtype, is_paged, lens_q, H, Hk, 0)
+    bad = [(1, 0), (sum(lens_q) - 4, H - 1), (sum(lens_q) // 2, 1)]
+    for row, head in bad:
+        q[row, head, 5] = NAN
+    out = torch.full_like(q, 7.0).to(dev)
+    into(out, dev, q.to(dev), kv, lens_q, lens_k, max(lens_q), 50, 2, table)
+    out, at = out.cpu(), 0
+    for row, head in bad:
+        assert torch.isnan(out[row, head]).all()
+        q[row, head] = 0  # the definition of a row of zeros in its place
+        seq = next(i for i in range(len(lens_q)) if sum(lens_q[:i + 1]) > row)
+        pos = lens_k[seq] - lens_q[seq] + row - sum(lens_q[:seq])
+        out[row, head] = W.attention_row(q[row], ks[seq], vs[seq], pos, 50, 2, SCALE)[0][head].to(dtype)
+    for i, (lq, lk) in enumerate(zip(lens_q, lens_k)):
+        near(out[at:at + lq], q[at:at + lq], ks[i], vs[i], range(lk - lq, lk), 50, 2, dtype)
+        at += lq
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_decode_writes_over_its_queries(cuda_device, dtype):
+    """The output may be the query's own buffer, for rows of one CTA and of a cluster."""
+    for ctx, H, Hk, window in (([900, 20], 16, 2, 800), ([60 + i for i in range(200)], 8, 4, 50), ([3000], 32, 2, 2500)):
+        g = torch.Generator().manual_seed(len(ctx))
+        kc, vc, table, ks, vs = paged(g, ctx, Hk, dtype)
+        q = normal(g, dtype, len(ctx), H, D)
+        want, dev = decode(cuda_device, q, kc, vc, table, ctx, window, 3), cuda_device
+        x, i32 = q.to(dev), torch.tensor(ctx, dtype=torch.int32, device=dev)
+        args = kc.to(dev), vc.to(dev), Hk, SCALE, table.to(dev), i32, 16, max(ctx), window, 3
+        for _ in range(5):
+            x.copy_(q)
+            tch_cuda.paged_attention_window(x, x, *args)
+            assert torch.equal(x.cpu(), want)
