@@ -182,8 +182,8 @@ struct WindowTiles {
 // the others, and real ones behind them: one prompt of 4096 and 63 of 20 tokens, 8/2 heads, window 512: 114
 // and 37 us; 4 prompts of 64 to 512, 32 heads, window 128: 15.1 and 13.4 us; 200 of 1 to 400, 8/2 heads: 135
 // and 139 us.  Where all sequences are as long as the longest the finding alone would cost 0.4 us a CTA.)
-// Sequences and their tiles are counted from the last.  All lanes of a warp take part.  (Clamped sums: with them
-// no more tiles exist than the grid has places, whatever they hold.)
+// Sequences and their tiles are counted from the last.  All lanes of a warp take part.  (Clamped sums, as
+// long as they do not decrease: no more tiles exist than the grid has places.)
 struct BatchTile {
   int b, mb;  // sequence (-1: no tile) and row tile
   int q0, lq, k0, lk;
